@@ -19,13 +19,14 @@ random weights and diffusers' interface to run it on
 """
 
 from .bridge_k import bridge_k_plan
+from .int8 import Int8Rows, int8_linear, quantize_rows
 from .head_parallel import PeerAllGather, all_gather_heads, head_parallel_attention
 from .paired_kernel import RasterOrder, device_status, paired_attention, raster_order, token_order_map
 from .paired_metadata import PairedMetadata, pair_metadata, unpair_metadata
 from .plan import AttentionPlan, PhasePlan, build_plan, full_attention_plan
 from .plan_bank import PlanBank
 from .plan_cache import PlanCache, load_plan, save_plan
-from .prep import norm_rope_pack, prepare_qkv
+from .prep import norm_rope_pack, norm_rope_qk, prepare_qkv
 from .processor import HilbertAProcessor
 from .flux_adapter import persistent_flux_attention
 from .sampling_layout import sample_flux_persistent
@@ -56,6 +57,10 @@ __all__ = [
     "load_plan",
     "prepare_qkv",
     "norm_rope_pack",
+    "norm_rope_qk",
+    "Int8Rows",
+    "quantize_rows",
+    "int8_linear",
     "PeerAllGather",
     "all_gather_heads",
     "head_parallel_attention",

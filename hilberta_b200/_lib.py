@@ -8,6 +8,7 @@ is missing.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 from pathlib import Path
@@ -34,6 +35,7 @@ HB_DEV_PEER_TIMEOUT = 8
 HB_DEV_SMEM_ALIGN = 16
 
 HB_MAX_RANKS = 8
+HB_INT8_MAX_K = 131072
 HB_IPC_HANDLE_BYTES = 64
 
 # Every exported symbol of include/hilberta_b200.h (checked by the CPU tests).
@@ -60,6 +62,11 @@ EXPORTS = (
     "hb_peer_scatter",
     "hb_adaln_residual",
     "hb_expand_kv128",
+    "hb_quantize_rows",
+    "hb_int8_linear",
+    "hb_int8_status",
+    "hb_adaln_residual_int8",
+    "hb_norm_rope_qk",
 )
 
 
@@ -139,6 +146,18 @@ _SIGS = {
         _I,
         [_P, _I64, _P, _I64, _P, _P, _P, _I64, _P, _I64, _P, _I64, _I, _I, _I, ctypes.c_float, _I, _P],
     ),
+    "hb_quantize_rows": (_I, [_P, _I64, _I, _P, _I64, _I, _I, _P, _I64, _P, _I, _P]),
+    "hb_int8_linear": (_I, [_P, _I64, _P, _P, _I64, _P, _P, _P, _I64, _I, _I, _I, _I, _I, _P]),
+    "hb_int8_status": (_I, [_I, ctypes.POINTER(ctypes.c_int32), _P]),
+    "hb_adaln_residual_int8": (
+        _I,
+        [_P, _I64, _P, _I64, _P, _P, _P, _I64, _P, _I64, _P, _I64, _P, _I, _I, _I, ctypes.c_float, _I, _P],
+    ),
+    "hb_norm_rope_qk": (
+        _I,
+        [_P, ctypes.POINTER(ctypes.c_int64), _P, ctypes.POINTER(ctypes.c_int64), _P, ctypes.POINTER(ctypes.c_int64), _P,
+         ctypes.POINTER(ctypes.c_int64), _I, _I, _I, _I, _I, _I, _P, _P, _P, _P, ctypes.c_float, _P, _P, _I, _P],
+    ),
     "hb_paired_fwd_noalloc": (
         _I,
         [_P, _P, _P, _P, ctypes.POINTER(ctypes.c_int64), _I, _I, _I, _I, _I, _I, _I, _P, _P, _P, ctypes.c_float, _I, _P],
@@ -182,6 +201,10 @@ def check(code: int, what: str):
 
 def ptr(t: torch.Tensor | None):
     return None if t is None else ctypes.c_void_p(t.data_ptr())
+
+
+# For ``with``: the current device is the launch's device already.
+SAME_DEVICE = contextlib.nullcontext()
 
 
 def stream_ptr(device) -> ctypes.c_void_p:

@@ -7,6 +7,10 @@ step uses around the attention (``NativeBlockOps``).
 ``gate_residual_adaln(x, y, gate, shift, scale)``
                                         x += gate * y; h = LayerNorm(x) * (1 + scale) + shift
 
+``adaln_int8(x, shift, scale)``, ``gate_residual_adaln_int8(x, y, gate, shift, scale)``
+                                        the same with h quantised per token in the
+                                        pass (``Int8Rows``, the input of ``int8_linear``)
+
 ``x``/``y``: ``[B, S, C]`` (or ``[S, C]``) 16-bit with unit element stride;
 ``shift``/``scale``/``gate``: ``[B, C]`` with unit element stride (chunks of a
 modulation output are fine).  LayerNorm without affine weights.
@@ -17,6 +21,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
+from .int8 import _empty_rows
 
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1}
 
@@ -46,7 +51,8 @@ def _mod(m, B, C, x, name):
     return m, (m.stride(0) if B > 1 else 0)
 
 
-def _call(x, y, gate, shift, scale, x_out, h_out, eps):
+def _call(x, y, gate, shift, scale, x_out, h_out, eps, rows8=None):
+    """One launch; the modulated rows go to ``h_out``, or quantised to ``rows8``."""
     if not x.is_cuda:
         raise ValueError("CUDA tensors required")
     if x.dtype not in _DTYPES:
@@ -67,6 +73,18 @@ def _call(x, y, gate, shift, scale, x_out, h_out, eps):
                 raise ValueError(f"{name} must match x's shape, dtype and device")
             strides[name] = _rows(t, name)[1]
     dev = x.device
+    if rows8 is not None:
+        with torch.cuda.device(dev) if dev.index != torch.cuda.current_device() else _lib.SAME_DEVICE:
+            rc = _lib.lib().hb_adaln_residual_int8(
+                x.data_ptr(), x_rs, None if y is None else y.data_ptr(), strides.get("y", 0),
+                None if gate is None else gate.data_ptr(), shift.data_ptr(), scale.data_ptr(), mod_bs or 0,
+                None if x_out is None else x_out.data_ptr(), strides.get("x_out", 0), rows8.values.data_ptr(),
+                rows8.row_stride, rows8.scales.data_ptr(), B * S, S, C, float(eps), _DTYPES[x.dtype],
+                torch.cuda.current_stream(dev).cuda_stream)
+        if rc == _lib.HB_ERR_UNSUPPORTED:
+            raise NotImplementedError("the channel count must be a multiple of 256 up to 4096")
+        _lib.check(rc, "hb_adaln_residual_int8")
+        return
     with torch.cuda.device(dev):
         rc = _lib.lib().hb_adaln_residual(
             _lib.ptr(x), x_rs, _lib.ptr(y) if y is not None else None, strides.get("y", 0),
@@ -93,6 +111,28 @@ def gate_residual_adaln(x, y, gate, shift, scale, eps=1e-6, out=None):
     h = torch.empty_like(x, memory_format=torch.contiguous_format) if out is None else out
     _call(x, y, gate, shift, scale, x, h, eps)
     return x, h
+
+
+def _check_inference(*tensors):
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise ValueError("Inference only; disable autograd")
+
+
+def adaln_int8(x, shift, scale, eps=1e-6):
+    """``Int8Rows`` of LayerNorm(x) * (1 + scale) + shift, quantised from its fp32 values."""
+    _check_inference(x, shift, scale)
+    rows = _empty_rows(x.shape, x.dtype, x.device)
+    _call(x, None, None, shift, scale, None, None, eps, rows)
+    return rows
+
+
+def gate_residual_adaln_int8(x, y, gate, shift, scale, eps=1e-6, x_out=None):
+    """(x, rows): x += gate * y (into ``x_out`` if given) and ``adaln_int8`` of the new stream."""
+    _check_inference(x, y, gate, shift, scale)
+    x_out = x if x_out is None else x_out
+    rows = _empty_rows(x.shape, x.dtype, x.device)
+    _call(x, y, gate, shift, scale, x_out, None, eps, rows)
+    return x_out, rows
 
 
 class NativeBlockOps:
@@ -135,4 +175,4 @@ class NativeBlockOps:
         return out.view(*a.shape[:-1], weight_a.shape[0])
 
 
-__all__ = ["adaln", "gate_residual", "gate_residual_adaln", "NativeBlockOps"]
+__all__ = ["adaln", "gate_residual", "gate_residual_adaln", "adaln_int8", "gate_residual_adaln_int8", "NativeBlockOps"]

@@ -23,6 +23,7 @@
 #include <cstdint>
 
 #include "common.cuh"
+#include "int8_codes.cuh"
 
 namespace hb {
 namespace {
@@ -164,6 +165,116 @@ __global__ void __launch_bounds__(256) k_adaln(AdaParams p) {
     }
 }
 
+struct AdaInt8Params {
+    AdaParams a;  // h_out unused
+    int8_t* codes;  // [rows][C], row stride c_rs (bytes)
+    int64_t c_rs;
+    float* scales;  // [rows]
+};
+
+// The same pass with h quantised instead of rounded to 16 bits: one warp per row,
+// the row's h formed twice from the registers (once for its largest magnitude,
+// once for its codes), so the int8 product reads half the bytes and no separate
+// pass over h exists.  Memory-bound: 2 C (4 C with the residual) bytes read and
+// C (3 C) written per row.
+template <bool BF16, bool RESIDUAL>
+__global__ void __launch_bounds__(256) k_adaln_int8(const __grid_constant__ AdaInt8Params q) {
+    using V = Vec8<BF16>;
+    using T = typename V::T;
+    const AdaParams& p = q.a;
+    const int lane = threadIdx.x & 31;
+    const int row = blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (row >= p.rows) return;  // whole warps leave together
+    const int b = row / p.rows_per_batch;
+    const int nv = p.C >> 8;
+    const T* x = static_cast<const T*>(p.x) + row * p.x_rs;
+    uint4 xv[kMaxVec];
+#pragma unroll
+    for (int i = 0; i < kMaxVec; ++i)
+        if (i < nv) xv[i] = *reinterpret_cast<const uint4*>(x + 8 * (lane + 32 * i));
+    if constexpr (RESIDUAL) {
+        const T* y = static_cast<const T*>(p.y) + row * p.y_rs;
+        const T* g = static_cast<const T*>(p.gate) + b * p.mod_bs;
+        T* xo = static_cast<T*>(p.x_out) + row * p.xo_rs;
+#pragma unroll
+        for (int i = 0; i < kMaxVec; ++i) {
+            if (i < nv) {
+                const int c = 8 * (lane + 32 * i);
+                float fx[8], fy[8], fg[8];
+                V::load(&xv[i], fx);
+                V::load(y + c, fy);
+                V::load(g + c, fg);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) fx[e] = fmaf(fg[e], fy[e], fx[e]);
+                xv[i] = V::pack(fx);  // the stored residual stream, rounded
+                *reinterpret_cast<uint4*>(xo + c) = xv[i];
+            }
+        }
+    }
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < kMaxVec; ++i) {
+        if (i < nv) {
+            float f[8];
+            V::load(&xv[i], f);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s += f[e];
+        }
+    }
+    const float inv_c = 1.f / static_cast<float>(p.C);
+    const float mean = warp_sum(s) * inv_c;
+    float v = 0.f;
+#pragma unroll
+    for (int i = 0; i < kMaxVec; ++i) {
+        if (i < nv) {
+            float f[8];
+            V::load(&xv[i], f);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float d = f[e] - mean;
+                v = fmaf(d, d, v);
+            }
+        }
+    }
+    const float rstd = rsqrtf(warp_sum(v) * inv_c + p.eps);
+    const T* sh = static_cast<const T*>(p.shift) + b * p.mod_bs;
+    const T* sc = static_cast<const T*>(p.scale) + b * p.mod_bs;
+    auto modulated = [&](int i, float (&f)[8]) {
+        const int c = 8 * (lane + 32 * i);
+        float fs[8], fc[8];
+        V::load(&xv[i], f);
+        V::load(sh + c, fs);
+        V::load(sc + c, fc);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = fmaf((f[e] - mean) * rstd, 1.f + fc[e], fs[e]);
+    };
+    uint32_t mag = 0;  // magnitude bits: NaN sorts above infinity above every number
+#pragma unroll
+    for (int i = 0; i < kMaxVec; ++i) {
+        if (i < nv) {
+            float f[8];
+            modulated(i, f);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) mag = max(mag, __float_as_uint(f[e]) & 0x7fffffffu);
+        }
+    }
+    const RowScale rs = row_scale(__uint_as_float(__reduce_max_sync(0xffffffffu, mag)));
+    if (lane == 0) q.scales[row] = rs.scale;
+    int8_t* out = q.codes + row * q.c_rs;
+#pragma unroll
+    for (int i = 0; i < kMaxVec; ++i) {
+        if (i < nv) {
+            float f[8];
+            modulated(i, f);
+            uint32_t c[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) c[e] = rs.live ? code_bits(f[e], rs.inv) : 0u;
+            *reinterpret_cast<uint2*>(out + 8 * (lane + 32 * i)) =
+                make_uint2(pack_codes(c[0], c[1], c[2], c[3]), pack_codes(c[4], c[5], c[6], c[7]));
+        }
+    }
+}
+
 template <bool BF16>
 int launch_adaln(const AdaParams& p, cudaStream_t st) {
     const dim3 grid((p.rows + 7) / 8), block(256);
@@ -201,4 +312,41 @@ extern "C" int hb_adaln_residual(const void* x, int64_t x_rs, const void* y, int
     AdaParams p{x, y, gate, shift, scale, x_out, h_out, x_rs, y_rs, xo_rs, h_rs, mod_bs, rows, rows_per_batch, C, eps};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     return dtype == 1 ? launch_adaln<true>(p, st) : launch_adaln<false>(p, st);
+}
+
+extern "C" int hb_adaln_residual_int8(const void* x, int64_t x_rs, const void* y, int64_t y_rs, const void* gate,
+                                      const void* shift, const void* scale, int64_t mod_bs, void* x_out,
+                                      int64_t xo_rs, int8_t* codes, int64_t codes_rs, float* scales, int rows,
+                                      int rows_per_batch, int C, float eps, int dtype, void* stream) {
+    using namespace hb;
+    if (!x || !codes || !scales || !shift || !scale || rows < 0 || rows_per_batch <= 0 || C <= 0 || !(eps >= 0.f))
+        return HB_ERR_ARG;
+    if (y && (!gate || !x_out)) return HB_ERR_ARG;  // residual needs its gate and destination
+    if (dtype != 0 && dtype != 1) return HB_ERR_UNSUPPORTED;
+    if (C % 256 || C > 256 * kMaxVec) return HB_ERR_UNSUPPORTED;
+    if (rows > 1 && codes_rs < C) return HB_ERR_ARG;
+    auto a16 = [](const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15) == 0; };
+    auto s8 = [](int64_t st) { return st % 8 == 0; };
+    if (!a16(x) || !a16(shift) || !a16(scale) || !a16(codes) || (y && (!a16(y) || !a16(gate) || !a16(x_out))) ||
+        (reinterpret_cast<uintptr_t>(scales) & 3))
+        return HB_ERR_ALIGN;
+    if (!s8(x_rs) || !s8(y_rs) || !s8(xo_rs) || !s8(mod_bs) || codes_rs % 16) return HB_ERR_ALIGN;
+    if (rows == 0) return HB_OK;
+    const AdaInt8Params p{{x, y, gate, shift, scale, x_out, nullptr, x_rs, y_rs, xo_rs, 0, mod_bs, rows, rows_per_batch, C, eps},
+                          codes, codes_rs, scales};
+    const dim3 grid((rows + 7) / 8), block(256);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (dtype == 1) {
+        if (y)
+            k_adaln_int8<true, true><<<grid, block, 0, st>>>(p);
+        else
+            k_adaln_int8<true, false><<<grid, block, 0, st>>>(p);
+    } else {
+        if (y)
+            k_adaln_int8<false, true><<<grid, block, 0, st>>>(p);
+        else
+            k_adaln_int8<false, false><<<grid, block, 0, st>>>(p);
+    }
+    HB_LAUNCH_CHECK();
+    return HB_OK;
 }

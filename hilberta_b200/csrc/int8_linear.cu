@@ -1,0 +1,509 @@
+// Linear layers in 8-bit integers: rows of 16-bit values quantised with one scale
+// a row, and the product of two such matrices with scales, bias and activation.
+//
+//   scale_m = max_k |x_mk| / 127            code_mk = rint(x_mk * (127 / max_k |x_mk|))
+//   y_mn = act((sum_k xcode_mk * wcode_nk) * (xscale_m * wscale_n) + bias_n)
+//
+// The sum is exact in 32-bit integers (K <= 131072: 127^2 * K < 2^31), so the
+// order in which it is taken, and how K is split over CTAs, cannot change a
+// result; the rest is fp32, rounded once to the 16-bit output type.
+//
+// No counterpart in the reference (it runs the model's bf16 layers as they are);
+// these serve the FLUX blocks' projections and MLPs (hilberta/flux_adapter.py:
+// 280-340 calls the projections around the attention).
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+#include <climits>
+#include <cstdint>
+#include <mutex>
+
+#include "common.cuh"
+#include "int8_codes.cuh"
+#include "sm100_ptx.cuh"
+
+namespace hb {
+namespace {
+
+using namespace ptx;
+constexpr unsigned FULL = 0xffffffffu;
+
+// HB_DEV_* bits of the launches on this device (read by hb_int8_status).
+__device__ int32_t g_int8_status;
+
+template <bool BF16>
+__device__ __forceinline__ float2 unpack2(uint32_t u) {
+    if constexpr (BF16) return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+    return __half22float2(*reinterpret_cast<const __half2*>(&u));
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    if constexpr (BF16) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&v);
+    } else {
+        const __half2 v = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&v);
+    }
+}
+template <bool BF16>
+__device__ __forceinline__ float load16(const uint16_t* p) {
+    return unpack2<BF16>(*p).x;
+}
+
+// Largest magnitude of a pair of 16-bit values as magnitude bits (NaN sorts
+// above infinity above every number, so non-finite values are never lost).
+__device__ __forceinline__ uint32_t max_mag(uint32_t m, uint32_t u) { return __vmaxu2(m, u & 0x7fff7fffu); }
+template <bool BF16>
+__device__ __forceinline__ float mag_value(uint32_t m) {
+    const uint32_t v = max(m & 0xffffu, m >> 16);
+    if constexpr (BF16) return __uint_as_float(v << 16);
+    return load16<false>(reinterpret_cast<const uint16_t*>(&v));
+}
+
+// Codes of four 16-bit values, in order from the low byte.
+template <bool BF16>
+__device__ __forceinline__ uint32_t codes4(uint32_t u0, uint32_t u1, float inv) {
+    const float2 f = unpack2<BF16>(u0), g = unpack2<BF16>(u1);
+    return pack_codes(code_bits(f.x, inv), code_bits(f.y, inv), code_bits(g.x, inv), code_bits(g.y, inv));
+}
+
+// ---- row quantisation ---------------------------------------------------------
+
+struct QuantParams {
+    const uint16_t* a;  // [rows][ka], row stride a_rs (elements)
+    const uint16_t* b;  // [rows][kb] or null: columns ka .. ka + kb of the row
+    int64_t a_rs, b_rs;
+    int ka, k;  // k = ka + kb
+    int rows;
+    int8_t* codes;  // [rows][k], row stride c_rs (bytes)
+    int64_t c_rs;
+    float* scales;  // [rows]
+};
+
+// Eight values of a row from column c.  VEC: rows start on 16 bytes and ka and k
+// are multiples of 8; otherwise element by element (zeros past the end).
+template <bool VEC>
+__device__ __forceinline__ uint4 load8(const QuantParams& p, int64_t row, int c) {
+    if constexpr (VEC) {
+        const uint16_t* src = c < p.ka ? p.a + row * p.a_rs + c : p.b + row * p.b_rs + (c - p.ka);
+        return *reinterpret_cast<const uint4*>(src);
+    } else {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            uint32_t e[2];
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const int x = c + 2 * i + j;
+                e[j] = x < p.ka ? p.a[row * p.a_rs + x] : (x < p.k ? p.b[row * p.b_rs + (x - p.ka)] : 0);
+            }
+            w[i] = e[0] | (e[1] << 16);
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
+// T threads per row (several rows per CTA when T = 32), the row read once and
+// held in registers between its maximum and its codes: up to 8 vectors of 8
+// values a thread; longer rows read the rest again.
+template <bool BF16, bool VEC, int T>
+__global__ void __launch_bounds__(T < 128 ? 128 : T) k_quantize_rows(const __grid_constant__ QuantParams p) {
+    constexpr int CTA = T < 128 ? 128 : T;
+    constexpr int RPC = CTA / T;
+    constexpr int NV = 8;
+    __shared__ uint32_t s_max[CTA / 32];
+    const int t = threadIdx.x % T;
+    const int64_t row = (int64_t)blockIdx.x * RPC + threadIdx.x / T;
+    if (row >= p.rows) return;  // whole warps; RPC > 1 has no block barrier
+    const int nv = (p.k + 7) / 8;
+    uint4 v[NV];
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+        const int j = t + i * T;
+        v[i] = j < nv ? load8<VEC>(p, row, 8 * j) : make_uint4(0, 0, 0, 0);
+        m = max_mag(max_mag(max_mag(max_mag(m, v[i].x), v[i].y), v[i].z), v[i].w);
+    }
+    for (int j = t + NV * T; j < nv; j += T) {
+        const uint4 u = load8<VEC>(p, row, 8 * j);
+        m = max_mag(max_mag(max_mag(max_mag(m, u.x), u.y), u.z), u.w);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = __vmaxu2(m, __shfl_xor_sync(FULL, m, o));
+    if constexpr (T > 32) {
+        if ((threadIdx.x & 31) == 0) s_max[threadIdx.x / 32] = m;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < T / 32; w++) m = __vmaxu2(m, s_max[w]);
+    }
+    const RowScale s = row_scale(mag_value<BF16>(m));
+    if (t == 0) p.scales[row] = s.scale;
+    int8_t* out = p.codes + row * p.c_rs;
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+        const int j = t + i * T;
+        if (j < nv) {
+            uint2 c = make_uint2(codes4<BF16>(v[i].x, v[i].y, s.inv), codes4<BF16>(v[i].z, v[i].w, s.inv));
+            if (!s.live) c = make_uint2(0, 0);
+            *reinterpret_cast<uint2*>(out + 8 * j) = c;  // rows are padded to 16 bytes
+        }
+    }
+    for (int j = t + NV * T; j < nv; j += T) {
+        const uint4 u = load8<VEC>(p, row, 8 * j);
+        uint2 c = make_uint2(codes4<BF16>(u.x, u.y, s.inv), codes4<BF16>(u.z, u.w, s.inv));
+        if (!s.live) c = make_uint2(0, 0);
+        *reinterpret_cast<uint2*>(out + 8 * j) = c;
+    }
+}
+
+template <bool BF16, bool VEC>
+int launch_quantize(const QuantParams& p, cudaStream_t st) {
+    // threads per row: a warp up to 2048 columns (8 vectors a thread), then 4 and 16 warps
+    if (p.k <= 2048)
+        k_quantize_rows<BF16, VEC, 32><<<(unsigned)ceil_div(p.rows, 4), 128, 0, st>>>(p);
+    else if (p.k <= 8192)
+        k_quantize_rows<BF16, VEC, 128><<<p.rows, 128, 0, st>>>(p);
+    else
+        k_quantize_rows<BF16, VEC, 512><<<p.rows, 512, 0, st>>>(p);
+    HB_LAUNCH_CHECK();
+    return HB_OK;
+}
+
+// ---- product ------------------------------------------------------------------
+
+struct LinearParams {
+    CUtensorMap tmap_x;  // int8 [M][K], box 128 x 128 bytes
+    CUtensorMap tmap_w;  // int8 [N][K]
+    const float* x_scales;
+    const float* w_scales;
+    const uint16_t* bias;  // [N] or null
+    uint16_t* out;
+    int64_t out_rs;
+    int M, N, K;
+    int vec_out;  // 8-byte stores allowed
+    long long timeout;
+};
+
+// tanh-GELU(v) = v / (1 + exp(-2u)), u = sqrt(2/pi) (v + 0.044715 v^3), the
+// exponential taken in base 2.
+__device__ __forceinline__ float gelu_tanh(float v) {
+    const float k0 = -2.f * 1.4426950408889634f * 0.7978845608028654f;
+    const float e = ex2(v * fmaf(k0 * 0.044715f, v * v, k0));
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+    return v * r;
+}
+template <int ACT>
+__device__ __forceinline__ float finish(int acc, float sx, float sw, float b) {
+    const float v = fmaf(__int2float_rn(acc) * sx, sw, b);
+    return ACT ? gelu_tanh(v) : v;
+}
+
+// One 128 x 128 output tile per CTA; the CTAs of a cluster split K and add their
+// 32-bit sums through distributed shared memory.
+struct TileCfg {
+    static constexpr int BM = 128, BN = 128, BK = 128;
+    static constexpr int A_BYTES = BM * BK, B_BYTES = BN * BK;
+    static constexpr int STAGES = 6;
+    static constexpr int PITCH = BN + 4;  // 32-bit words: row writes of 16 bytes hit all banks
+    struct Ctl {
+        uint64_t full[STAGES], empty[STAGES], done;
+        uint32_t tmem_base;
+        int abort;
+    };
+    static constexpr int CTL_OFF = STAGES * (A_BYTES + B_BYTES);
+    static constexpr int SMEM = CTL_OFF + (int)((sizeof(Ctl) + 15) / 16 * 16);
+    static_assert(BM * PITCH * 4 <= CTL_OFF, "partial sums reuse the stages");
+};
+
+template <bool BF16, int ACT>
+__global__ void __launch_bounds__(128) k_int8_tile(const __grid_constant__ LinearParams p, int split) {
+    using C = TileCfg;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    auto* ctl = reinterpret_cast<C::Ctl*>(smem + C::CTL_OFF);
+    volatile int* abort_flag = &ctl->abort;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = blockIdx.x % split;
+    const int n0 = (blockIdx.x / split) * C::BN, m0 = blockIdx.y * C::BM;
+    const int nkb = (p.K + C::BK - 1) / C::BK;
+    const int kb0 = (int)((int64_t)nkb * rank / split), kb1 = (int)((int64_t)nkb * (rank + 1) / split);
+
+    if (smem_u32(smem) & 1023) {  // uniform over the cluster
+        if (threadIdx.x == 0) atomicOr(&g_int8_status, HB_DEV_SMEM_ALIGN);
+        return;
+    }
+    if (warp == 0 && lane == 0) {
+        for (int i = 0; i < C::STAGES; i++) {
+            mbar_init(&ctl->full[i], 1);
+            mbar_init(&ctl->empty[i], 1);
+        }
+        mbar_init(&ctl->done, 1);
+        ctl->abort = 0;
+        fence_barrier_init();
+        prefetch_tmap(&p.tmap_x);
+        prefetch_tmap(&p.tmap_w);
+    }
+    if (warp == 2) {
+        tmem_alloc(&ctl->tmem_base, C::BN);
+        tmem_relinquish();
+        tc_fence_before();
+    }
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = ctl->tmem_base;
+
+    if (warp == 0 && lane == 0) {
+        int it = 0;
+        bool ok = true;
+        for (int kb = kb0; kb < kb1; kb++, it++) {
+            const int s = it % C::STAGES;
+            if (it >= C::STAGES && !mbar_wait(&ctl->empty[s], (it / C::STAGES - 1) & 1, abort_flag, p.timeout)) {
+                ok = false;
+                break;
+            }
+            uint8_t* st = smem + s * (C::A_BYTES + C::B_BYTES);
+            mbar_arrive_expect_tx(&ctl->full[s], C::A_BYTES + C::B_BYTES);
+            tma_load_2d(st, &p.tmap_x, &ctl->full[s], kb * C::BK, m0);
+            tma_load_2d(st + C::A_BYTES, &p.tmap_w, &ctl->full[s], kb * C::BK, n0);
+        }
+        if (!ok) {  // let the copies in flight land before the CTA gives up its memory
+            volatile int ignore = 0;
+            for (int j = max(0, it - C::STAGES); j < it; j++)
+                mbar_wait(&ctl->full[j % C::STAGES], (j / C::STAGES) & 1, &ignore, p.timeout);
+        }
+    } else if (warp == 1 && lane == 0) {
+        constexpr uint32_t idesc = idesc_i8(C::BM, C::BN);
+        bool ok = true;
+        int it = 0;
+        for (int kb = kb0; kb < kb1; kb++, it++) {
+            const int s = it % C::STAGES;
+            if (!mbar_wait(&ctl->full[s], (it / C::STAGES) & 1, abort_flag, p.timeout)) {
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+            const uint32_t a = smem_u32(smem + s * (C::A_BYTES + C::B_BYTES)), b = a + C::A_BYTES;
+#pragma unroll
+            for (int k = 0; k < C::BK; k += 32)
+                mma_i8_ss(tmem, desc_sw128(a + k, 16, 1024), desc_sw128(b + k, 16, 1024), idesc, it > 0 || k > 0);
+            tc_commit(&ctl->empty[s]);
+        }
+        if (ok) tc_commit(&ctl->done);
+    }
+    __syncwarp();
+    bool ok = mbar_wait(&ctl->done, 0, abort_flag, p.timeout);
+    ok = __all_sync(FULL, ok);
+    if (!ok && lane == 0) atomicOr(&g_int8_status, HB_DEV_TIMEOUT);
+    int* part = reinterpret_cast<int*>(smem);
+    if (ok) {  // every MMA has read its stage: the tiles' memory is free
+        tc_fence_after();
+        int* dst = part + threadIdx.x * C::PITCH;
+#pragma unroll
+        for (int c = 0; c < C::BN; c += 32) {
+            uint32_t r[32];
+            tmem_ld32(tmem + ((uint32_t)(warp * 32) << 16) + c, r);
+#pragma unroll
+            for (int i = 0; i < 32; i += 4)
+                *reinterpret_cast<uint4*>(dst + c + i) = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
+        }
+        tc_fence_before();
+    }
+    ok = __syncthreads_and(ok);
+    if (split > 1) cluster_sync();  // every CTA of the cluster arrives here, whatever happened before
+    if (warp == 2) {
+        tc_fence_after();
+        tmem_dealloc(tmem, C::BN);
+    }
+    // this CTA's share of the rows, one warp per row, four columns a lane
+    const int r0 = C::BM * rank / split, r1 = C::BM * (rank + 1) / split;
+    const int col = n0 + 4 * lane;
+    if (ok && col < p.N) {
+        float sw[4], b[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const bool in = col + i < p.N;
+            sw[i] = in ? p.w_scales[col + i] : 0.f;
+            b[i] = in && p.bias ? load16<BF16>(p.bias + col + i) : 0.f;
+        }
+        for (int r = r0 + warp; r < r1 && m0 + r < p.M; r += 4) {
+            const int* src = part + r * C::PITCH + 4 * lane;
+            int4 acc = *reinterpret_cast<const int4*>(src);
+            for (int q = 1; q < split; q++) {
+                const int4 v = ld_cluster_v4(cluster_map(smem_u32(src), (rank + q) % split));
+                acc.x += v.x;
+                acc.y += v.y;
+                acc.z += v.z;
+                acc.w += v.w;
+            }
+            const float sx = p.x_scales[m0 + r];
+            const uint2 o = make_uint2(pack2<BF16>(finish<ACT>(acc.x, sx, sw[0], b[0]), finish<ACT>(acc.y, sx, sw[1], b[1])),
+                                       pack2<BF16>(finish<ACT>(acc.z, sx, sw[2], b[2]), finish<ACT>(acc.w, sx, sw[3], b[3])));
+            uint16_t* dst = p.out + (int64_t)(m0 + r) * p.out_rs + col;
+            if (p.vec_out && col + 4 <= p.N) {
+                *reinterpret_cast<uint2*>(dst) = o;
+            } else {
+                const uint16_t e[4] = {(uint16_t)o.x, (uint16_t)(o.x >> 16), (uint16_t)o.y, (uint16_t)(o.y >> 16)};
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (col + i < p.N) dst[i] = e[i];
+            }
+        }
+    }
+    __syncwarp();
+    if (split > 1) cluster_sync();  // peers may still read this CTA's sums
+}
+
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_fn() {
+    static EncodeTiledFn fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void* ptr = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<EncodeTiledFn>(ptr);
+    });
+    return fn;
+}
+
+// [rows][cols] matrix of `type` (elements of `size` bytes, row stride rs bytes)
+// as a 2-D map with 128-byte swizzle and a box of 128 bytes x box_rows.
+int make_tmap_2d(CUtensorMap* map, CUtensorMapDataType type, int size, const void* base, int64_t rows, int64_t cols,
+                 int64_t rs, int box_rows) {
+    EncodeTiledFn enc = encode_fn();
+    if (!enc) return HB_ERR_CUDA;
+    if (rows == 1) rs = (cols * size + 15) / 16 * 16;  // never used for addressing
+    cuuint64_t gdim[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    cuuint64_t gstride[1] = {(cuuint64_t)rs};
+    cuuint32_t box[2] = {(cuuint32_t)(128 / size), (cuuint32_t)box_rows}, estride[2] = {1, 1};
+    const CUresult r = enc(map, type, 2, const_cast<void*>(base), gdim, gstride, box, estride,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? HB_OK : HB_ERR_TMA;
+}
+
+struct DeviceInfo {
+    int sms = 0;
+    int clock_khz = 0;
+    unsigned configured = 0;  // kernels whose shared-memory limit is set
+};
+std::mutex g_mu;
+DeviceInfo g_dev[64];
+
+template <class Kernel>
+int configure(Kernel kern, int dev, int slot, int smem, DeviceInfo* info) {
+    std::lock_guard<std::mutex> lk(g_mu);
+    DeviceInfo& di = g_dev[dev];
+    if (!di.sms) {
+        HB_CUDA_TRY(cudaDeviceGetAttribute(&di.clock_khz, cudaDevAttrClockRate, dev));
+        HB_CUDA_TRY(cudaDeviceGetAttribute(&di.sms, cudaDevAttrMultiProcessorCount, dev));
+    }
+    if (!(di.configured >> slot & 1u)) {
+        HB_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        di.configured |= 1u << slot;
+    }
+    *info = di;
+    return HB_OK;
+}
+
+template <bool BF16, int ACT>
+int launch_tile(LinearParams& p, int dev, cudaStream_t st) {
+    DeviceInfo di;
+    auto kern = k_int8_tile<BF16, ACT>;
+    if (const int rc = configure(kern, dev, BF16 * 2 + ACT, TileCfg::SMEM, &di)) return rc;
+    p.timeout = 2000LL * di.clock_khz;
+    const int64_t tn = ceil_div(p.N, TileCfg::BN), tm = ceil_div(p.M, TileCfg::BM);
+    const int nkb = (int)ceil_div(p.K, TileCfg::BK);
+    int split = 1;  // fill the SMs: double while a tile per CTA leaves half of them idle
+    while (split < 8 && tn * tm * split * 2 <= di.sms && nkb >= 4 * split) split *= 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(tn * split), (unsigned)tm);
+    cfg.blockDim = dim3(128);
+    cfg.dynamicSmemBytes = TileCfg::SMEM;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = split;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    HB_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, p, split));
+    return HB_OK;
+}
+
+inline bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+}  // namespace
+}  // namespace hb
+
+using namespace hb;
+
+extern "C" int hb_quantize_rows(const void* a, int64_t a_rs, int ka, const void* b, int64_t b_rs, int kb, int rows,
+                                int8_t* codes, int64_t codes_rs, float* scales, int dtype, void* stream) {
+    if (rows < 0 || ka <= 0 || kb < 0 || (kb > 0 && !b) || (int64_t)ka + kb > HB_INT8_MAX_K) return HB_ERR_ARG;
+    if (dtype != 0 && dtype != 1) return HB_ERR_UNSUPPORTED;
+    if (rows == 0) return HB_OK;
+    if (!a || !codes || !scales) return HB_ERR_ARG;
+    const int k = ka + kb;
+    if (rows > 1 && codes_rs < k) return HB_ERR_ARG;
+    if (!aligned(a, 2) || !aligned(b, 2) || !aligned(scales, 4) || !aligned(codes, 16) || codes_rs % 16) return HB_ERR_ALIGN;
+    QuantParams p{static_cast<const uint16_t*>(a), static_cast<const uint16_t*>(b), a_rs, b_rs, ka, k, rows, codes, codes_rs, scales};
+    const bool vec = aligned(a, 16) && a_rs % 8 == 0 && ka % 8 == 0 && (!kb || (aligned(b, 16) && b_rs % 8 == 0 && kb % 8 == 0));
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (dtype == 1) return vec ? launch_quantize<true, true>(p, st) : launch_quantize<true, false>(p, st);
+    return vec ? launch_quantize<false, true>(p, st) : launch_quantize<false, false>(p, st);
+}
+
+extern "C" int hb_int8_linear(const int8_t* x, int64_t x_rs, const float* x_scales, const int8_t* w, int64_t w_rs,
+                              const float* w_scales, const void* bias, void* out, int64_t out_rs, int M, int N, int K,
+                              int act, int dtype, void* stream) {
+    if (M < 0 || N < 0 || K <= 0 || K > HB_INT8_MAX_K || act < 0 || act > 1) return HB_ERR_ARG;
+    if (dtype != 0 && dtype != 1) return HB_ERR_UNSUPPORTED;
+    if (M == 0 || N == 0) return HB_OK;
+    if (!x || !x_scales || !w || !w_scales || !out) return HB_ERR_ARG;
+    if ((M > 1 && (x_rs < K || out_rs < N)) || (N > 1 && w_rs < K)) return HB_ERR_ARG;
+    if (!aligned(x, 16) || !aligned(w, 16) || (M > 1 && x_rs % 16) || (N > 1 && w_rs % 16) || !aligned(x_scales, 4) ||
+        !aligned(w_scales, 4) || !aligned(bias, 2) || !aligned(out, 2))
+        return HB_ERR_ALIGN;
+    if (ceil_div(M, 128) > 65535 || ceil_div(N, 128) * 8 > INT32_MAX) return HB_ERR_UNSUPPORTED;
+    LinearParams p;
+    int rc;
+    if ((rc = make_tmap_2d(&p.tmap_x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, x, M, K, x_rs, 128))) return rc;
+    if ((rc = make_tmap_2d(&p.tmap_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w, N, K, w_rs, 128))) return rc;
+    p.x_scales = x_scales;
+    p.w_scales = w_scales;
+    p.bias = static_cast<const uint16_t*>(bias);
+    p.out = static_cast<uint16_t*>(out);
+    p.out_rs = out_rs;
+    p.M = M;
+    p.N = N;
+    p.K = K;
+    p.vec_out = aligned(out, 8) && out_rs % 4 == 0;
+    int dev = 0;
+    HB_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev >= 64) return HB_ERR_UNSUPPORTED;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (dtype == 1) return act ? launch_tile<true, 1>(p, dev, st) : launch_tile<true, 0>(p, dev, st);
+    return act ? launch_tile<false, 1>(p, dev, st) : launch_tile<false, 0>(p, dev, st);
+}
+
+extern "C" int hb_int8_status(int clear, int32_t* bits, void* stream) {
+    if (!bits) return HB_ERR_ARG;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    HB_CUDA_TRY(cudaMemcpyFromSymbolAsync(bits, g_int8_status, sizeof(int32_t), 0, cudaMemcpyDeviceToHost, st));
+    HB_CUDA_TRY(cudaStreamSynchronize(st));
+    if (clear && *bits) {
+        static const int32_t zero = 0;
+        HB_CUDA_TRY(cudaMemcpyToSymbolAsync(g_int8_status, &zero, sizeof(int32_t), 0, cudaMemcpyHostToDevice, st));
+        HB_CUDA_TRY(cudaStreamSynchronize(st));
+    }
+    return HB_OK;
+}

@@ -23,6 +23,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
 #include <climits>
 #include <cstdint>
 
@@ -181,10 +182,166 @@ __global__ void __launch_bounds__(256) k_norm_rope_pack(const __grid_constant__ 
     }
 }
 
+// Query and key heads of one token block together (hb_norm_rope_qk):
+//   r = rsqrt(mean over D of x^2 + eps),  z = x * r * w,
+//   (z[2i], z[2i+1]) -> (z[2i] cos[2i] - z[2i+1] sin[2i], z[2i+1] cos[2i+1] + z[2i] sin[2i+1])
+// in fp32 with one rounding at the end.  Memory-bound: every row is read and
+// written once.  One warp per (token, run of heads): D / 8 lanes hold a row, the
+// token's cos/sin and the head weights stay in registers over the heads, so they
+// are read once per run instead of once per row.
+struct QkParams {
+    const void* x[2];  // query, key: [B][S][H][D]
+    void* out[2];      // may equal x
+    int64_t x_sb[2], x_sn[2], x_sh[2], o_sb[2], o_sn[2], o_sh[2];
+    int H[2];
+    const void* w[2];      // [D] of the rows from token T on
+    const void* w_txt[2];  // [D] of the rows before token T, or null (T == 0)
+    const float* cos;      // [S][D]
+    const float* sin;
+    int B, S, T;
+    int runs, run;  // head runs per token, heads per run (a run never mixes query and key heads)
+    int q_runs;     // runs of the query heads
+    float eps;
+};
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(256) k_norm_rope_qk(const __grid_constant__ QkParams p) {
+    using H16 = Half16<BF16>;
+    constexpr int LPR = D / 8;    // lanes per row
+    constexpr int RPW = 32 / LPR; // rows (heads) a warp handles at once
+    constexpr int U = 4;          // row groups in flight
+    const int lane = threadIdx.x & 31;
+    const int col = 8 * (lane % LPR), sub = lane / LPR;
+    const int64_t items = (int64_t)p.B * p.S * p.runs;
+    const int64_t warps = (int64_t)gridDim.x * 8;
+    for (int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); item < items; item += warps) {
+        const int64_t tok = item / p.runs;
+        const int run = (int)(item - tok * p.runs);
+        const int b = (int)(tok / p.S), s = (int)(tok - (int64_t)b * p.S);
+        const int which = run >= p.q_runs;
+        const int h0 = (run - (which ? p.q_runs : 0)) * p.run;
+        const int h1 = min(h0 + p.run, p.H[which]);
+        const uint16_t* src = static_cast<const uint16_t*>(p.x[which]) + b * p.x_sb[which] + s * p.x_sn[which] + col;
+        uint16_t* dst = static_cast<uint16_t*>(p.out[which]) + b * p.o_sb[which] + s * p.o_sn[which] + col;
+        float cs[8], sn[8], w[8];
+        {
+            const float4* c4 = reinterpret_cast<const float4*>(p.cos + (int64_t)s * D + col);
+            const float4* s4 = reinterpret_cast<const float4*>(p.sin + (int64_t)s * D + col);
+            const float4 ca = c4[0], cb = c4[1], sa = s4[0], sb = s4[1];
+            const uint4 wr = *reinterpret_cast<const uint4*>(
+                static_cast<const uint16_t*>(s < p.T ? p.w_txt[which] : p.w[which]) + col);
+            const uint32_t wu[4] = {wr.x, wr.y, wr.z, wr.w};
+            cs[0] = ca.x, cs[1] = ca.y, cs[2] = ca.z, cs[3] = ca.w, cs[4] = cb.x, cs[5] = cb.y, cs[6] = cb.z, cs[7] = cb.w;
+            sn[0] = sa.x, sn[1] = sa.y, sn[2] = sa.z, sn[3] = sa.w, sn[4] = sb.x, sn[5] = sb.y, sn[6] = sb.z, sn[7] = sb.w;
+#pragma unroll
+            for (int i = 0; i < 4; i++) H16::unpack(wu[i], w[2 * i], w[2 * i + 1]);
+        }
+        for (int h = h0; h < h1; h += U * RPW) {  // uniform over the warp
+            uint4 raw[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int hh = h + u * RPW + sub;
+                raw[u] = hh < h1 ? *reinterpret_cast<const uint4*>(src + hh * p.x_sh[which]) : make_uint4(0, 0, 0, 0);
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int hh = h + u * RPW + sub;
+                const uint32_t in[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+                float f[8], ss = 0.f;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    H16::unpack(in[i], f[2 * i], f[2 * i + 1]);
+                    ss = fmaf(f[2 * i], f[2 * i], ss);
+                    ss = fmaf(f[2 * i + 1], f[2 * i + 1], ss);
+                }
+#pragma unroll
+                for (int o = 1; o < LPR; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+                const float r = rsqrtf(ss * (1.f / D) + p.eps);
+                uint32_t o[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float a = f[2 * i] * r * w[2 * i], c = f[2 * i + 1] * r * w[2 * i + 1];
+                    o[i] = H16::pack(a * cs[2 * i] - c * sn[2 * i], c * cs[2 * i + 1] + a * sn[2 * i + 1]);
+                }
+                if (hh < h1) *reinterpret_cast<uint4*>(dst + hh * p.o_sh[which]) = make_uint4(o[0], o[1], o[2], o[3]);
+            }
+        }
+    }
+}
+
+template <bool BF16>
+int launch_norm_rope_qk(const QkParams& p, int D, int grid, cudaStream_t st) {
+    if (D == 32)
+        k_norm_rope_qk<32, BF16><<<grid, 256, 0, st>>>(p);
+    else if (D == 64)
+        k_norm_rope_qk<64, BF16><<<grid, 256, 0, st>>>(p);
+    else if (D == 128)
+        k_norm_rope_qk<128, BF16><<<grid, 256, 0, st>>>(p);
+    else
+        k_norm_rope_qk<256, BF16><<<grid, 256, 0, st>>>(p);
+    HB_LAUNCH_CHECK();
+    return HB_OK;
+}
+
 }  // namespace
 }  // namespace hb
 
 using namespace hb;
+
+extern "C" int hb_norm_rope_qk(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                               void* q_out, const int64_t* q_out_strides, void* k_out, const int64_t* k_out_strides,
+                               int B, int S, int T, int Hq, int Hk, int D, const void* w_q, const void* w_k,
+                               const void* w_txt_q, const void* w_txt_k, float eps, const float* cos, const float* sin,
+                               int dtype, void* stream) {
+    if (B < 0 || S < 0 || Hq <= 0 || Hk <= 0 || T < 0 || T > S || !(eps >= 0.f)) return HB_ERR_ARG;
+    if (D != 32 && D != 64 && D != 128 && D != 256) return HB_ERR_UNSUPPORTED;
+    if (dtype != 0 && dtype != 1) return HB_ERR_UNSUPPORTED;
+    if (B == 0 || S == 0) return HB_OK;
+    if (!q || !k || !q_out || !k_out || !q_strides || !k_strides || !q_out_strides || !k_out_strides || !w_q || !w_k ||
+        !cos || !sin || (T > 0 && (!w_txt_q || !w_txt_k)))
+        return HB_ERR_ARG;
+    // 16-byte vector accesses: every row start and stride must keep them aligned
+    for (const void* ptr : {q, k, (const void*)q_out, (const void*)k_out, w_q, w_k, T > 0 ? w_txt_q : w_q,
+                            T > 0 ? w_txt_k : w_k, (const void*)cos, (const void*)sin})
+        if (reinterpret_cast<uintptr_t>(ptr) & 15) return HB_ERR_ALIGN;
+    const int64_t* strides[4] = {q_strides, k_strides, q_out_strides, k_out_strides};
+    for (const int64_t* st : strides)
+        for (int i = 0; i < 3; i++)
+            if (st[i] % 8) return HB_ERR_ALIGN;
+    QkParams p;
+    const void* in[2] = {q, k};
+    void* out[2] = {q_out, k_out};
+    for (int i = 0; i < 2; i++) {
+        p.x[i] = in[i];
+        p.out[i] = out[i];
+        p.x_sb[i] = strides[i][0], p.x_sn[i] = strides[i][1], p.x_sh[i] = strides[i][2];
+        p.o_sb[i] = strides[2 + i][0], p.o_sn[i] = strides[2 + i][1], p.o_sh[i] = strides[2 + i][2];
+    }
+    p.H[0] = Hq, p.H[1] = Hk;
+    p.w[0] = w_q, p.w[1] = w_k;
+    p.w_txt[0] = w_txt_q, p.w_txt[1] = w_txt_k;
+    p.cos = cos;
+    p.sin = sin;
+    p.B = B, p.S = S, p.T = T;
+    p.eps = eps;
+    int dev = 0, sms = 0;
+    HB_CUDA_TRY(cudaGetDevice(&dev));
+    HB_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+    // Heads per run: as many as leave a warp's worth of work per resident warp
+    // (the run shares its cos/sin and weights), at least one group of rows.
+    const int rpw = 256 / D, most = std::max(Hq, Hk);
+    const int64_t warps = (int64_t)sms * 32, tokens = (int64_t)B * S;
+    int run = (most + rpw - 1) / rpw * rpw;
+    while (run > rpw && tokens * (((int64_t)Hq + run - 1) / run + ((int64_t)Hk + run - 1) / run) < warps)
+        run = (run / 2 + rpw - 1) / rpw * rpw;
+    p.run = run;
+    p.q_runs = (Hq + run - 1) / run;
+    p.runs = p.q_runs + (Hk + run - 1) / run;
+    const int64_t want = (tokens * p.runs + 7) / 8;
+    const int grid = (int)std::min<int64_t>(want, (int64_t)sms * 8);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return dtype == 1 ? launch_norm_rope_qk<true>(p, D, grid, st) : launch_norm_rope_qk<false>(p, D, grid, st);
+}
 
 extern "C" int hb_norm_rope_pack(const void* txt, int64_t txt_sb, int64_t txt_sn, const void* img, int64_t img_sb,
                                  int64_t img_sn, int B, int T, int n, int H, int D, const void* w_txt,

@@ -1,0 +1,230 @@
+"""Linear layers in 8-bit integers (``hb_quantize_rows``, ``hb_int8_linear``): weights
+and activations as int8 codes with one fp32 scale per row (per output channel,
+per token), products summed exactly in 32-bit integers.
+
+``quantize_rows(x)``                  16-bit rows -> ``Int8Rows`` (weights and activations alike)
+``quantize_rows(a, joined=b)``        the rows [a | b] without the concatenation
+``int8_linear(x, weight, bias, ...)`` act((x @ weight^T) + bias) in 16 bits
+
+A row's scale is max|x| / 127 and its codes round(x * (127 / max|x|)), ties to
+even.  A row holding an infinity or NaN gets the scale NaN: every output made
+from it is NaN.  Inference only, CUDA only.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+
+_DTYPES = {torch.float16: 0, torch.bfloat16: 1}
+_ACTIVATIONS = {None: 0, "gelu_tanh": 1}
+_used: set = set()  # devices with int8 launches (read by paired_kernel.device_status)
+
+
+def _row_stride(t):
+    """Row stride of a [..., K] tensor whose rows are equally spaced; None if they are not."""
+    if t.ndim == 2:
+        return t.stride(0)
+    if t.ndim == 1:
+        return t.shape[0]
+    shape, strides = t.shape, t.stride()
+    rs, want = None, None
+    for d in range(t.ndim - 2, -1, -1):
+        if shape[d] == 1:
+            continue
+        if want is None:
+            rs = strides[d]
+        elif strides[d] != want:
+            return None
+        want = strides[d] * shape[d]
+    return t.shape[-1] if rs is None else rs
+
+
+class Int8Rows:
+    """A matrix in 8 bits: ``values`` int8 ``[..., K]`` and ``scales`` fp32 ``[...]``;
+    row r stands for ``values[r] * scales[r]``.  ``dtype`` is the 16-bit type it
+    stands in for (the output type of products).  Rows are equally spaced and
+    start on 16-byte boundaries (``quantize_rows`` pads them)."""
+
+    __slots__ = ("values", "scales", "dtype", "row_stride")
+
+    def __init__(self, values, scales, dtype):
+        if values.dtype != torch.int8 or scales.dtype != torch.float32:
+            raise TypeError("int8 values and float32 scales required")
+        if dtype not in _DTYPES:
+            raise TypeError("dtype must be float16 or bfloat16")
+        if not values.is_cuda or scales.device != values.device:
+            raise ValueError("values and scales must be on the same CUDA device")
+        if values.ndim < 1 or scales.shape != values.shape[:-1] or not scales.is_contiguous():
+            raise ValueError("scales must be contiguous with one entry per row of values")
+        rs = _row_stride(values)
+        if values.shape[-1] > 1 and values.stride(-1) != 1:
+            raise ValueError("values must have a contiguous last dimension")
+        if scales.numel() <= 1:  # the stride of a single row is never used
+            rs = -(-values.shape[-1] // 16) * 16
+        if rs is None or rs % 16 or rs < values.shape[-1] or values.data_ptr() % 16:
+            raise ValueError("rows of values must be equally spaced, 16-byte aligned and must not overlap")
+        self.values, self.scales, self.dtype, self.row_stride = values, scales, dtype, rs
+
+    @property
+    def shape(self):
+        return self.values.shape
+
+    @property
+    def device(self):
+        return self.values.device
+
+    @property
+    def ndim(self):
+        return self.values.ndim
+
+    def dequantize(self):
+        """The values in 16 bits (for checks; products never form them)."""
+        return (self.values.float() * self.scales.unsqueeze(-1)).to(self.dtype)
+
+    def row_slice(self, start, stop):
+        """Rows [start, stop) of a 2-D matrix, sharing its storage (e.g. the output
+        channels of one projection of a joined weight)."""
+        if self.ndim != 2:
+            raise ValueError("row_slice needs a 2-D matrix")
+        return Int8Rows(self.values[start:stop], self.scales[start:stop], self.dtype)
+
+
+def _empty_rows(shape, dtype, device):
+    K = shape[-1]
+    pitch = -(-K // 16) * 16
+    values = torch.empty(*shape[:-1], pitch, dtype=torch.int8, device=device)
+    return Int8Rows(values if pitch == K else values[..., :K], torch.empty(shape[:-1], dtype=torch.float32, device=device),
+                    dtype)
+
+
+def _check_source(x, what):
+    if not isinstance(x, torch.Tensor) or x.ndim < 1:
+        raise TypeError(f"{what} must be a tensor of rows")
+    if not x.is_cuda:
+        raise ValueError("CUDA tensors required")
+    if x.dtype not in _DTYPES:
+        raise TypeError(f"{what} must be float16 or bfloat16")
+    if x.shape[-1] < 1 or (x.shape[-1] > 1 and x.stride(-1) != 1):
+        raise ValueError(f"{what} must have a nonempty contiguous last dimension")
+    if torch.is_grad_enabled() and x.requires_grad:
+        raise ValueError("Inference only; disable autograd")
+
+
+def _on(device):
+    """The launches of the library go to the current device."""
+    return torch.cuda.device(device) if device.index != torch.cuda.current_device() else _lib.SAME_DEVICE
+
+
+def quantize_rows(x, *, joined=None):
+    """``Int8Rows`` of ``x`` (``[..., K]``, float16 or bfloat16, contiguous last
+    dimension, rows equally spaced); with ``joined`` (``[..., Kj]``, same leading
+    shape and type) of the rows ``[x | joined]``, one scale for both parts."""
+    _check_source(x, "x")
+    ka, kb, j_rs = x.shape[-1], 0, 0
+    if joined is not None:
+        _check_source(joined, "joined")
+        if joined.shape[:-1] != x.shape[:-1] or joined.dtype != x.dtype or joined.device != x.device:
+            raise ValueError("joined must match x's leading shape, dtype and device")
+        kb, j_rs = joined.shape[-1], _row_stride(joined)
+    x_rs = _row_stride(x)
+    if x_rs is None or j_rs is None:
+        raise ValueError("rows must be equally spaced")
+    if ka + kb > _lib.HB_INT8_MAX_K:
+        raise NotImplementedError(f"rows of more than {_lib.HB_INT8_MAX_K} values are not supported")
+    out = _empty_rows((*x.shape[:-1], ka + kb), x.dtype, x.device)
+    rows = out.scales.numel()
+    if rows >= 1 << 31:
+        raise NotImplementedError("2^31 rows or more are not supported")
+    with _on(x.device):
+        rc = _lib.lib().hb_quantize_rows(
+            x.data_ptr(), x_rs, ka, None if joined is None else joined.data_ptr(), j_rs, kb, rows, out.values.data_ptr(),
+            out.row_stride, out.scales.data_ptr(), _DTYPES[x.dtype], torch.cuda.current_stream(x.device).cuda_stream)
+    _lib.check(rc, "hb_quantize_rows")
+    return out
+
+
+def int8_linear(x, weight, bias=None, *, activation=None, out=None):
+    """``act(x @ weight^T + bias)`` with both operands in 8 bits.
+
+    ``x``: ``Int8Rows [..., K]``, or a 16-bit tensor ``[..., K]`` that is quantised
+    in the call.  ``weight``: ``Int8Rows [N, K]``.  ``bias``: ``[N]`` in x's type or
+    None.  ``activation``: None or ``"gelu_tanh"``.  ``out`` (allocated when not
+    given): ``[..., N]`` in x's type with a contiguous last dimension; rows may be
+    spaced (a slice of a wider buffer), a leading dimension whose rows are not
+    equally spaced takes one launch per index.  Integer sums are exact, so equal
+    inputs give equal outputs whatever the number of tokens."""
+    if not isinstance(weight, Int8Rows) or weight.ndim != 2:
+        raise TypeError("weight must be 2-D Int8Rows [N, K] (quantize_rows of a weight matrix)")
+    if not isinstance(x, Int8Rows):
+        _check_source(x, "x")
+    if x.ndim < 1 or x.shape[-1] != weight.shape[1]:
+        raise ValueError("x and weight must have the same inner size")
+    if x.device != weight.device:
+        raise ValueError("x and weight must be on the same CUDA device")
+    if activation not in _ACTIVATIONS:
+        raise ValueError('activation must be None or "gelu_tanh"')
+    N = weight.shape[0]
+    if bias is not None:
+        if bias.shape != (N,) or bias.dtype != x.dtype or bias.device != x.device or not bias.is_contiguous():
+            raise ValueError("bias must be a contiguous [N] tensor of x's type and device")
+        if torch.is_grad_enabled() and bias.requires_grad:
+            raise ValueError("Inference only; disable autograd")
+    shape = (*x.shape[:-1], N)
+    if out is None:
+        out = torch.empty(shape, dtype=x.dtype, device=x.device)
+    else:
+        if out.shape != shape or out.dtype != x.dtype or out.device != x.device or (N > 1 and out.stride(-1) != 1):
+            raise ValueError("out must be [..., N] of x's type and device with a contiguous last dimension")
+        if torch.is_grad_enabled() and out.requires_grad:
+            raise ValueError("Inference output cannot require gradients")
+        _check_out(out, x, weight, bias)
+    rows = x if isinstance(x, Int8Rows) else quantize_rows(x)
+    _product(rows, weight, bias, _ACTIVATIONS[activation], out)
+    return out
+
+
+def _check_out(out, x, weight, bias):
+    strides = sorted((st, n) for st, n in zip(out.stride(), out.shape) if n > 1)
+    reach = 0
+    for st, n in strides:
+        if st <= reach:
+            raise ValueError("out must not overlap itself")
+        reach += st * (n - 1)
+    begin, end = _span(out)
+    parts = [x.values, x.scales] if isinstance(x, Int8Rows) else [x]
+    for t in (*parts, weight.values, weight.scales, bias):
+        if t is not None:
+            first, last = _span(t)
+            if begin < last and first < end:
+                raise ValueError("out cannot alias inputs")
+
+
+def _span(t):
+    if t.numel() == 0:
+        return t.data_ptr(), t.data_ptr()
+    extent = sum((n - 1) * st for n, st in zip(t.shape, t.stride())) + 1
+    return t.data_ptr(), t.data_ptr() + extent * t.element_size()
+
+
+def _product(x, weight, bias, act, out):
+    out_rs = _row_stride(out)
+    if out_rs is None:  # a leading index at a time
+        for i in range(out.shape[0]):
+            _product(Int8Rows(x.values[i], x.scales[i], x.dtype), weight, bias, act, out[i])
+        return
+    dev = x.device
+    N, K = weight.shape
+    with _on(dev):
+        rc = _lib.lib().hb_int8_linear(
+            x.values.data_ptr(), x.row_stride, x.scales.data_ptr(), weight.values.data_ptr(), weight.row_stride,
+            weight.scales.data_ptr(), None if bias is None else bias.data_ptr(), out.data_ptr(), out_rs,
+            x.scales.numel(), N, K, act, _DTYPES[x.dtype], torch.cuda.current_stream(dev).cuda_stream)
+    if rc == _lib.HB_ERR_UNSUPPORTED:
+        raise NotImplementedError(f"int8_linear: {_lib.status_text(rc)}")
+    _lib.check(rc, "hb_int8_linear")
+    _used.add(dev.index)
+
+
+__all__ = ["Int8Rows", "quantize_rows", "int8_linear"]

@@ -16,7 +16,7 @@ from numbers import Integral, Real
 
 import torch
 
-from . import _lib
+from . import _lib, int8
 from .sparse_kernel import _non_overlapping_strides, _tensor_byte_span
 
 LOG2E = 1.4426950408889634
@@ -40,7 +40,8 @@ def _workspace(device: torch.device, stream_handle: int, nbytes: int) -> torch.T
 
 
 def device_status(device=None, *, clear=True) -> int:
-    """OR of the HB_DEV_* bits the kernel reported on `device` (synchronises).
+    """OR of the HB_DEV_* bits the attention and 8-bit product kernels reported on
+    `device` (synchronises).
 
     With ``clear``, resets the status word; a workspace whose launch gave up on a
     wait (HB_DEV_TIMEOUT) may hold stale scheduler words and is zeroed whole."""
@@ -52,6 +53,13 @@ def device_status(device=None, *, clear=True) -> int:
             bits |= word
             if clear:
                 (ws if word & (_lib.HB_DEV_TIMEOUT | _lib.HB_DEV_SMEM_ALIGN) else ws[2]).zero_()
+    if dev.index in int8._used:
+        word = ctypes.c_int32()
+        with torch.cuda.device(dev):
+            torch.cuda.synchronize()
+            rc = _lib.lib().hb_int8_status(int(bool(clear)), ctypes.byref(word), _lib.stream_ptr(dev))
+        _lib.check(rc, "hb_int8_status")
+        bits |= word.value
     return bits
 
 

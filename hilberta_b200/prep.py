@@ -102,3 +102,111 @@ def prepare_qkv(q_txt, k_txt, v_txt, q_img, k_img, v_img, *, heads, norm_q, norm
                        sin=sin, image_rows=image_rows)
     v = norm_rope_pack(v_txt, v_img, heads=heads, image_rows=image_rows)
     return q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2)
+
+
+def _strides3(t):
+    return (ctypes.c_int64 * 3)(*t.stride()[:3])
+
+
+def _bytes(t):
+    """First byte and one past the last of a tensor's elements."""
+    extent = sum((n - 1) * st for n, st in zip(t.shape, t.stride())) + 1
+    return t.data_ptr(), t.data_ptr() + (extent * t.element_size() if t.numel() else 0)
+
+
+def norm_rope_qk(q, k, *, weight_q, weight_k, cos, sin, text_tokens=0, weight_txt_q=None, weight_txt_k=None, eps=1e-6,
+                 out=None):
+    """RMSNorm over the head dimension and rotary embedding of query and key heads,
+    both in one launch (``hb_norm_rope_qk``).
+
+    ``q`` [B, S, Hq, D] and ``k`` [B, S, Hk, D] (Hk may differ: shared key heads),
+    16-bit, D 32/64/128/256 contiguous, any 16-byte aligned outer strides: e.g. the
+    query and key slices of one joined projection.  Weights [D] in the same type;
+    the first ``text_tokens`` tokens use ``weight_txt_q`` / ``weight_txt_k``.
+    ``cos``/``sin`` fp32 [S, D] by token, pairs (2i, 2i+1).  Arithmetic is fp32 with
+    one rounding at the end (``norm_rope_pack`` keeps the rounding of the separate
+    ops it replaces).  ``out`` is a pair of tensors like q and k, ``(q, k)`` itself
+    for in place; by default new contiguous ones.  Returns the pair."""
+    for name, x in (("q", q), ("k", k)):
+        if x.ndim != 4 or not x.is_cuda or x.stride(-1) != 1:
+            raise ValueError(f"{name} must be a CUDA tensor [B, S, heads, D] with contiguous D")
+    dtype = _dtype_code(q)
+    B, S, Hq, D = q.shape
+    Hk = k.shape[2]
+    if k.shape[:2] != (B, S) or k.shape[3] != D or k.dtype != q.dtype or k.device != q.device:
+        raise ValueError("q and k must agree in batch, tokens, D, dtype and device")
+    if Hq < 1 or Hk < 1:
+        raise ValueError("at least one query and one key head required")
+    T = int(text_tokens)
+    if not 0 <= T <= S:
+        raise ValueError("text_tokens must lie within the tokens")
+    if T > 0 and (weight_txt_q is None or weight_txt_k is None):
+        raise ValueError("text tokens need weight_txt_q and weight_txt_k")
+    for w in (weight_q, weight_k, weight_txt_q, weight_txt_k):
+        if w is not None and (w.shape != (D,) or w.dtype != q.dtype or w.device != q.device or not w.is_contiguous()):
+            raise ValueError("norm weights must be contiguous [D] in the heads' dtype")
+    for c in (cos, sin):
+        if c.shape != (S, D) or c.dtype != torch.float32 or c.device != q.device or not c.is_contiguous():
+            raise ValueError("cos/sin must be contiguous fp32 [S, D] on the heads' device")
+    if not eps >= 0:
+        raise ValueError("eps must not be negative")
+    if torch.is_grad_enabled() and any(
+            t is not None and t.requires_grad for t in (q, k, weight_q, weight_k, weight_txt_q, weight_txt_k, cos, sin)):
+        raise ValueError("Inference only; disable autograd")
+    if out is None:
+        out = tuple(torch.empty(x.shape, dtype=q.dtype, device=q.device) for x in (q, k))
+    else:
+        _check_qk_out(q, k, out, (weight_q, weight_k, weight_txt_q, weight_txt_k, cos, sin))
+    q_out, k_out = out
+    dev = q.device
+    with torch.cuda.device(dev) if dev.index != torch.cuda.current_device() else _lib.SAME_DEVICE:
+        rc = _lib.lib().hb_norm_rope_qk(
+            q.data_ptr(), _strides3(q), k.data_ptr(), _strides3(k), q_out.data_ptr(), _strides3(q_out), k_out.data_ptr(),
+            _strides3(k_out), B, S, T, Hq, Hk, D, weight_q.data_ptr(), weight_k.data_ptr(), _lib.ptr(weight_txt_q),
+            _lib.ptr(weight_txt_k), float(eps), cos.data_ptr(), sin.data_ptr(), dtype,
+            torch.cuda.current_stream(dev).cuda_stream)
+    if rc == _lib.HB_ERR_ALIGN:
+        raise ValueError("hb_norm_rope_qk needs 16-byte aligned rows (strides multiples of 8 elements)")
+    if rc == _lib.HB_ERR_UNSUPPORTED:
+        raise NotImplementedError("hb_norm_rope_qk supports D 32, 64, 128 or 256, fp16/bf16")
+    _lib.check(rc, "hb_norm_rope_qk")
+    return q_out, k_out
+
+
+def _check_qk_out(q, k, out, others):
+    """Outputs: like q and k, each either its input in place or apart from everything read."""
+    q_out, k_out = out
+    for name, x, o in (("q", q, q_out), ("k", k, k_out)):
+        if o.shape != x.shape or o.dtype != x.dtype or o.device != x.device or o.stride(-1) != 1:
+            raise ValueError(f"the output of {name} must match its shape, dtype and device with contiguous D")
+        if torch.is_grad_enabled() and o.requires_grad:
+            raise ValueError("Inference output cannot require gradients")
+        reach = 0
+        for st, n in sorted((st, n) for st, n in zip(o.stride(), o.shape) if n > 1):
+            if st <= reach:
+                raise ValueError(f"the output of {name} must not overlap itself")
+            reach += st * (n - 1)
+    same = [o.data_ptr() == x.data_ptr() and o.stride() == x.stride() for x, o in ((q, q_out), (k, k_out))]
+    if all(same) and _interleaved(q, k):
+        return
+    for o, in_place, own in ((q_out, same[0], q), (k_out, same[1], k)):
+        begin, end = _bytes(o)
+        for t in (q, k, *others, *(x for x in out if x is not o)):
+            if t is None or (in_place and t is own):
+                continue
+            first, last = _bytes(t)
+            if begin < last and first < end and not (t.dtype == o.dtype and _interleaved(o, t)):
+                raise ValueError("outputs must be their inputs in place or must not overlap any input")
+
+
+def _interleaved(a, b):
+    """a and b are slices of equally strided rows, side by side within the token
+    stride (as the query and key parts of one joined projection), sharing no element."""
+    if a.ndim != 4 or b.ndim != 4 or a.stride()[:2] != b.stride()[:2]:
+        return False
+    if a.shape[0] > 1 and a.stride(0) < a.shape[1] * a.stride(1):
+        return False
+    width = lambda t: ((t.shape[2] - 1) * t.stride(2) + t.shape[3]) * t.element_size()  # noqa: E731
+    pitch = a.stride(1) * a.element_size()
+    shift = (b.data_ptr() - a.data_ptr()) % pitch if pitch else 0
+    return pitch > 0 and shift >= width(a) and shift + width(b) <= pitch

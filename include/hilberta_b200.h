@@ -28,6 +28,9 @@
  *                                  key_block_size=128) as the equivalent KV64 table
  *   hb_adaln_residual              the adaLN-Zero modulation / gated residual of the FLUX
  *                                  blocks around the processor of flux_adapter.py:259-340
+ *   hb_quantize_rows, hb_int8_linear, hb_adaln_residual_int8, hb_norm_rope_qk
+ *                                  none: the projections, modulation and Q/K preparation
+ *                                  around that processor with 8-bit weights and activations
  */
 #ifndef HILBERTA_B200_H
 #define HILBERTA_B200_H
@@ -313,6 +316,60 @@ int hb_adaln_residual(const void* x, int64_t x_rs, const void* y, int64_t y_rs, 
                       const void* shift, const void* scale, int64_t mod_bs, void* x_out,
                       int64_t xo_rs, void* h_out, int64_t h_rs, int rows, int rows_per_batch, int C,
                       float eps, int dtype, void* stream);
+
+/* ---- 8-bit linear layers -------------------------------------------------- */
+/* No counterpart in the reference (it runs the model's 16-bit layers).  A matrix
+ * in 8 bits is int8 codes [rows][k] (row stride a multiple of 16 bytes, base
+ * 16-byte aligned) and one fp32 scale per row: value = code * scale. */
+#define HB_INT8_MAX_K 131072 /* 127 * 127 * K stays below 2^31 */
+
+/* Quantise rows of 16-bit values (dtype 0 fp16, 1 bf16): scale = max|x| / 127,
+ * code = rint(x * (127 / max|x|)), ties to even, each operation rounded in fp32.
+ * A row is the ka values of a followed by the kb values of b (b may be NULL with
+ * kb 0; element row strides a_rs, b_rs).  A row holding an infinity or NaN gets
+ * codes 0 and scale NaN; a row whose magnitudes are all below 2^-100 codes 0 and
+ * scale 0.  Bytes of a codes row past ka + kb, up to the next multiple of 8, are
+ * written too.  Any alignment of a and b; 16-byte aligned rows with ka and kb
+ * multiples of 8 are read in 16-byte vectors. */
+int hb_quantize_rows(const void* a, int64_t a_rs, int ka, const void* b, int64_t b_rs, int kb,
+                     int rows, int8_t* codes, int64_t codes_rs, float* scales, int dtype,
+                     void* stream);
+
+/* out[m][n] = act(sum_k x[m][k] w[n][k] * (x_scales[m] * w_scales[n]) + bias[n]) for
+ * x [M][K], w [N][K] in 8 bits.  bias: [N] in the output type or NULL; act 0 none,
+ * 1 tanh-GELU; out: 16-bit rows (dtype) with element row stride out_rs.  The sum
+ * is exact; the rest is fp32, rounded once.  A NaN scale makes its outputs NaN.
+ * M or N 0 is a no-op. */
+int hb_int8_linear(const int8_t* x, int64_t x_rs, const float* x_scales, const int8_t* w, int64_t w_rs,
+                   const float* w_scales, const void* bias, void* out, int64_t out_rs, int M, int N,
+                   int K, int act, int dtype, void* stream);
+
+/* HB_DEV_* bits that hb_int8_linear launches on the current device reported
+ * (HB_DEV_TIMEOUT: a bounded wait ran out, some outputs were not written); with
+ * clear, resets them.  Synchronises `stream`. */
+int hb_int8_status(int clear, int32_t* bits, void* stream);
+
+/* hb_adaln_residual with h quantised as hb_quantize_rows does, from its fp32
+ * values: codes [rows][C] (row stride codes_rs bytes, a multiple of 16), one scale
+ * per row.  y NULL: no residual. */
+int hb_adaln_residual_int8(const void* x, int64_t x_rs, const void* y, int64_t y_rs, const void* gate,
+                           const void* shift, const void* scale, int64_t mod_bs, void* x_out,
+                           int64_t xo_rs, int8_t* codes, int64_t codes_rs, float* scales, int rows,
+                           int rows_per_batch, int C, float eps, int dtype, void* stream);
+
+/* Query and key heads after the projections, both in one launch: RMS-normalise
+ * every (token, head) row over D with a learned weight (tokens before T use the
+ * w_txt weights), then rotate pairs (2i, 2i+1) by cos/sin (fp32 [S][D], indexed by
+ * token).  q [B][S][Hq][D], k [B][S][Hk][D], 16-bit, element strides (b, s, h),
+ * D contiguous; outputs likewise (q_out == q with equal strides: in place).  fp32
+ * arithmetic, one rounding at the end (hb_norm_rope_pack rounds after each step,
+ * as the separate ops it replaces do).  w_txt_*: NULL when T is 0.  Pointers
+ * 16-byte aligned, strides multiples of 8 elements; D 32, 64, 128 or 256. */
+int hb_norm_rope_qk(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                    void* q_out, const int64_t* q_out_strides, void* k_out,
+                    const int64_t* k_out_strides, int B, int S, int T, int Hq, int Hk, int D,
+                    const void* w_q, const void* w_k, const void* w_txt_q, const void* w_txt_k,
+                    float eps, const float* cos, const float* sin, int dtype, void* stream);
 
 /* ---- allocation-free variant of hb_paired_fwd --------------------------- */
 /* No counterpart in the reference: an addition for callers that must not

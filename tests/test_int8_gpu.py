@@ -1,0 +1,345 @@
+"""8-bit linear layers (hilberta_b200/int8.py, the int8 forms of block_ops) against
+their formulas in 64 bits.
+
+Row quantisation is elementwise, correctly rounded fp32 arithmetic, so codes and
+scales are compared exactly.  A product's integer sum is exact; what follows is fp32:
+converting the sum, two scale multiplications (one fused with the bias) round
+four times, each by at most 2^-24 of |product| + |bias|, and the result once to
+16 bits, by at most eps/2 of itself.  tanh-GELU has slope at most 1.13, and its
+own fp32 steps stay within 2^-18 of the result: the exponent's three roundings
+are magnified by |exponent| * ln 2 <= 20 where the result is not negligible.
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+BF16, FP16 = torch.bfloat16, torch.float16
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _rows(m, k, dtype, seed, spread=1.0):
+    g = _gen(seed)
+    x = torch.randn(m, k, generator=g, device="cuda") * torch.exp(spread * torch.randn(k, generator=g, device="cuda"))
+    return x.to(dtype)
+
+
+def _quantised(x):
+    """(codes, scales) of the rows of x by the definition: each fp32 operation as the
+    64-bit one rounded to fp32, which is the same (products of two fp32 numbers are
+    exact in 64 bits, and a 64-bit quotient rounds to the correctly rounded one)."""
+    f = x.double()
+    top = f.abs().amax(-1)
+    live = (top >= 2.0**-100) & torch.isfinite(top)
+    inv = torch.where(live, 127 / top, 0.0).float().double()
+    scale = torch.where(live, (top / 127).float(), torch.where(top < 2.0**-100, 0.0, math.nan))
+    codes = torch.where(live[..., None], torch.round((f * inv[..., None]).float()), 0.0)
+    return codes.to(torch.int8), scale
+
+
+def _gelu64(v):
+    return 0.5 * v * (1 + torch.tanh(math.sqrt(2 / math.pi) * (v + 0.044715 * v**3)))
+
+
+def _check_product(got, xc, xs, wc, ws, bias, act):
+    acc = (xc.double() @ wc.double().t()) * (xs.double()[:, None] * ws.double())
+    b = 0.0 if bias is None else bias.double()
+    ref = acc + b
+    slack = 4 * 2.0**-24 * (acc.abs() + (b.abs() if bias is not None else 0.0))
+    rel = torch.finfo(got.dtype).eps / 2
+    if act:
+        slack, rel, ref = 1.13 * slack + 1e-9, rel + 2.0**-18, _gelu64(ref)
+    tiny = 2.0**-25 if got.dtype == FP16 else 0.0  # half a step of the subnormals
+    err = (got.double() - ref).abs()
+    bound = ref.abs() * rel + slack * (1 + rel) + tiny
+    assert bool((err <= bound).all()), (float((err - bound).max()), int((err > bound).sum()))
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("m,k", [(1, 1), (3, 7), (5, 8), (130, 768), (64, 1001), (33, 2048), (17, 2056), (9, 8192),
+                                 (6, 15360), (2, 33000), (2, 131072)])
+def test_quantize_rows_is_exact(m, k, dtype):
+    import hilberta_b200 as hb
+
+    x = _rows(m, k, dtype, seed=k + m)
+    got = hb.quantize_rows(x)
+    codes, scales = _quantised(x)
+    assert torch.equal(got.values, codes) and torch.equal(got.scales, scales)
+    assert got.shape == (m, k) and got.dtype == dtype and got.values.data_ptr() % 16 == 0
+    # half a step from the value, and the rounding of x * inv (2^-24 of at most 127 steps)
+    off = (got.values.double() * got.scales.double()[:, None] - x.double()).abs()
+    assert bool((off <= got.scales.double()[:, None] * (0.5 + 127 * 2.0**-22)).all())
+
+
+def test_quantize_rows_strides_joined_and_leading_shape():
+    import hilberta_b200 as hb
+
+    big = _rows(40, 700, BF16, seed=1)
+    for view in (big[:, 4:300], big[::2, 8:264], big.view(4, 10, 700)[:, :, :64]):  # 8-byte offset, row step 2, 3-D
+        got = hb.quantize_rows(view)
+        codes, scales = _quantised(view)
+        assert torch.equal(got.values, codes) and torch.equal(got.scales, scales)
+    for ka, kb in ((256, 1024), (5, 12), (3072, 12288), (9, 130)):
+        a, b = _rows(21, ka, FP16, seed=2), _rows(21, kb, FP16, seed=3, spread=1.5)
+        got = hb.quantize_rows(a, joined=b)
+        codes, scales = _quantised(torch.cat([a, b], 1))
+        assert torch.equal(got.values, codes) and torch.equal(got.scales, scales)
+    one = hb.quantize_rows(big[7])
+    assert one.values.shape == (700,) and one.scales.shape == ()
+    assert hb.quantize_rows(big[:0]).values.shape == (0, 700)
+
+
+@pytest.mark.parametrize("k", [64, 3000, 20000])
+def test_quantize_rows_special_values(k):
+    import hilberta_b200 as hb
+
+    x = _rows(8, k, BF16, seed=5)
+    x[0] = 0
+    x[1, k // 2] = math.inf
+    x[2, 0] = math.nan
+    x[3, -1] = -math.inf
+    x[4] = 1e-35  # below 2^-100
+    x[5] = torch.finfo(BF16).max
+    x[6] = -x[6].abs()
+    got = hb.quantize_rows(x)
+    codes, scales = _quantised(x)
+    assert torch.equal(got.values, codes)
+    assert torch.equal(got.scales.nan_to_num(-1.0), scales.nan_to_num(-1.0))
+    assert got.scales[0] == 0 and got.scales[1:4].isnan().all() and got.scales[4] == 0
+    # their products: the bias alone for zero rows, NaN for rows that held a non-finite value
+    w = hb.quantize_rows(_rows(48, k, BF16, seed=6))
+    bias = _rows(1, 48, BF16, seed=7)[0]
+    out = hb.int8_linear(got, w, bias)
+    assert torch.equal(out[0], bias) and torch.equal(out[4], bias)
+    assert out[1:4].isnan().all() and out[6:].isfinite().all()
+    assert not out[5].isnan().any()  # K values of 3.4e38 each: sums past the type's range are infinite
+
+
+SIZES = [(1, 1, 1), (1, 64, 16), (2, 768, 3072), (3, 130, 127), (4, 4096, 1000), (5, 1000, 300), (7, 65, 9), (8, 512, 256),
+         (16, 3072, 1280), (65, 1001, 129), (127, 128, 128), (128, 2048, 64), (129, 136, 1333), (256, 640, 256),
+         (257, 1024, 260), (300, 5000, 384), (512, 3072, 1024), (1000, 100, 2048), (1771, 1001, 1333), (2500, 384, 2560),
+         (4173, 512, 3000)]
+
+
+@pytest.mark.parametrize("m,k,n", SIZES)
+@pytest.mark.parametrize("dtype,bias,act", [(BF16, True, None), (FP16, False, "gelu_tanh")])
+def test_int8_linear(m, k, n, dtype, bias, act):
+    import hilberta_b200 as hb
+
+    x = _rows(m, k, dtype, seed=m + k + n, spread=0.5)
+    w = hb.quantize_rows((_rows(n, k, dtype, seed=11, spread=0.0) / math.sqrt(k)).to(dtype))
+    b = _rows(1, n, dtype, seed=12)[0] if bias else None
+    got = hb.int8_linear(x, w, b, activation=act)
+    codes, scales = _quantised(x)
+    assert got.shape == (m, n) and got.dtype == dtype
+    _check_product(got, codes, scales, w.values, w.scales, b, act)
+    assert torch.equal(hb.int8_linear(hb.quantize_rows(x), w, b, activation=act), got)
+    assert hb.device_status() == 0
+
+
+def test_int8_linear_extreme_codes_are_exact():
+    """Sums up to 127 * 127 * K: every product 127 * +-127, in types that hold the result's leading bits."""
+    import hilberta_b200 as hb
+
+    for m, k, n in ((2, 131072, 256), (200, 131072, 144)):
+        x = torch.full((m, k), 127, dtype=torch.int8, device="cuda")
+        w = torch.full((n, k), 127, dtype=torch.int8, device="cuda")
+        w[1::2] = -127
+        w[:, ::3] = 5
+        rows = hb.Int8Rows(x, torch.full((m,), 2.0**-16, device="cuda"), BF16)
+        weight = hb.Int8Rows(w, torch.ones(n, device="cuda"), BF16)
+        _check_product(hb.int8_linear(rows, weight), x, rows.scales, w, weight.scales, None, None)
+
+
+@pytest.mark.parametrize("m", [3, 200, 2000])
+def test_int8_linear_out_views_and_neighbours(m):
+    """Rows of a wider buffer: the columns around them stay as they are."""
+    import hilberta_b200 as hb
+
+    k, n = 384, 520
+    x, w = _rows(m, k, BF16, seed=1), hb.quantize_rows(_rows(n, k, BF16, seed=2))
+    want = hb.int8_linear(x, w)
+    for left, width in ((0, 1024), (8, 1024), (3, 1001), (1, 530)):  # aligned, offset, odd row pitch, odd offset
+        buf = torch.full((m + 2, width), 7.0, dtype=BF16, device="cuda")
+        out = buf[1:m + 1, left:left + n]
+        assert hb.int8_linear(x, w, out=out) is out
+        assert torch.equal(out, want)
+        out.fill_(7.0)
+        assert bool((buf == 7.0).all())
+    # a batch whose rows are not equally spaced
+    x3 = _rows(2 * m, k, BF16, seed=3).view(2, m, k)
+    buf = torch.full((2, m + 5, n), 7.0, dtype=BF16, device="cuda")
+    hb.int8_linear(x3, w, out=buf[:, 5:])
+    assert torch.equal(buf[:, 5:], hb.int8_linear(x3, w)) and bool((buf[:, :5] == 7.0).all())
+
+
+def test_int8_linear_row_does_not_depend_on_its_batch():
+    import hilberta_b200 as hb
+
+    x, w = _rows(1500, 1024, BF16, seed=1), hb.quantize_rows(_rows(768, 1024, BF16, seed=2))
+    want = hb.int8_linear(x, w)
+    for lo, hi in ((0, 1), (3, 7), (100, 300), (1100, 1500)):
+        assert torch.equal(hb.int8_linear(x[lo:hi], w), want[lo:hi])
+
+
+def test_int8_linear_streams_graph_and_repeat():
+    import hilberta_b200 as hb
+
+    sizes = [(2, 768, 640), (300, 1536, 512), (3000, 512, 1024)]
+    cases = [(_rows(m, k, BF16, seed=m), hb.quantize_rows(_rows(n, k, BF16, seed=n))) for m, k, n in sizes]
+    want = [hb.int8_linear(x, w, activation="gelu_tanh") for x, w in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    for _ in range(3):
+        got = []
+        for (x, w), s in zip(cases, streams):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                got.append(hb.int8_linear(x, w, activation="gelu_tanh"))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = [hb.int8_linear(x, w, activation="gelu_tanh") for x, w in cases]
+    for x, _ in cases:
+        x.mul_(-1.5)
+    graph.replay()
+    torch.cuda.synchronize()
+    for (x, w), o in zip(cases, out):
+        assert torch.equal(o, hb.int8_linear(x, w, activation="gelu_tanh"))
+
+
+def _modulation(b, c, dtype, seed):
+    return (torch.randn(b, 6 * c, generator=_gen(seed), device="cuda") * 0.5).to(dtype).chunk(6, dim=-1)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("b,s,c", [(1, 1, 256), (2, 77, 768), (3, 130, 3072), (1, 9, 4096)])
+def test_adaln_int8(b, s, c, dtype):
+    from hilberta_b200.block_ops import adaln_int8, gate_residual, gate_residual_adaln_int8
+
+    x = (_rows(b * s, c, dtype, seed=s, spread=0.5) + 0.5).view(b, s, c)
+    y = _rows(b * s, c, dtype, seed=s + 1).view(b, s, c)
+    shift, scale, gate, *_ = _modulation(b, c, dtype, seed=c)
+
+    def check(stream, rows):
+        f = stream.double()
+        h = (f - f.mean(-1, keepdim=True)) / (f.var(-1, correction=0, keepdim=True) + 1e-6).sqrt()
+        h = h * (1 + scale.double()[:, None]) + shift.double()[:, None]
+        top = h.abs().amax(-1)
+        # fp32 mean and variance over C elements and five elementwise steps
+        fuzz = 2.0**-19 * (h.abs() + shift.double()[:, None].abs() + top[..., None])
+        assert bool(((rows.scales.double() - top / 127).abs() <= top / 127 * 2.0**-17).all())
+        off = (rows.values.double() * rows.scales.double()[..., None] - h).abs()
+        assert bool((off <= rows.scales.double()[..., None] * 0.5 + fuzz).all())
+        assert bool((rows.values.abs().amax(-1) == 127).all())
+
+    rows = adaln_int8(x, shift, scale)
+    assert rows.shape == (b, s, c) and rows.dtype == dtype
+    check(x, rows)
+    apart = torch.empty_like(x)
+    before = x.clone()
+    got, rows = gate_residual_adaln_int8(x, y, gate, shift, scale, x_out=apart)
+    assert got is apart and torch.equal(x, before)
+    assert torch.equal(apart, gate_residual(before.clone(), y, gate))
+    check(apart, rows)
+    got, again = gate_residual_adaln_int8(x, y, gate, shift, scale)
+    assert got is x and torch.equal(x, apart) and torch.equal(again.values, rows.values) and torch.equal(again.scales, rows.scales)
+
+
+def test_adaln_int8_non_finite_rows():
+    from hilberta_b200.block_ops import adaln_int8
+
+    x = _rows(12, 512, BF16, seed=1).view(1, 12, 512)
+    x[0, 3, 100], x[0, 7, 0] = math.nan, math.inf
+    x[0, 5] = 0
+    shift, scale, *_ = _modulation(1, 512, BF16, seed=2)
+    rows = adaln_int8(x, torch.zeros_like(shift), scale)
+    assert rows.scales[0, [3, 7]].isnan().all() and rows.scales[0, 5] == 0
+    assert bool((rows.values[0, [3, 5, 7]] == 0).all())
+    keep = [i for i in range(12) if i not in (3, 7)]
+    assert rows.scales[0, keep].isfinite().all()
+
+
+def test_modulation_then_products_together():
+    """The calls of a block one after the other: modulation, joined Q/K/V product
+    into a wider buffer, norms and rotation in place, MLP, joined output projection."""
+    import hilberta_b200 as hb
+    from hilberta_b200.block_ops import adaln_int8
+
+    b, s, c, heads = 1, 333, 512, 4
+    x = _rows(b * s, c, BF16, seed=1, spread=0.3).view(b, s, c)
+    shift, scale, *_ = _modulation(b, c, BF16, seed=2)
+    wqkv, wup = (hb.quantize_rows((_rows(n, c, BF16, seed=n, spread=0) / math.sqrt(c)).to(BF16)) for n in (3 * c, 4 * c))
+    wout = hb.quantize_rows((_rows(c, 5 * c, BF16, seed=3, spread=0) / math.sqrt(5 * c)).to(BF16))
+    ones = torch.ones(c // heads, dtype=BF16, device="cuda")
+    ang = torch.rand(s, c // heads // 2, generator=_gen(4), device="cuda", dtype=torch.float64) * 6.28
+    cos, sin = (f(ang).repeat_interleave(2, 1).float() for f in (torch.cos, torch.sin))
+    rows = adaln_int8(x, shift, scale)
+    qkv = hb.int8_linear(rows, wqkv).unflatten(-1, (3, heads, c // heads))
+    raw = qkv.clone()
+    q, k = hb.norm_rope_qk(qkv[:, :, 0], qkv[:, :, 1], weight_q=ones, weight_k=ones, cos=cos, sin=sin,
+                           out=(qkv[:, :, 0], qkv[:, :, 1]))
+    assert q.data_ptr() == qkv.data_ptr() and torch.equal(qkv[:, :, 2], raw[:, :, 2])
+    apart = hb.norm_rope_qk(raw[:, :, 0], raw[:, :, 1], weight_q=ones, weight_k=ones, cos=cos, sin=sin)
+    assert torch.equal(apart[0], q) and torch.equal(apart[1], k)
+    up = hb.int8_linear(rows, wup, activation="gelu_tanh")
+    attn = q.flatten(2)
+    out = hb.int8_linear(hb.quantize_rows(attn, joined=up), wout)
+    codes, scales = _quantised(torch.cat([attn, up], -1))
+    _check_product(out[0], codes[0], scales[0], wout.values, wout.scales, None, None)
+    assert hb.device_status() == 0
+
+
+def test_refusals():
+    import hilberta_b200 as hb
+    from hilberta_b200.block_ops import adaln_int8
+
+    x = _rows(8, 64, BF16, seed=1)
+    w = hb.quantize_rows(_rows(32, 64, BF16, seed=2))
+    with pytest.raises(TypeError, match="float16 or bfloat16"):
+        hb.quantize_rows(x.float())
+    with pytest.raises(ValueError, match="contiguous last"):
+        hb.quantize_rows(x.t())
+    with pytest.raises(ValueError, match="equally spaced"):
+        hb.quantize_rows(_rows(64, 64, BF16, seed=3).view(4, 16, 64)[:, :7])
+    with pytest.raises(ValueError, match="leading shape"):
+        hb.quantize_rows(x, joined=x[:4])
+    with pytest.raises(ValueError, match="disable autograd"):
+        hb.quantize_rows(x.clone().requires_grad_())
+    with pytest.raises(TypeError, match="Int8Rows"):
+        hb.int8_linear(x, x)
+    with pytest.raises(ValueError, match="inner size"):
+        hb.int8_linear(x[:, :32], w)
+    with pytest.raises(ValueError, match="activation"):
+        hb.int8_linear(x, w, activation="relu")
+    with pytest.raises(ValueError, match="bias"):
+        hb.int8_linear(x, w, x[0, :32].float())
+    with pytest.raises(ValueError, match="out must be"):
+        hb.int8_linear(x, w, out=torch.empty(8, 31, dtype=BF16, device="cuda"))
+    with pytest.raises(ValueError, match="overlap itself"):
+        hb.int8_linear(x, w, out=torch.empty(1, 32, dtype=BF16, device="cuda").expand(8, 32))
+    wide = _rows(8, 96, BF16, seed=4)
+    with pytest.raises(ValueError, match="alias"):
+        hb.int8_linear(wide[:, :64], w, out=wide[:, 40:72])
+    with pytest.raises(ValueError, match="disable autograd"):
+        hb.int8_linear(x.clone().requires_grad_(), w)
+    values = torch.zeros(4, 72, dtype=torch.int8, device="cuda")
+    with pytest.raises(ValueError, match="16-byte aligned"):
+        hb.Int8Rows(values, torch.ones(4, device="cuda"), BF16)  # row pitch 72
+    with pytest.raises(ValueError, match="one entry per row"):
+        hb.Int8Rows(values[:, :64], torch.ones(3, device="cuda"), BF16)
+    with pytest.raises(TypeError, match="int8"):
+        hb.Int8Rows(values.int(), torch.ones(4, device="cuda"), BF16)
+    with pytest.raises(NotImplementedError):
+        hb.quantize_rows(torch.zeros(1, 131073, dtype=BF16, device="cuda"))
+    m = torch.zeros(1, 128, dtype=BF16, device="cuda")
+    with pytest.raises(NotImplementedError, match="multiple of 256"):
+        adaln_int8(torch.zeros(1, 8, 128, dtype=BF16, device="cuda"), m, m)
