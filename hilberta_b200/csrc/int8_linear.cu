@@ -175,8 +175,9 @@ int launch_quantize(const QuantParams& p, cudaStream_t st) {
 // ---- product ------------------------------------------------------------------
 
 struct LinearParams {
-    CUtensorMap tmap_x;  // int8 [M][K], box 128 x 128 bytes
-    CUtensorMap tmap_w;  // int8 [N][K]
+    CUtensorMap tmap_x;    // int8 [M][K], box 128 x 128 bytes
+    CUtensorMap tmap_w;    // int8 [N][K]
+    CUtensorMap tmap_out;  // 16-bit [M][N], box 32 x 128 bytes (pair kernel, tma_out)
     const float* x_scales;
     const float* w_scales;
     const uint16_t* bias;  // [N] or null
@@ -184,6 +185,8 @@ struct LinearParams {
     int64_t out_rs;
     int M, N, K;
     int vec_out;  // 8-byte stores allowed
+    int tma_out;  // out rows start on 16 bytes: TMA stores
+    int tiles_m, tiles_n;
     long long timeout;
 };
 
@@ -356,6 +359,224 @@ __global__ void __launch_bounds__(128) k_int8_tile(const __grid_constant__ Linea
     if (split > 1) cluster_sync();  // peers may still read this CTA's sums
 }
 
+// 256 x 256 output tiles by CTA pairs, persistent.  One MMA of a pair covers 256
+// x 256 x 32: each CTA stages 128 rows of both operands, so a CTA reads half of
+// the weight tile's bytes that it would need alone, and both keep 128 rows of the
+// accumulator.  Two accumulators fill the TMEM: the epilogue of a tile runs under
+// the products of the next.
+struct PairCfg {
+    static constexpr int BM = 256, BN = 256, BK = 128;
+    static constexpr int A_BYTES = 128 * BK, B_BYTES = 128 * BK, STAGE = A_BYTES + B_BYTES;
+    static constexpr int STAGES = 6;
+    static constexpr int EPI_WARPS = 8;         // two per TMEM lane quarter, half of the columns each
+    static constexpr int STAGING = 32 * 128;    // per warp: 32 rows x 64 columns of the output
+    static constexpr int THREADS = 128 + 32 * EPI_WARPS;
+    struct Ctl {
+        uint64_t full[STAGES], empty[STAGES], acc_full[2], acc_empty[2];
+        uint32_t tmem_base;
+        int abort;
+        alignas(16) float2 cols[BN];  // weight scale and bias of the tile's columns, read two at a time
+    };
+    static constexpr int STG_OFF = STAGES * STAGE;
+    static constexpr int CTL_OFF = STG_OFF + EPI_WARPS * STAGING;
+    static constexpr int SMEM = CTL_OFF + (int)((sizeof(Ctl) + 15) / 16 * 16);
+    static_assert(SMEM <= 227 * 1024, "shared memory of one CTA");
+    // Tiles are walked down columns of GROUP row tiles, so the tiles in flight at
+    // one time share few rows of both operands (both stay in L2).
+    static constexpr int GROUP = 8;
+};
+
+__device__ __forceinline__ void pair_tile(const LinearParams& p, int t, int& m0, int& n0) {
+    const int per = PairCfg::GROUP * p.tiles_n;
+    const int g = t / per, r = t - g * per;
+    const int gm = min(PairCfg::GROUP, p.tiles_m - g * PairCfg::GROUP);
+    m0 = (g * PairCfg::GROUP + r % gm) * PairCfg::BM;
+    n0 = r / gm * PairCfg::BN;
+}
+
+template <bool BF16, int ACT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::THREADS, 1)
+    k_int8_pair(const __grid_constant__ LinearParams p) {
+    using C = PairCfg;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    auto* ctl = reinterpret_cast<C::Ctl*>(smem + C::CTL_OFF);
+    volatile int* abort_flag = &ctl->abort;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = (int)cluster_rank();
+    const int first = blockIdx.x >> 1, step = gridDim.x >> 1, tiles = p.tiles_m * p.tiles_n;
+    const int nkb = (p.K + C::BK - 1) / C::BK;
+
+    if (smem_u32(smem) & 1023) {  // the same in both CTAs
+        if (threadIdx.x == 0) atomicOr(&g_int8_status, HB_DEV_SMEM_ALIGN);
+        return;
+    }
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < C::STAGES; i++) {
+            mbar_init(&ctl->full[i], 1);
+            mbar_init(&ctl->empty[i], 1);
+        }
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&ctl->acc_full[i], 1);
+            mbar_init(&ctl->acc_empty[i], 2 * C::EPI_WARPS);
+        }
+        ctl->abort = 0;
+        fence_barrier_init();
+        prefetch_tmap(&p.tmap_x);
+        prefetch_tmap(&p.tmap_w);
+        if (p.tma_out) prefetch_tmap(&p.tmap_out);
+    }
+    if (warp == 2) {
+        tmem_alloc_pair(&ctl->tmem_base, 512);
+        tc_fence_before();
+    }
+    __syncthreads();
+    cluster_sync();
+    tc_fence_after();
+    const uint32_t tmem = ctl->tmem_base;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int it = 0;
+            bool ok = true;
+            for (int t = first; t < tiles && ok; t += step) {
+                int m0, n0;
+                pair_tile(p, t, m0, n0);
+                for (int kb = 0; kb < nkb; kb++, it++) {
+                    const int s = it % C::STAGES;
+                    if (it >= C::STAGES &&
+                        !mbar_wait_cluster(&ctl->empty[s], (it / C::STAGES - 1) & 1, abort_flag, p.timeout)) {
+                        ok = false;
+                        break;
+                    }
+                    uint8_t* st = smem + s * C::STAGE;
+                    if (rank == 0) mbar_arrive_expect_tx(&ctl->full[s], 2 * C::STAGE);
+                    const uint32_t bar = cluster_map(smem_u32(&ctl->full[s]), 0);
+                    tma_load_2d_pair(st, &p.tmap_x, bar, kb * C::BK, m0 + 128 * rank);
+                    tma_load_2d_pair(st + C::A_BYTES, &p.tmap_w, bar, kb * C::BK, n0 + 128 * rank);
+                }
+            }
+            if (!ok) {  // gave up: time for the copies and MMAs in flight to end before the memory is given back
+                const long long t0 = clock64();
+                while (clock64() - t0 < p.timeout / 1000) {
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            constexpr uint32_t idesc = idesc_i8(C::BM, C::BN);
+            int it = 0, i = 0;
+            bool ok = true;
+            for (int t = first; t < tiles && ok; t += step, i++) {
+                const uint32_t d = tmem + (i & 1) * C::BN;
+                if (i >= 2 && !mbar_wait_cluster(&ctl->acc_empty[i & 1], (i / 2 - 1) & 1, abort_flag, p.timeout)) break;
+                tc_fence_after();
+                for (int kb = 0; kb < nkb; kb++, it++) {
+                    const int s = it % C::STAGES;
+                    if (!mbar_wait_cluster(&ctl->full[s], (it / C::STAGES) & 1, abort_flag, p.timeout)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t a = smem_u32(smem + s * C::STAGE), b = a + C::A_BYTES;
+#pragma unroll
+                    for (int k = 0; k < C::BK; k += 32)
+                        mma_i8_ss_pair(d, desc_sw128(a + k, 16, 1024), desc_sw128(b + k, 16, 1024), idesc, kb > 0 || k > 0);
+                    tc_commit_pair(&ctl->empty[s], 3);
+                }
+                if (ok) tc_commit_pair(&ctl->acc_full[i & 1], 3);
+            }
+        }
+    } else if (warp >= 4) {
+        const int ew = warp - 4, quarter = warp & 3, half = ew >> 2;
+        uint8_t* stg = smem + C::STG_OFF + ew * C::STAGING;
+        float2* cols = ctl->cols + 128 * half;
+        int i = 0;
+        bool dead = false;  // a wait ran out: only the barriers of the remaining tiles are kept, so that no warp is left at one
+        for (int t = first; t < tiles; t += step, i++) {
+            int m0, n0;
+            pair_tile(p, t, m0, n0);
+            const int row0 = m0 + 128 * rank + 32 * quarter, col0 = n0 + 128 * half;
+            {  // this half's column scales and biases (its four warps only)
+                const int c = threadIdx.x & 127;
+                float2 v = make_float2(0.f, 0.f);
+                if (col0 + c < p.N) {
+                    v.x = p.w_scales[col0 + c];
+                    if (p.bias) v.y = load16<BF16>(p.bias + col0 + c);
+                }
+                asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");
+                cols[c] = v;
+                asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");
+            }
+            if (dead) continue;
+            const float sx = row0 + lane < p.M ? p.x_scales[row0 + lane] : 0.f;
+            const bool ok = mbar_wait_cluster(&ctl->acc_full[i & 1], (i >> 1) & 1, abort_flag, p.timeout);
+            if (!__all_sync(FULL, ok)) {
+                if (lane == 0) atomicOr(&g_int8_status, HB_DEV_TIMEOUT);
+                dead = true;
+                continue;
+            }
+            tc_fence_after();
+            const uint32_t acc = tmem + ((uint32_t)(32 * quarter) << 16) + (i & 1) * C::BN + 128 * half;
+#pragma unroll
+            for (int c = 0; c < 128; c += 64) {
+                uint32_t lo[32], hi[32];
+                tmem_ld32_async(acc + c, lo);
+                tmem_ld32_async(acc + c + 32, hi);
+                tmem_wait_ld(lo);
+                tmem_wait_ld(hi);
+                if (c == 64) {  // the accumulator is in registers: the next tile but one may take its place
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster(cluster_map(smem_u32(&ctl->acc_empty[i & 1]), 0));
+                }
+                if (lane == 0) bulk_wait_read<0>();
+                __syncwarp();
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    uint32_t o[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int x = 8 * j + 2 * e;
+                        const float4 sb = *reinterpret_cast<const float4*>(cols + c + x);
+                        const int u = (int)(x < 32 ? lo[x & 31] : hi[x & 31]);
+                        const int v = (int)(x < 32 ? lo[(x + 1) & 31] : hi[(x + 1) & 31]);
+                        o[e] = pack2<BF16>(finish<ACT>(u, sx, sb.x, sb.y), finish<ACT>(v, sx, sb.z, sb.w));
+                    }
+                    // 128-byte rows with the map's swizzle: conflict-free 16-byte stores
+                    *reinterpret_cast<uint4*>(stg + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+                }
+                if (p.tma_out) {
+                    fence_async_smem();
+                    __syncwarp();
+                    if (lane == 0 && row0 < p.M && col0 + c < p.N) {
+                        tma_store_2d(&p.tmap_out, stg, col0 + c, row0);
+                        bulk_commit();
+                    }
+                } else {
+                    __syncwarp();
+                    for (int r = 0; r < 32 && row0 + r < p.M; r++)
+#pragma unroll
+                        for (int k = 0; k < 64; k += 32) {
+                            const int x = k + lane;
+                            if (col0 + c + x < p.N)
+                                p.out[(int64_t)(row0 + r) * p.out_rs + col0 + c + x] = *reinterpret_cast<const uint16_t*>(
+                                    stg + r * 128 + (((x >> 3) ^ (r & 7)) << 4) + (x & 7) * 2);
+                        }
+                    __syncwarp();
+                }
+            }
+        }
+        if (lane == 0) bulk_wait<0>();
+    }
+    __syncwarp();
+    __syncthreads();
+    cluster_sync();  // no CTA leaves while the other's MMAs read its memory or arrivals are on the way
+    if (warp == 2) {
+        tc_fence_after();
+        tmem_dealloc_pair(tmem, 512);
+    }
+}
+
 using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                    const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                    CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -396,6 +617,8 @@ struct DeviceInfo {
 };
 std::mutex g_mu;
 DeviceInfo g_dev[64];
+
+inline bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
 template <class Kernel>
 int configure(Kernel kern, int dev, int slot, int smem, DeviceInfo* info) {
@@ -439,7 +662,63 @@ int launch_tile(LinearParams& p, int dev, cudaStream_t st) {
     return HB_OK;
 }
 
-inline bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+// CTA pairs that can be resident at once (every SM, unless pairs do not fit some).
+template <class Kernel>
+int max_pairs(Kernel kern, int dev, int slot, int* pairs) {
+    static int known[64][8];
+    std::lock_guard<std::mutex> lk(g_mu);
+    int& n = known[dev][slot];
+    if (!n) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(2);
+        cfg.blockDim = dim3(PairCfg::THREADS);
+        cfg.dynamicSmemBytes = PairCfg::SMEM;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = 2;
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        HB_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, kern, &cfg));
+        if (n <= 0) {
+            n = 0;
+            return HB_ERR_UNSUPPORTED;
+        }
+    }
+    *pairs = n;
+    return HB_OK;
+}
+
+template <bool BF16, int ACT>
+int launch_pair(LinearParams& p, int dev, cudaStream_t st) {
+    DeviceInfo di;
+    auto kern = k_int8_pair<BF16, ACT>;
+    const int slot = 4 + BF16 * 2 + ACT;
+    int pairs = 0, rc;
+    if ((rc = configure(kern, dev, slot, PairCfg::SMEM, &di))) return rc;
+    if ((rc = max_pairs(kern, dev, slot, &pairs))) return rc;
+    p.timeout = 2000LL * di.clock_khz;
+    p.tiles_m = (int)ceil_div(p.M, PairCfg::BM);
+    p.tiles_n = (int)ceil_div(p.N, PairCfg::BN);
+    p.tma_out = aligned(p.out, 16) && (p.M == 1 || p.out_rs % 8 == 0);
+    if (p.tma_out &&
+        (rc = make_tmap_2d(&p.tmap_out, BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, p.out,
+                           p.M, p.N, p.out_rs * 2, 32)))
+        return rc;
+    const int tiles = p.tiles_m * p.tiles_n;
+    k_int8_pair<BF16, ACT><<<2 * std::min(tiles, pairs), PairCfg::THREADS, PairCfg::SMEM, st>>>(p);
+    HB_LAUNCH_CHECK();
+    return HB_OK;
+}
+
+template <bool BF16, int ACT>
+int launch_linear(LinearParams& p, int dev, cudaStream_t st) {
+    // Pairs once their tiles would occupy half of the SMs; below that the smaller
+    // tiles and the split of K spread the work further.
+    if (ceil_div(p.M, PairCfg::BM) * ceil_div(p.N, PairCfg::BN) >= 37) return launch_pair<BF16, ACT>(p, dev, st);
+    return launch_tile<BF16, ACT>(p, dev, st);
+}
 
 }  // namespace
 }  // namespace hb
@@ -473,7 +752,7 @@ extern "C" int hb_int8_linear(const int8_t* x, int64_t x_rs, const float* x_scal
     if (!aligned(x, 16) || !aligned(w, 16) || (M > 1 && x_rs % 16) || (N > 1 && w_rs % 16) || !aligned(x_scales, 4) ||
         !aligned(w_scales, 4) || !aligned(bias, 2) || !aligned(out, 2))
         return HB_ERR_ALIGN;
-    if (ceil_div(M, 128) > 65535 || ceil_div(N, 128) * 8 > INT32_MAX) return HB_ERR_UNSUPPORTED;
+    if (ceil_div(M, 128) > 65535 || ceil_div(M, 128) * ceil_div(N, 128) > INT32_MAX / 8) return HB_ERR_UNSUPPORTED;
     LinearParams p;
     int rc;
     if ((rc = make_tmap_2d(&p.tmap_x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, x, M, K, x_rs, 128))) return rc;
@@ -491,8 +770,8 @@ extern "C" int hb_int8_linear(const int8_t* x, int64_t x_rs, const float* x_scal
     HB_CUDA_TRY(cudaGetDevice(&dev));
     if (dev >= 64) return HB_ERR_UNSUPPORTED;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (dtype == 1) return act ? launch_tile<true, 1>(p, dev, st) : launch_tile<true, 0>(p, dev, st);
-    return act ? launch_tile<false, 1>(p, dev, st) : launch_tile<false, 0>(p, dev, st);
+    if (dtype == 1) return act ? launch_linear<true, 1>(p, dev, st) : launch_linear<true, 0>(p, dev, st);
+    return act ? launch_linear<false, 1>(p, dev, st) : launch_linear<false, 0>(p, dev, st);
 }
 
 extern "C" int hb_int8_status(int clear, int32_t* bits, void* stream) {
