@@ -216,6 +216,7 @@ struct TileCfg {
         uint64_t full[STAGES], empty[STAGES], done;
         uint32_t tmem_base;
         int abort;
+        float rows[BM];  // row scales of the tile
     };
     static constexpr int CTL_OFF = STAGES * (A_BYTES + B_BYTES);
     static constexpr int SMEM = CTL_OFF + (int)((sizeof(Ctl) + 15) / 16 * 16);
@@ -248,6 +249,15 @@ __global__ void __launch_bounds__(128) k_int8_tile(const __grid_constant__ Linea
         fence_barrier_init();
         prefetch_tmap(&p.tmap_x);
         prefetch_tmap(&p.tmap_w);
+    }
+    ctl->rows[threadIdx.x] = m0 + (int)threadIdx.x < p.M ? p.x_scales[m0 + threadIdx.x] : 0.f;
+    const int col = n0 + 4 * lane;  // this lane's output columns
+    float sw[4], b[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const bool in = col + i < p.N;
+        sw[i] = in ? p.w_scales[col + i] : 0.f;
+        b[i] = in && p.bias ? load16<BF16>(p.bias + col + i) : 0.f;
     }
     if (warp == 2) {
         tmem_alloc(&ctl->tmem_base, C::BN);
@@ -322,16 +332,9 @@ __global__ void __launch_bounds__(128) k_int8_tile(const __grid_constant__ Linea
     }
     // this CTA's share of the rows, one warp per row, four columns a lane
     const int r0 = C::BM * rank / split, r1 = C::BM * (rank + 1) / split;
-    const int col = n0 + 4 * lane;
     if (ok && col < p.N) {
-        float sw[4], b[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const bool in = col + i < p.N;
-            sw[i] = in ? p.w_scales[col + i] : 0.f;
-            b[i] = in && p.bias ? load16<BF16>(p.bias + col + i) : 0.f;
-        }
-        for (int r = r0 + warp; r < r1 && m0 + r < p.M; r += 4) {
+#pragma unroll 4
+        for (int r = r0 + warp; r < min(r1, p.M - m0); r += 4) {
             const int* src = part + r * C::PITCH + 4 * lane;
             int4 acc = *reinterpret_cast<const int4*>(src);
             for (int q = 1; q < split; q++) {
@@ -341,7 +344,7 @@ __global__ void __launch_bounds__(128) k_int8_tile(const __grid_constant__ Linea
                 acc.z += v.z;
                 acc.w += v.w;
             }
-            const float sx = p.x_scales[m0 + r];
+            const float sx = ctl->rows[r];
             const uint2 o = make_uint2(pack2<BF16>(finish<ACT>(acc.x, sx, sw[0], b[0]), finish<ACT>(acc.y, sx, sw[1], b[1])),
                                        pack2<BF16>(finish<ACT>(acc.z, sx, sw[2], b[2]), finish<ACT>(acc.w, sx, sw[3], b[3])));
             uint16_t* dst = p.out + (int64_t)(m0 + r) * p.out_rs + col;
