@@ -64,6 +64,8 @@ EXPORTS = (
     "hb_expand_kv128",
     "hb_quantize_rows",
     "hb_int8_linear",
+    "hb_int8_linear16_workspace_bytes",
+    "hb_int8_linear16",
     "hb_int8_status",
     "hb_adaln_residual_int8",
     "hb_norm_rope_qk",
@@ -148,6 +150,8 @@ _SIGS = {
     ),
     "hb_quantize_rows": (_I, [_P, _I64, _I, _P, _I64, _I, _I, _P, _I64, _P, _I, _P]),
     "hb_int8_linear": (_I, [_P, _I64, _P, _P, _I64, _P, _P, _P, _I64, _I, _I, _I, _I, _I, _P]),
+    "hb_int8_linear16_workspace_bytes": (ctypes.c_size_t, [_I, _I]),
+    "hb_int8_linear16": (_I, [_P, _I64, _P, _I64, _P, _P, _P, _I64, _I, _I, _I, _I, _I, _P, ctypes.c_size_t, _P]),
     "hb_int8_status": (_I, [_I, ctypes.POINTER(ctypes.c_int32), _P]),
     "hb_adaln_residual_int8": (
         _I,

@@ -205,6 +205,145 @@ __device__ __forceinline__ float finish(int acc, float sx, float sw, float b) {
     return ACT ? gelu_tanh(v) : v;
 }
 
+// A few tokens: every weight is read once and takes part in M products, so the
+// bytes of the weights bound it.  A warp forms R output channels at a time, each
+// lane 16 bytes of every channel's row, with 4-way 8-bit dot products; the tokens'
+// codes lie in shared memory, quantised there from 16 bits by each CTA (they are a
+// few KB; the first weights are on their way meanwhile).  Sums and results are
+// those of the tensor-core kernels, bit for bit.
+struct FewParams {
+    const void* x;  // 16-bit [M][K] (x_scales null) or int8 codes
+    int64_t x_rs;   // elements
+    const float* x_scales;
+    const int8_t* w;
+    int64_t w_rs;
+    const float* w_scales;
+    const uint16_t* bias;
+    uint16_t* out;
+    int64_t out_rs;
+    int M, N, K, act;
+};
+constexpr int kFewRows = 8;
+constexpr int kFewSmem = 64 * 1024;  // codes of the tokens, at most
+inline int64_t few_bytes(int64_t M, int64_t K) { return M * ((K + 15) / 16 * 16); }
+inline bool is_few(int64_t M, int64_t K) { return M <= kFewRows && few_bytes(M, K) <= kFewSmem; }
+
+// 16 bytes of a row of codes, of which `left` (at least 1) are inside it.
+__device__ __forceinline__ int4 load_codes(const int8_t* p, int left) {
+    if (left >= 16) return __ldg(reinterpret_cast<const int4*>(p));
+    uint32_t w[4] = {0, 0, 0, 0};
+    for (int i = 0; i < left; i++) w[i / 4] |= (uint32_t)(uint8_t)p[i] << (8 * (i & 3));
+    return make_int4(w[0], w[1], w[2], w[3]);
+}
+
+// M: the tokens rounded up to a power of two; rows from p.M on do not exist.
+template <bool BF16, bool CODES, int M, int R>
+__global__ void __launch_bounds__(256) k_int8_few(const __grid_constant__ FewParams p) {
+    extern __shared__ __align__(16) int8_t s_codes[];  // [M][pitch]
+    __shared__ uint32_t s_mag[M][8];
+    __shared__ float s_scale[M];
+    constexpr int U = R == 4 ? 2 : 4;  // 16-byte chunks of each channel in flight
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int n0 = (blockIdx.x * 8 + warp) * R;
+    const int chunks = (p.K + 15) / 16, pitch = 16 * chunks;
+    int4 w[U][R];
+    auto fetch = [&](int c0) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int c = c0 + 32 * u + lane;
+#pragma unroll
+            for (int r = 0; r < R; r++)
+                w[u][r] = c < chunks && n0 + r < p.N ? load_codes(p.w + (n0 + r) * p.w_rs + 16 * c, p.K - 16 * c) : make_int4(0, 0, 0, 0);
+        }
+    };
+    fetch(0);
+
+    if constexpr (CODES) {
+        for (int i = threadIdx.x; i < p.M * chunks; i += 256) {
+            const int m = i / chunks, c = i - m * chunks;
+            *reinterpret_cast<int4*>(s_codes + m * pitch + 16 * c) =
+                load_codes(static_cast<const int8_t*>(p.x) + m * p.x_rs + 16 * c, p.K - 16 * c);
+        }
+        if (threadIdx.x < p.M) s_scale[threadIdx.x] = p.x_scales[threadIdx.x];
+        __syncthreads();
+    } else {
+        const uint16_t* x = static_cast<const uint16_t*>(p.x);
+        const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && p.x_rs % 8 == 0;
+        // eight values of row m from column c, zeros past the end
+        auto load8 = [&](int m, int c) {
+            const uint16_t* src = x + m * p.x_rs + c;
+            if (vec && c + 8 <= p.K) return *reinterpret_cast<const uint4*>(src);
+            uint32_t e[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (c + i < p.K) e[i / 2] |= (uint32_t)src[i] << (16 * (i & 1));
+            return make_uint4(e[0], e[1], e[2], e[3]);
+        };
+        uint32_t mag[M];
+#pragma unroll
+        for (int m = 0; m < M; m++) {
+            mag[m] = 0;
+            for (int c = 8 * threadIdx.x; c < p.K && m < p.M; c += 8 * 256) {
+                const uint4 v = load8(m, c);
+                mag[m] = max_mag(max_mag(max_mag(max_mag(mag[m], v.x), v.y), v.z), v.w);
+            }
+        }
+#pragma unroll
+        for (int m = 0; m < M; m++) {
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) mag[m] = __vmaxu2(mag[m], __shfl_xor_sync(FULL, mag[m], o));
+            if (lane == 0) s_mag[m][warp] = mag[m];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int m = 0; m < M; m++) {
+            uint32_t g = s_mag[m][0];
+#pragma unroll
+            for (int i = 1; i < 8; i++) g = __vmaxu2(g, s_mag[m][i]);
+            const RowScale s = row_scale(mag_value<BF16>(g));
+            if (threadIdx.x == 0) s_scale[m] = s.scale;
+            for (int c = 8 * threadIdx.x; c < pitch && m < p.M; c += 8 * 256) {
+                const uint4 v = load8(m, c);
+                uint2 q = make_uint2(codes4<BF16>(v.x, v.y, s.inv), codes4<BF16>(v.z, v.w, s.inv));
+                if (!s.live) q = make_uint2(0, 0);
+                *reinterpret_cast<uint2*>(s_codes + m * pitch + c) = q;
+            }
+        }
+        __syncthreads();
+    }
+
+    int acc[R][M] = {};
+    for (int c0 = 0; c0 < chunks; c0 += 32 * U) {
+        if (c0 > 0) fetch(c0);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int c = c0 + 32 * u + lane;
+            if (c < chunks) {
+#pragma unroll
+                for (int m = 0; m < M; m++) {
+                    if (m >= p.M) break;
+                    const int4 x = *reinterpret_cast<const int4*>(s_codes + m * pitch + 16 * c);
+#pragma unroll
+                    for (int r = 0; r < R; r++)
+                        acc[r][m] = __dp4a(w[u][r].w, x.w, __dp4a(w[u][r].z, x.z, __dp4a(w[u][r].y, x.y, __dp4a(w[u][r].x, x.x, acc[r][m]))));
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+#pragma unroll
+        for (int m = 0; m < M; m++) {
+            const int sum = __reduce_add_sync(FULL, acc[r][m]);
+            if (lane == r * M + m && n0 + r < p.N && m < p.M) {
+                const float ws = p.w_scales[n0 + r], b = p.bias ? load16<BF16>(p.bias + n0 + r) : 0.f;
+                const float y = p.act ? finish<1>(sum, s_scale[m], ws, b) : finish<0>(sum, s_scale[m], ws, b);
+                p.out[m * p.out_rs + n0 + r] = (uint16_t)pack2<BF16>(y, 0.f);
+            }
+        }
+    }
+}
+
 // One 128 x 128 output tile per CTA; the CTAs of a cluster split K and add their
 // 32-bit sums through distributed shared memory.
 struct TileCfg {
@@ -623,20 +762,56 @@ DeviceInfo g_dev[64];
 
 inline bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
-template <class Kernel>
-int configure(Kernel kern, int dev, int slot, int smem, DeviceInfo* info) {
+int device_info(int dev, DeviceInfo* info) {
     std::lock_guard<std::mutex> lk(g_mu);
     DeviceInfo& di = g_dev[dev];
     if (!di.sms) {
         HB_CUDA_TRY(cudaDeviceGetAttribute(&di.clock_khz, cudaDevAttrClockRate, dev));
         HB_CUDA_TRY(cudaDeviceGetAttribute(&di.sms, cudaDevAttrMultiProcessorCount, dev));
     }
+    *info = di;
+    return HB_OK;
+}
+
+template <class Kernel>
+int configure(Kernel kern, int dev, int slot, int smem, DeviceInfo* info) {
+    if (const int rc = device_info(dev, info)) return rc;
+    std::lock_guard<std::mutex> lk(g_mu);
+    DeviceInfo& di = g_dev[dev];
     if (!(di.configured >> slot & 1u)) {
         HB_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
         di.configured |= 1u << slot;
     }
-    *info = di;
     return HB_OK;
+}
+
+template <bool BF16, bool CODES, int M, int R>
+int launch_few(const FewParams& p, cudaStream_t st) {
+    const int smem = (int)few_bytes(p.M, p.K);
+    auto kern = k_int8_few<BF16, CODES, M, R>;
+    if (smem > 46 * 1024)  // near the default limit and above it: rare, so the limit is set each time
+        HB_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem));
+    kern<<<(unsigned)ceil_div(p.N, 8 * R), 256, smem, st>>>(p);
+    HB_LAUNCH_CHECK();
+    return HB_OK;
+}
+
+template <bool BF16, bool CODES>
+int launch_few(const FewParams& p, int dev, cudaStream_t st) {
+    DeviceInfo di;
+    if (const int rc = device_info(dev, &di)) return rc;
+    // Channels per warp: four where that still leaves two CTAs per SM, so that a
+    // token's codes are read from shared memory once for four channels.
+    const bool wide = p.N >= 64 * di.sms;
+    if (p.M == 1) return wide ? launch_few<BF16, CODES, 1, 4>(p, st) : launch_few<BF16, CODES, 1, 1>(p, st);
+    if (p.M == 2) return wide ? launch_few<BF16, CODES, 2, 4>(p, st) : launch_few<BF16, CODES, 2, 1>(p, st);
+    if (p.M <= 4) return wide ? launch_few<BF16, CODES, 4, 4>(p, st) : launch_few<BF16, CODES, 4, 1>(p, st);
+    return wide ? launch_few<BF16, CODES, 8, 4>(p, st) : launch_few<BF16, CODES, 8, 1>(p, st);
+}
+
+template <bool CODES>
+int launch_few(const FewParams& p, int dtype, int dev, cudaStream_t st) {
+    return dtype == 1 ? launch_few<true, CODES>(p, dev, st) : launch_few<false, CODES>(p, dev, st);
 }
 
 template <bool BF16, int ACT>
@@ -744,18 +919,30 @@ extern "C" int hb_quantize_rows(const void* a, int64_t a_rs, int ka, const void*
     return vec ? launch_quantize<false, true>(p, st) : launch_quantize<false, false>(p, st);
 }
 
-extern "C" int hb_int8_linear(const int8_t* x, int64_t x_rs, const float* x_scales, const int8_t* w, int64_t w_rs,
-                              const float* w_scales, const void* bias, void* out, int64_t out_rs, int M, int N, int K,
-                              int act, int dtype, void* stream) {
+namespace hb {
+namespace {
+// Checks shared by the two linear entries; 1: nothing to do.
+int check_linear(const void* x, const int8_t* w, int64_t w_rs, const float* w_scales, const void* bias, const void* out,
+                 int64_t out_rs, int M, int N, int K, int act, int dtype) {
     if (M < 0 || N < 0 || K <= 0 || K > HB_INT8_MAX_K || act < 0 || act > 1) return HB_ERR_ARG;
     if (dtype != 0 && dtype != 1) return HB_ERR_UNSUPPORTED;
-    if (M == 0 || N == 0) return HB_OK;
-    if (!x || !x_scales || !w || !w_scales || !out) return HB_ERR_ARG;
-    if ((M > 1 && (x_rs < K || out_rs < N)) || (N > 1 && w_rs < K)) return HB_ERR_ARG;
-    if (!aligned(x, 16) || !aligned(w, 16) || (M > 1 && x_rs % 16) || (N > 1 && w_rs % 16) || !aligned(x_scales, 4) ||
-        !aligned(w_scales, 4) || !aligned(bias, 2) || !aligned(out, 2))
+    if (M == 0 || N == 0) return 1;
+    if (!x || !w || !w_scales || !out) return HB_ERR_ARG;
+    if ((M > 1 && out_rs < N) || (N > 1 && w_rs < K)) return HB_ERR_ARG;
+    if (!aligned(w, 16) || (N > 1 && w_rs % 16) || !aligned(w_scales, 4) || !aligned(bias, 2) || !aligned(out, 2))
         return HB_ERR_ALIGN;
     if (ceil_div(M, 128) > 65535 || ceil_div(M, 128) * ceil_div(N, 128) > INT32_MAX / 8) return HB_ERR_UNSUPPORTED;
+    return HB_OK;
+}
+
+int current_device(int* dev) {
+    HB_CUDA_TRY(cudaGetDevice(dev));
+    return *dev < 64 ? HB_OK : HB_ERR_UNSUPPORTED;
+}
+
+int linear_codes(const int8_t* x, int64_t x_rs, const float* x_scales, const int8_t* w, int64_t w_rs, const float* w_scales,
+                 const void* bias, void* out, int64_t out_rs, int M, int N, int K, int act, int dtype, int dev,
+                 cudaStream_t st) {
     LinearParams p;
     int rc;
     if ((rc = make_tmap_2d(&p.tmap_x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, x, M, K, x_rs, 128))) return rc;
@@ -769,12 +956,52 @@ extern "C" int hb_int8_linear(const int8_t* x, int64_t x_rs, const float* x_scal
     p.N = N;
     p.K = K;
     p.vec_out = aligned(out, 8) && out_rs % 4 == 0;
-    int dev = 0;
-    HB_CUDA_TRY(cudaGetDevice(&dev));
-    if (dev >= 64) return HB_ERR_UNSUPPORTED;
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (dtype == 1) return act ? launch_linear<true, 1>(p, dev, st) : launch_linear<true, 0>(p, dev, st);
     return act ? launch_linear<false, 1>(p, dev, st) : launch_linear<false, 0>(p, dev, st);
+}
+}  // namespace
+}  // namespace hb
+
+extern "C" int hb_int8_linear(const int8_t* x, int64_t x_rs, const float* x_scales, const int8_t* w, int64_t w_rs,
+                              const float* w_scales, const void* bias, void* out, int64_t out_rs, int M, int N, int K,
+                              int act, int dtype, void* stream) {
+    int rc = check_linear(x, w, w_rs, w_scales, bias, out, out_rs, M, N, K, act, dtype), dev = 0;
+    if (rc) return rc > 0 ? HB_OK : rc;
+    if (!x_scales || (M > 1 && x_rs < K)) return HB_ERR_ARG;
+    if (!aligned(x, 16) || (M > 1 && x_rs % 16) || !aligned(x_scales, 4)) return HB_ERR_ALIGN;
+    if ((rc = current_device(&dev))) return rc;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (is_few(M, K)) {
+        const FewParams p{x, x_rs, x_scales, w, w_rs, w_scales, static_cast<const uint16_t*>(bias), static_cast<uint16_t*>(out), out_rs, M, N, K, act};
+        return launch_few<true>(p, dtype, dev, st);
+    }
+    return linear_codes(x, x_rs, x_scales, w, w_rs, w_scales, bias, out, out_rs, M, N, K, act, dtype, dev, st);
+}
+
+extern "C" size_t hb_int8_linear16_workspace_bytes(int M, int K) {
+    if (M <= 0 || K <= 0 || K > HB_INT8_MAX_K || is_few(M, K)) return 0;
+    return (size_t)(few_bytes(M, K) + 4 * (int64_t)M);
+}
+
+extern "C" int hb_int8_linear16(const void* x, int64_t x_rs, const int8_t* w, int64_t w_rs, const float* w_scales,
+                                const void* bias, void* out, int64_t out_rs, int M, int N, int K, int act, int dtype,
+                                void* workspace, size_t workspace_bytes, void* stream) {
+    int rc = check_linear(x, w, w_rs, w_scales, bias, out, out_rs, M, N, K, act, dtype), dev = 0;
+    if (rc) return rc > 0 ? HB_OK : rc;
+    if (!aligned(x, 2)) return HB_ERR_ALIGN;
+    const size_t need = hb_int8_linear16_workspace_bytes(M, K);
+    if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16))) return HB_ERR_WORKSPACE;
+    if ((rc = current_device(&dev))) return rc;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (!need) {
+        const FewParams p{x, x_rs, nullptr, w, w_rs, w_scales, static_cast<const uint16_t*>(bias), static_cast<uint16_t*>(out), out_rs, M, N, K, act};
+        return launch_few<false>(p, dtype, dev, st);
+    }
+    int8_t* codes = static_cast<int8_t*>(workspace);
+    const int64_t pitch = few_bytes(1, K);
+    float* scales = reinterpret_cast<float*>(codes + pitch * M);
+    if ((rc = hb_quantize_rows(x, x_rs, K, nullptr, 0, 0, M, codes, pitch, scales, dtype, stream))) return rc;
+    return linear_codes(codes, pitch, scales, w, w_rs, w_scales, bias, out, out_rs, M, N, K, act, dtype, dev, st);
 }
 
 extern "C" int hb_int8_status(int clear, int32_t* bits, void* stream) {

@@ -180,8 +180,7 @@ def int8_linear(x, weight, bias=None, *, activation=None, out=None):
         if torch.is_grad_enabled() and out.requires_grad:
             raise ValueError("Inference output cannot require gradients")
         _check_out(out, x, weight, bias)
-    rows = x if isinstance(x, Int8Rows) else quantize_rows(x)
-    _product(rows, weight, bias, _ACTIVATIONS[activation], out)
+    _product(x, weight, bias, _ACTIVATIONS[activation], out)
     return out
 
 
@@ -209,18 +208,28 @@ def _span(t):
 
 
 def _product(x, weight, bias, act, out):
+    coded = isinstance(x, Int8Rows)
     out_rs = _row_stride(out)
-    if out_rs is None:  # a leading index at a time
+    x_rs = x.row_stride if coded else _row_stride(x)
+    if out_rs is None or x_rs is None:  # a leading index at a time
         for i in range(out.shape[0]):
-            _product(Int8Rows(x.values[i], x.scales[i], x.dtype), weight, bias, act, out[i])
+            part = Int8Rows(x.values[i], x.scales[i], x.dtype) if coded else x[i]
+            _product(part, weight, bias, act, out[i])
         return
     dev = x.device
-    N, K = weight.shape
+    lib = _lib.lib()
+    N, K = weight.values.shape
+    M = x.scales.numel() if coded else x.numel() // K
+    tail = (weight.values.data_ptr(), weight.row_stride, weight.scales.data_ptr(), None if bias is None else bias.data_ptr(),
+            out.data_ptr(), out_rs, M, N, K, act, _DTYPES[x.dtype])
     with _on(dev):
-        rc = _lib.lib().hb_int8_linear(
-            x.values.data_ptr(), x.row_stride, x.scales.data_ptr(), weight.values.data_ptr(), weight.row_stride,
-            weight.scales.data_ptr(), None if bias is None else bias.data_ptr(), out.data_ptr(), out_rs,
-            x.scales.numel(), N, K, act, _DTYPES[x.dtype], torch.cuda.current_stream(dev).cuda_stream)
+        stream = torch._C._cuda_getCurrentRawStream(dev.index)
+        if coded:
+            rc = lib.hb_int8_linear(x.values.data_ptr(), x_rs, x.scales.data_ptr(), *tail, stream)
+        else:
+            nbytes = lib.hb_int8_linear16_workspace_bytes(M, K)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+            rc = lib.hb_int8_linear16(x.data_ptr(), x_rs, *tail, None if ws is None else ws.data_ptr(), nbytes, stream)
     if rc == _lib.HB_ERR_UNSUPPORTED:
         raise NotImplementedError(f"int8_linear: {_lib.status_text(rc)}")
     _lib.check(rc, "hb_int8_linear")

@@ -344,7 +344,17 @@ int hb_int8_linear(const int8_t* x, int64_t x_rs, const float* x_scales, const i
                    const float* w_scales, const void* bias, void* out, int64_t out_rs, int M, int N,
                    int K, int act, int dtype, void* stream);
 
-/* HB_DEV_* bits that hb_int8_linear launches on the current device reported
+/* The same for x in 16 bits (element row stride x_rs, any alignment), quantised as
+ * hb_quantize_rows does: the result equals hb_quantize_rows + hb_int8_linear bit for
+ * bit.  A few tokens are quantised inside the product's kernel; otherwise the codes
+ * and scales go to the workspace (16-byte aligned, at least
+ * hb_int8_linear16_workspace_bytes(M, K), which is 0 when none is needed). */
+size_t hb_int8_linear16_workspace_bytes(int M, int K);
+int hb_int8_linear16(const void* x, int64_t x_rs, const int8_t* w, int64_t w_rs, const float* w_scales,
+                     const void* bias, void* out, int64_t out_rs, int M, int N, int K, int act,
+                     int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/* HB_DEV_* bits that hb_int8_linear and hb_int8_linear16 launches on the current device reported
  * (HB_DEV_TIMEOUT: a bounded wait ran out, some outputs were not written); with
  * clear, resets them.  Synchronises `stream`. */
 int hb_int8_status(int clear, int32_t* bits, void* stream);

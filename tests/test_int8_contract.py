@@ -54,6 +54,18 @@ def test_int8_linear_checks(lib):
     assert call(dtype=2) == _lib.HB_ERR_UNSUPPORTED
     assert call(M=0, x=None, out=None) == _lib.HB_OK
     assert call(N=0, w=None, out=None) == _lib.HB_OK
+    ws = lib.hb_int8_linear16_workspace_bytes
+    assert ws(0, 64) == 0 and ws(1, 0) == 0 and ws(1, 64) == 0  # nothing to do; few tokens stay on chip
+    assert ws(100, 70) == 100 * 80 + 400 and ws(8, 131072) == 8 * 131072 + 32
+
+    def call16(x=F, M=100, K=64, w=F, out=F, wsp=F, nbytes=100 * 64 + 400, dtype=1):
+        return lib.hb_int8_linear16(x, 64, w, 64, F, None, out, 32, M, 32, K, 0, dtype, wsp, nbytes, None)
+
+    assert call16(x=None) == _lib.HB_ERR_ARG and call16(out=None) == _lib.HB_ERR_ARG and call16(K=0) == _lib.HB_ERR_ARG
+    assert call16(x=_at(1)) == _lib.HB_ERR_ALIGN and call16(dtype=3) == _lib.HB_ERR_UNSUPPORTED
+    for bad in (dict(wsp=None), dict(nbytes=100 * 64 + 399), dict(wsp=_at(8))):
+        assert call16(**bad) == _lib.HB_ERR_WORKSPACE, bad
+    assert call16(M=0, x=None, wsp=None) == _lib.HB_OK
     assert lib.hb_int8_status(0, None, None) == _lib.HB_ERR_ARG
 
 
