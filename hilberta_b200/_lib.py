@@ -159,8 +159,8 @@ _SIGS = {
     ),
     "hb_norm_rope_qk": (
         _I,
-        [_P, ctypes.POINTER(ctypes.c_int64), _P, ctypes.POINTER(ctypes.c_int64), _P, ctypes.POINTER(ctypes.c_int64), _P,
-         ctypes.POINTER(ctypes.c_int64), _I, _I, _I, _I, _I, _I, _P, _P, _P, _P, ctypes.c_float, _P, _P, _I, _P],
+        [_P, _P, _P, _P, ctypes.POINTER(ctypes.c_int64), _I, _I, _I, _I, _I, _I, _P, _P, _P, _P, ctypes.c_float, _P, _P,
+         _I, _P],
     ),
     "hb_paired_fwd_noalloc": (
         _I,
@@ -209,6 +209,11 @@ def ptr(t: torch.Tensor | None):
 
 # For ``with``: the current device is the launch's device already.
 SAME_DEVICE = contextlib.nullcontext()
+
+
+def stream_handle(device) -> int:
+    """The current stream of ``device`` as an integer (no Stream object is made)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def stream_ptr(device) -> ctypes.c_void_p:

@@ -21,7 +21,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .int8 import _empty_rows
+from .int8 import _empty_rows, _span
 
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1}
 
@@ -51,8 +51,7 @@ def _mod(m, B, C, x, name):
     return m, (m.stride(0) if B > 1 else 0)
 
 
-def _call(x, y, gate, shift, scale, x_out, h_out, eps, rows8=None):
-    """One launch; the modulated rows go to ``h_out``, or quantised to ``rows8``."""
+def _call(x, y, gate, shift, scale, x_out, h_out, eps):
     if not x.is_cuda:
         raise ValueError("CUDA tensors required")
     if x.dtype not in _DTYPES:
@@ -73,18 +72,6 @@ def _call(x, y, gate, shift, scale, x_out, h_out, eps, rows8=None):
                 raise ValueError(f"{name} must match x's shape, dtype and device")
             strides[name] = _rows(t, name)[1]
     dev = x.device
-    if rows8 is not None:
-        with torch.cuda.device(dev) if dev.index != torch.cuda.current_device() else _lib.SAME_DEVICE:
-            rc = _lib.lib().hb_adaln_residual_int8(
-                x.data_ptr(), x_rs, None if y is None else y.data_ptr(), strides.get("y", 0),
-                None if gate is None else gate.data_ptr(), shift.data_ptr(), scale.data_ptr(), mod_bs or 0,
-                None if x_out is None else x_out.data_ptr(), strides.get("x_out", 0), rows8.values.data_ptr(),
-                rows8.row_stride, rows8.scales.data_ptr(), B * S, S, C, float(eps), _DTYPES[x.dtype],
-                torch.cuda.current_stream(dev).cuda_stream)
-        if rc == _lib.HB_ERR_UNSUPPORTED:
-            raise NotImplementedError("the channel count must be a multiple of 256 up to 4096")
-        _lib.check(rc, "hb_adaln_residual_int8")
-        return
     with torch.cuda.device(dev):
         rc = _lib.lib().hb_adaln_residual(
             _lib.ptr(x), x_rs, _lib.ptr(y) if y is not None else None, strides.get("y", 0),
@@ -113,26 +100,63 @@ def gate_residual_adaln(x, y, gate, shift, scale, eps=1e-6, out=None):
     return x, h
 
 
-def _check_inference(*tensors):
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+def _call_int8(x, y, gate, shift, scale, x_out, eps):
+    """``hb_adaln_residual_int8``: the modulated rows quantised per token."""
+    if not x.is_cuda:
+        raise ValueError("CUDA tensors required")
+    kind, dev = x.dtype, x.device
+    if kind not in _DTYPES:
+        raise ValueError("x must be float16 or bfloat16")
+    x3, x_rs, B, S = _rows(x, "x")
+    C = x3.shape[-1]
+    mods = (shift, scale) if gate is None else (shift, scale, gate)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, y, *mods)):
         raise ValueError("Inference only; disable autograd")
+    mod_bs = _mod(shift, B, C, x, "shift")[1]
+    for name, m in zip(("scale", "gate"), mods[1:]):
+        if _mod(m, B, C, x, name)[1] != mod_bs:
+            raise ValueError("gate, shift and scale must share one batch stride")
+    y_rs = xo_rs = 0
+    if y is not None:
+        for name, t in (("y", y), ("x_out", x_out)):
+            if t.shape != x.shape or t.dtype != kind or t.device != dev:
+                raise ValueError(f"{name} must match x's shape, dtype and device")
+        y_rs, xo_rs = _rows(y, "y")[1], _rows(x_out, "x_out")[1]
+        if x_out is not x:
+            _check_apart(x_out, x, y, *mods)
+    rows = _empty_rows(x.shape, kind, dev)
+    with torch.cuda.device(dev) if dev.index != torch.cuda.current_device() else _lib.SAME_DEVICE:
+        rc = _lib.lib().hb_adaln_residual_int8(
+            x.data_ptr(), x_rs, None if y is None else y.data_ptr(), y_rs, None if y is None else gate.data_ptr(),
+            shift.data_ptr(), scale.data_ptr(), mod_bs, None if y is None else x_out.data_ptr(), xo_rs,
+            rows.values.data_ptr(), rows.row_stride, rows.scales.data_ptr(), B * S, max(S, 1), C, eps, _DTYPES[kind],
+            _lib.stream_handle(dev))
+    if rc == _lib.HB_ERR_UNSUPPORTED:
+        raise NotImplementedError("the channel count must be a multiple of 256 up to 4096")
+    if rc == _lib.HB_ERR_ALIGN:
+        raise ValueError("rows and modulation vectors must start on 16-byte boundaries")
+    _lib.check(rc, "hb_adaln_residual_int8")
+    return rows
+
+
+def _check_apart(out, *inputs):
+    """``out`` is x itself elsewhere; here it must share no memory with what is read."""
+    begin, end = _span(out)
+    for t in inputs:
+        first, last = _span(t)
+        if begin < last and first < end:
+            raise ValueError("x_out must be x itself or apart from every input")
 
 
 def adaln_int8(x, shift, scale, eps=1e-6):
     """``Int8Rows`` of LayerNorm(x) * (1 + scale) + shift, quantised from its fp32 values."""
-    _check_inference(x, shift, scale)
-    rows = _empty_rows(x.shape, x.dtype, x.device)
-    _call(x, None, None, shift, scale, None, None, eps, rows)
-    return rows
+    return _call_int8(x, None, None, shift, scale, None, eps)
 
 
 def gate_residual_adaln_int8(x, y, gate, shift, scale, eps=1e-6, x_out=None):
     """(x, rows): x += gate * y (into ``x_out`` if given) and ``adaln_int8`` of the new stream."""
-    _check_inference(x, y, gate, shift, scale)
     x_out = x if x_out is None else x_out
-    rows = _empty_rows(x.shape, x.dtype, x.device)
-    _call(x, y, gate, shift, scale, x_out, None, eps, rows)
-    return x_out, rows
+    return x_out, _call_int8(x, y, gate, shift, scale, x_out, eps)
 
 
 class NativeBlockOps:

@@ -288,34 +288,30 @@ int launch_norm_rope_qk(const QkParams& p, int D, int grid, cudaStream_t st) {
 
 using namespace hb;
 
-extern "C" int hb_norm_rope_qk(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
-                               void* q_out, const int64_t* q_out_strides, void* k_out, const int64_t* k_out_strides,
-                               int B, int S, int T, int Hq, int Hk, int D, const void* w_q, const void* w_k,
-                               const void* w_txt_q, const void* w_txt_k, float eps, const float* cos, const float* sin,
-                               int dtype, void* stream) {
+extern "C" int hb_norm_rope_qk(const void* q, const void* k, void* q_out, void* k_out, const int64_t* strides, int B, int S,
+                               int T, int Hq, int Hk, int D, const void* w_q, const void* w_k, const void* w_txt_q,
+                               const void* w_txt_k, float eps, const float* cos, const float* sin, int dtype, void* stream) {
     if (B < 0 || S < 0 || Hq <= 0 || Hk <= 0 || T < 0 || T > S || !(eps >= 0.f)) return HB_ERR_ARG;
     if (D != 32 && D != 64 && D != 128 && D != 256) return HB_ERR_UNSUPPORTED;
     if (dtype != 0 && dtype != 1) return HB_ERR_UNSUPPORTED;
     if (B == 0 || S == 0) return HB_OK;
-    if (!q || !k || !q_out || !k_out || !q_strides || !k_strides || !q_out_strides || !k_out_strides || !w_q || !w_k ||
-        !cos || !sin || (T > 0 && (!w_txt_q || !w_txt_k)))
+    if (!q || !k || !q_out || !k_out || !strides || !w_q || !w_k || !cos || !sin || (T > 0 && (!w_txt_q || !w_txt_k)))
         return HB_ERR_ARG;
     // 16-byte vector accesses: every row start and stride must keep them aligned
     for (const void* ptr : {q, k, (const void*)q_out, (const void*)k_out, w_q, w_k, T > 0 ? w_txt_q : w_q,
                             T > 0 ? w_txt_k : w_k, (const void*)cos, (const void*)sin})
         if (reinterpret_cast<uintptr_t>(ptr) & 15) return HB_ERR_ALIGN;
-    const int64_t* strides[4] = {q_strides, k_strides, q_out_strides, k_out_strides};
-    for (const int64_t* st : strides)
-        for (int i = 0; i < 3; i++)
-            if (st[i] % 8) return HB_ERR_ALIGN;
+    for (int i = 0; i < 12; i++)
+        if (strides[i] % 8) return HB_ERR_ALIGN;
     QkParams p;
     const void* in[2] = {q, k};
     void* out[2] = {q_out, k_out};
     for (int i = 0; i < 2; i++) {
         p.x[i] = in[i];
         p.out[i] = out[i];
-        p.x_sb[i] = strides[i][0], p.x_sn[i] = strides[i][1], p.x_sh[i] = strides[i][2];
-        p.o_sb[i] = strides[2 + i][0], p.o_sn[i] = strides[2 + i][1], p.o_sh[i] = strides[2 + i][2];
+        const int64_t *x = strides + 3 * i, *o = strides + 6 + 3 * i;
+        p.x_sb[i] = x[0], p.x_sn[i] = x[1], p.x_sh[i] = x[2];
+        p.o_sb[i] = o[0], p.o_sn[i] = o[1], p.o_sh[i] = o[2];
     }
     p.H[0] = Hq, p.H[1] = Hk;
     p.w[0] = w_q, p.w[1] = w_k;

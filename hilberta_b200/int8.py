@@ -94,9 +94,12 @@ class Int8Rows:
 def _empty_rows(shape, dtype, device):
     K = shape[-1]
     pitch = -(-K // 16) * 16
-    values = torch.empty(*shape[:-1], pitch, dtype=torch.int8, device=device)
-    return Int8Rows(values if pitch == K else values[..., :K], torch.empty(shape[:-1], dtype=torch.float32, device=device),
-                    dtype)
+    values = torch.empty((*shape[:-1], pitch), dtype=torch.int8, device=device)
+    rows = object.__new__(Int8Rows)  # right by construction: none of the checks of Int8Rows(...)
+    rows.values = values if pitch == K else values[..., :K]
+    rows.scales = torch.empty(shape[:-1], dtype=torch.float32, device=device)
+    rows.dtype, rows.row_stride = dtype, pitch
+    return rows
 
 
 def _check_source(x, what):
@@ -140,7 +143,7 @@ def quantize_rows(x, *, joined=None):
     with _on(x.device):
         rc = _lib.lib().hb_quantize_rows(
             x.data_ptr(), x_rs, ka, None if joined is None else joined.data_ptr(), j_rs, kb, rows, out.values.data_ptr(),
-            out.row_stride, out.scales.data_ptr(), _DTYPES[x.dtype], torch.cuda.current_stream(x.device).cuda_stream)
+            out.row_stride, out.scales.data_ptr(), _DTYPES[x.dtype], _lib.stream_handle(x.device))
     _lib.check(rc, "hb_quantize_rows")
     return out
 
@@ -223,7 +226,7 @@ def _product(x, weight, bias, act, out):
     tail = (weight.values.data_ptr(), weight.row_stride, weight.scales.data_ptr(), None if bias is None else bias.data_ptr(),
             out.data_ptr(), out_rs, M, N, K, act, _DTYPES[x.dtype])
     with _on(dev):
-        stream = torch._C._cuda_getCurrentRawStream(dev.index)
+        stream = _lib.stream_handle(dev)
         if coded:
             rc = lib.hb_int8_linear(x.values.data_ptr(), x_rs, x.scales.data_ptr(), *tail, stream)
         else:

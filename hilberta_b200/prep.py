@@ -104,8 +104,7 @@ def prepare_qkv(q_txt, k_txt, v_txt, q_img, k_img, v_img, *, heads, norm_q, norm
     return q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2)
 
 
-def _strides3(t):
-    return (ctypes.c_int64 * 3)(*t.stride()[:3])
+_Strides = ctypes.c_int64 * 12
 
 
 def _bytes(t):
@@ -127,13 +126,13 @@ def norm_rope_qk(q, k, *, weight_q, weight_k, cos, sin, text_tokens=0, weight_tx
     one rounding at the end (``norm_rope_pack`` keeps the rounding of the separate
     ops it replaces).  ``out`` is a pair of tensors like q and k, ``(q, k)`` itself
     for in place; by default new contiguous ones.  Returns the pair."""
-    for name, x in (("q", q), ("k", k)):
-        if x.ndim != 4 or not x.is_cuda or x.stride(-1) != 1:
-            raise ValueError(f"{name} must be a CUDA tensor [B, S, heads, D] with contiguous D")
+    if q.ndim != 4 or k.ndim != 4 or not q.is_cuda or q.stride(3) != 1 or k.stride(3) != 1:
+        raise ValueError("q and k must be CUDA tensors [B, S, heads, D] with contiguous D")
+    kind, dev = q.dtype, q.device
     dtype = _dtype_code(q)
     B, S, Hq, D = q.shape
     Hk = k.shape[2]
-    if k.shape[:2] != (B, S) or k.shape[3] != D or k.dtype != q.dtype or k.device != q.device:
+    if k.shape != (B, S, Hk, D) or k.dtype != kind or k.device != dev:
         raise ValueError("q and k must agree in batch, tokens, D, dtype and device")
     if Hq < 1 or Hk < 1:
         raise ValueError("at least one query and one key head required")
@@ -142,29 +141,30 @@ def norm_rope_qk(q, k, *, weight_q, weight_k, cos, sin, text_tokens=0, weight_tx
         raise ValueError("text_tokens must lie within the tokens")
     if T > 0 and (weight_txt_q is None or weight_txt_k is None):
         raise ValueError("text tokens need weight_txt_q and weight_txt_k")
-    for w in (weight_q, weight_k, weight_txt_q, weight_txt_k):
-        if w is not None and (w.shape != (D,) or w.dtype != q.dtype or w.device != q.device or not w.is_contiguous()):
+    weights = [w for w in (weight_q, weight_k, weight_txt_q, weight_txt_k) if w is not None]
+    for w in weights:
+        if w.shape != (D,) or w.dtype != kind or w.device != dev or (D > 1 and w.stride(0) != 1):
             raise ValueError("norm weights must be contiguous [D] in the heads' dtype")
     for c in (cos, sin):
-        if c.shape != (S, D) or c.dtype != torch.float32 or c.device != q.device or not c.is_contiguous():
+        if c.shape != (S, D) or c.dtype != torch.float32 or c.device != dev or not c.is_contiguous():
             raise ValueError("cos/sin must be contiguous fp32 [S, D] on the heads' device")
     if not eps >= 0:
         raise ValueError("eps must not be negative")
-    if torch.is_grad_enabled() and any(
-            t is not None and t.requires_grad for t in (q, k, weight_q, weight_k, weight_txt_q, weight_txt_k, cos, sin)):
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, cos, sin, *weights)):
         raise ValueError("Inference only; disable autograd")
     if out is None:
-        out = tuple(torch.empty(x.shape, dtype=q.dtype, device=q.device) for x in (q, k))
+        q_out = torch.empty((B, S, Hq, D), dtype=kind, device=dev)
+        k_out = torch.empty((B, S, Hk, D), dtype=kind, device=dev)
     else:
-        _check_qk_out(q, k, out, (weight_q, weight_k, weight_txt_q, weight_txt_k, cos, sin))
-    q_out, k_out = out
-    dev = q.device
+        _check_qk_out(q, k, out, (cos, sin, *weights))
+        q_out, k_out = out
+    strides = _Strides(*q.stride()[:3], *k.stride()[:3], *q_out.stride()[:3], *k_out.stride()[:3])
     with torch.cuda.device(dev) if dev.index != torch.cuda.current_device() else _lib.SAME_DEVICE:
         rc = _lib.lib().hb_norm_rope_qk(
-            q.data_ptr(), _strides3(q), k.data_ptr(), _strides3(k), q_out.data_ptr(), _strides3(q_out), k_out.data_ptr(),
-            _strides3(k_out), B, S, T, Hq, Hk, D, weight_q.data_ptr(), weight_k.data_ptr(), _lib.ptr(weight_txt_q),
-            _lib.ptr(weight_txt_k), float(eps), cos.data_ptr(), sin.data_ptr(), dtype,
-            torch.cuda.current_stream(dev).cuda_stream)
+            q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr(), strides, B, S, T, Hq, Hk, D,
+            weight_q.data_ptr(), weight_k.data_ptr(), None if weight_txt_q is None else weight_txt_q.data_ptr(),
+            None if weight_txt_k is None else weight_txt_k.data_ptr(), eps, cos.data_ptr(), sin.data_ptr(), dtype,
+            _lib.stream_handle(dev))
     if rc == _lib.HB_ERR_ALIGN:
         raise ValueError("hb_norm_rope_qk needs 16-byte aligned rows (strides multiples of 8 elements)")
     if rc == _lib.HB_ERR_UNSUPPORTED:
@@ -192,7 +192,7 @@ def _check_qk_out(q, k, out, others):
     for o, in_place, own in ((q_out, same[0], q), (k_out, same[1], k)):
         begin, end = _bytes(o)
         for t in (q, k, *others, *(x for x in out if x is not o)):
-            if t is None or (in_place and t is own):
+            if in_place and t is own:
                 continue
             first, last = _bytes(t)
             if begin < last and first < end and not (t.dtype == o.dtype and _interleaved(o, t)):

@@ -370,16 +370,16 @@ int hb_adaln_residual_int8(const void* x, int64_t x_rs, const void* y, int64_t y
 /* Query and key heads after the projections, both in one launch: RMS-normalise
  * every (token, head) row over D with a learned weight (tokens before T use the
  * w_txt weights), then rotate pairs (2i, 2i+1) by cos/sin (fp32 [S][D], indexed by
- * token).  q [B][S][Hq][D], k [B][S][Hk][D], 16-bit, element strides (b, s, h),
- * D contiguous; outputs likewise (q_out == q with equal strides: in place).  fp32
- * arithmetic, one rounding at the end (hb_norm_rope_pack rounds after each step,
- * as the separate ops it replaces do).  w_txt_*: NULL when T is 0.  Pointers
- * 16-byte aligned, strides multiples of 8 elements; D 32, 64, 128 or 256. */
-int hb_norm_rope_qk(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
-                    void* q_out, const int64_t* q_out_strides, void* k_out,
-                    const int64_t* k_out_strides, int B, int S, int T, int Hq, int Hk, int D,
-                    const void* w_q, const void* w_k, const void* w_txt_q, const void* w_txt_k,
-                    float eps, const float* cos, const float* sin, int dtype, void* stream);
+ * token).  q [B][S][Hq][D], k [B][S][Hk][D], 16-bit, D contiguous, element strides
+ * strides[t*3 + {0,1,2}] = (b, s, h) for t = 0 q, 1 k, 2 q_out, 3 k_out (q_out == q
+ * with equal strides: in place).  fp32 arithmetic, one rounding at the end
+ * (hb_norm_rope_pack rounds after each step, as the separate ops it replaces do).
+ * w_txt_*: NULL when T is 0.  Pointers 16-byte aligned, strides multiples of 8
+ * elements; D 32, 64, 128 or 256. */
+int hb_norm_rope_qk(const void* q, const void* k, void* q_out, void* k_out, const int64_t* strides,
+                    int B, int S, int T, int Hq, int Hk, int D, const void* w_q, const void* w_k,
+                    const void* w_txt_q, const void* w_txt_k, float eps, const float* cos,
+                    const float* sin, int dtype, void* stream);
 
 /* ---- allocation-free variant of hb_paired_fwd --------------------------- */
 /* No counterpart in the reference: an addition for callers that must not

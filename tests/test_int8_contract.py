@@ -91,11 +91,9 @@ def test_adaln_residual_int8_checks(lib):
 def test_norm_rope_qk_checks(lib):
     from hilberta_b200 import _lib
 
-    st = lambda *v: (ctypes.c_int64 * 3)(*v)  # noqa: E731
-
     def call(q=F, k=F, qo=F, ko=F, B=1, S=4, T=0, Hq=2, Hk=1, D=64, wq=F, wtq=None, cos=F, sn=128, eps=1e-6, dtype=1):
-        s = st(4 * sn, sn, 64)
-        return lib.hb_norm_rope_qk(q, s, k, s, qo, s, ko, s, B, S, T, Hq, Hk, D, wq, F, wtq, wtq, eps, cos, F, dtype, None)
+        strides = (ctypes.c_int64 * 12)(*[4 * sn, sn, 64] * 4)
+        return lib.hb_norm_rope_qk(q, k, qo, ko, strides, B, S, T, Hq, Hk, D, wq, F, wtq, wtq, eps, cos, F, dtype, None)
 
     for bad in (dict(q=None), dict(k=None), dict(qo=None), dict(ko=None), dict(B=-1), dict(S=-1), dict(T=5), dict(T=-1),
                 dict(T=2), dict(Hq=0), dict(Hk=0), dict(wq=None), dict(cos=None), dict(eps=-1.0)):
