@@ -20,10 +20,12 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
 #include <cstdint>
 
 #include "common.cuh"
 #include "int8_codes.cuh"
+#include "sm100_ptx.cuh"
 
 namespace hb {
 namespace {
@@ -172,107 +174,227 @@ struct AdaInt8Params {
     float* scales;  // [rows]
 };
 
-// The same pass with h quantised instead of rounded to 16 bits: one warp per row,
-// the row's h formed twice from the registers (once for its largest magnitude,
-// once for its codes), so the int8 product reads half the bytes and no separate
-// pass over h exists.  Memory-bound: 2 C (4 C with the residual) bytes read and
-// C (3 C) written per row.
-template <bool BF16, bool RESIDUAL>
-__global__ void __launch_bounds__(256) k_adaln_int8(const __grid_constant__ AdaInt8Params q) {
-    using V = Vec8<BF16>;
-    using T = typename V::T;
+// Pairs of fp32 values in one register pair (two operations per instruction).
+template <bool BF16>
+struct Pairs {
+    static __device__ __forceinline__ void unpack(const uint4& u, uint64_t (&f)[4]) {
+        float v[8];
+        Vec8<BF16>::load(&u, v);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = ptx::f2_pack(v[2 * i], v[2 * i + 1]);
+    }
+    static __device__ __forceinline__ uint4 pack(const uint64_t (&f)[4]) {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ptx::f2_unpack(f[i], v[2 * i], v[2 * i + 1]);
+        return Vec8<BF16>::pack(v);
+    }
+};
+// max(|a|, |b|, m); NaN when any of them is (so a NaN in a row is never lost).
+__device__ __forceinline__ float max_abs(uint64_t pair, float m) {
+    float a, b, d;
+    ptx::f2_unpack(pair, a, b);
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(fabsf(a)), "f"(fabsf(b)), "f"(m));
+    return d;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+
+// The same pass with h quantised instead of rounded to 16 bits, so that the int8
+// product reads half the bytes and no separate pass over h exists.  T threads per
+// row (a warp, or a CTA of four), NV vectors of 8 elements each: row, modulation
+// and h stay in registers.  Memory-bound by its bytes (2 C, 4 C with the residual,
+// read and C, 3 C written per row), but only just: the instructions per element
+// and the block-wide reductions per row are kept few.  Few threads per row with
+// many elements each share the reductions' cost; two fp32 operations go in one
+// instruction; mean and variance come from one reduction; the CTAs are persistent,
+// keep the modulation of their batch entry and fetch DEPTH rows ahead.
+//
+// Mean and variance: a lane forms the mean m of its n elements and the sum d of
+// their squared deviations from m; two sets of n elements merge into
+//   mean (ma + mb) / 2,  deviations da + db + (ma - mb)^2 n / 2,
+// which never subtracts large sums.  The lanes of a warp hold equally many
+// elements (C is a multiple of 256); warps are joined by their counts.
+template <bool BF16, bool RESIDUAL, int T, int NV, int DEPTH>
+__global__ void __launch_bounds__(128) k_adaln_int8(const __grid_constant__ AdaInt8Params q) {
+    using namespace ptx;
+    using P = Pairs<BF16>;
+    using E = typename Vec8<BF16>::T;
+    constexpr int RPC = 128 / T;
+    __shared__ float2 s_stat[4];
+    __shared__ float s_mag[4];
     const AdaParams& p = q.a;
-    const int lane = threadIdx.x & 31;
-    const int row = blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (row >= p.rows) return;  // whole warps leave together
-    const int b = row / p.rows_per_batch;
-    const int nv = p.C >> 8;
-    const T* x = static_cast<const T*>(p.x) + row * p.x_rs;
-    uint4 xv[kMaxVec];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int t = threadIdx.x % T, row_warp = t >> 5;
+    const int groups = p.C >> 8;  // 32 vectors each, dealt to the row's warps in turn
+    const int cnt = (groups - row_warp + T / 32 - 1) / (T / 32);  // this warp's
+    const int step = gridDim.x * RPC;
+    const float n = 8.f * cnt, inv_n = 1.f / n, inv_c = 1.f / static_cast<float>(p.C);
+    uint4 x[DEPTH][NV], y[DEPTH][NV];
+    auto fetch = [&](int row, uint4 (&x)[NV], uint4 (&y)[NV]) {
+        if (row >= p.rows) return;
+        const E* px = static_cast<const E*>(p.x) + row * p.x_rs + 8 * t;
+        const E* py = static_cast<const E*>(p.y) + row * p.y_rs + 8 * t;
 #pragma unroll
-    for (int i = 0; i < kMaxVec; ++i)
-        if (i < nv) xv[i] = *reinterpret_cast<const uint4*>(x + 8 * (lane + 32 * i));
-    if constexpr (RESIDUAL) {
-        const T* y = static_cast<const T*>(p.y) + row * p.y_rs;
-        const T* g = static_cast<const T*>(p.gate) + b * p.mod_bs;
-        T* xo = static_cast<T*>(p.x_out) + row * p.xo_rs;
-#pragma unroll
-        for (int i = 0; i < kMaxVec; ++i) {
-            if (i < nv) {
-                const int c = 8 * (lane + 32 * i);
-                float fx[8], fy[8], fg[8];
-                V::load(&xv[i], fx);
-                V::load(y + c, fy);
-                V::load(g + c, fg);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) fx[e] = fmaf(fg[e], fy[e], fx[e]);
-                xv[i] = V::pack(fx);  // the stored residual stream, rounded
-                *reinterpret_cast<uint4*>(xo + c) = xv[i];
+        for (int i = 0; i < NV; ++i) {
+            if (i < cnt) {
+                x[i] = *reinterpret_cast<const uint4*>(px + 8 * i * T);
+                if constexpr (RESIDUAL) y[i] = *reinterpret_cast<const uint4*>(py + 8 * i * T);
             }
         }
-    }
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < kMaxVec; ++i) {
-        if (i < nv) {
-            float f[8];
-            V::load(&xv[i], f);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) s += f[e];
-        }
-    }
-    const float inv_c = 1.f / static_cast<float>(p.C);
-    const float mean = warp_sum(s) * inv_c;
-    float v = 0.f;
-#pragma unroll
-    for (int i = 0; i < kMaxVec; ++i) {
-        if (i < nv) {
-            float f[8];
-            V::load(&xv[i], f);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float d = f[e] - mean;
-                v = fmaf(d, d, v);
-            }
-        }
-    }
-    const float rstd = rsqrtf(warp_sum(v) * inv_c + p.eps);
-    const T* sh = static_cast<const T*>(p.shift) + b * p.mod_bs;
-    const T* sc = static_cast<const T*>(p.scale) + b * p.mod_bs;
-    auto modulated = [&](int i, float (&f)[8]) {
-        const int c = 8 * (lane + 32 * i);
-        float fs[8], fc[8];
-        V::load(&xv[i], f);
-        V::load(sh + c, fs);
-        V::load(sc + c, fc);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = fmaf((f[e] - mean) * rstd, 1.f + fc[e], fs[e]);
     };
-    uint32_t mag = 0;  // magnitude bits: NaN sorts above infinity above every number
+    uint64_t shift[NV][4], scale[NV][4];
+    uint4 gate[NV];
+    int batch_end = 0, batch = -1;  // modulation of rows [.., batch_end)
+    const uint64_t one = f2_pack(1.f, 1.f), magic = f2_pack(12582912.f, 12582912.f);
+    auto work = [&](int row, uint4 (&x)[NV], uint4 (&y)[NV]) {
+        if (row >= batch_end) {
+            batch = row / p.rows_per_batch;
+            batch_end = (batch + 1) * p.rows_per_batch;
+            const int64_t at = batch * p.mod_bs + 8 * t;
 #pragma unroll
-    for (int i = 0; i < kMaxVec; ++i) {
-        if (i < nv) {
-            float f[8];
-            modulated(i, f);
+            for (int i = 0; i < NV; ++i) {
+                if (i < cnt) {
+                    P::unpack(*reinterpret_cast<const uint4*>(static_cast<const E*>(p.shift) + at + 8 * i * T), shift[i]);
+                    P::unpack(*reinterpret_cast<const uint4*>(static_cast<const E*>(p.scale) + at + 8 * i * T), scale[i]);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) mag = max(mag, __float_as_uint(f[e]) & 0x7fffffffu);
+                    for (int e = 0; e < 4; ++e) scale[i][e] = f2_add(scale[i][e], one);
+                    if constexpr (RESIDUAL)
+                        gate[i] = *reinterpret_cast<const uint4*>(static_cast<const E*>(p.gate) + at + 8 * i * T);
+                }
+            }
+        }
+        uint64_t f[NV][4], sum = 0;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            if (i < cnt) {
+                P::unpack(x[i], f[i]);
+                if constexpr (RESIDUAL) {
+                    uint64_t fy[4], fg[4];
+                    P::unpack(y[i], fy);
+                    P::unpack(gate[i], fg);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) f[i][e] = f2_fma(fg[e], fy[e], f[i][e]);
+                    const uint4 stream = P::pack(f[i]);  // the stored residual stream, rounded
+                    *reinterpret_cast<uint4*>(static_cast<E*>(p.x_out) + row * p.xo_rs + 8 * (t + i * T)) = stream;
+                    P::unpack(stream, f[i]);
+                }
+                sum = f2_add(sum, f2_add(f2_add(f[i][0], f[i][1]), f2_add(f[i][2], f[i][3])));
+            }
+        }
+        fetch(row + DEPTH * step, x, y);
+        float a, b;
+        f2_unpack(sum, a, b);
+        float mean = (a + b) * inv_n;
+        uint64_t dev = 0;
+        const uint64_t minus = f2_pack(-mean, -mean);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            if (i < cnt) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint64_t d = f2_add(f[i][e], minus);
+                    dev = f2_fma(d, d, dev);
+                }
+            }
+        }
+        f2_unpack(dev, a, b);
+        float d = a + b, size = 0.5f * n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1, size *= 2.f) {
+            const float m2 = __shfl_xor_sync(0xffffffffu, mean, o), d2 = __shfl_xor_sync(0xffffffffu, d, o);
+            const float delta = m2 - mean;
+            d = fmaf(delta * delta, size, d + d2);
+            mean = 0.5f * (mean + m2);
+        }
+        if constexpr (T > 32) {
+            if (lane == 0) s_stat[warp] = make_float2(mean, d);
+            __syncthreads();
+            mean = d = 0.f;
+#pragma unroll
+            for (int w = 0; w < T / 32; ++w) mean = fmaf(256.f * ((groups - w + T / 32 - 1) / (T / 32)), s_stat[w].x, mean);
+            mean *= inv_c;
+#pragma unroll
+            for (int w = 0; w < T / 32; ++w) {
+                const float delta = s_stat[w].x - mean;
+                d = fmaf(delta * delta, 256.f * ((groups - w + T / 32 - 1) / (T / 32)), d + s_stat[w].y);
+            }
+        }
+        const float rstd = rsqrtf(fmaf(d, inv_c, p.eps));
+        const uint64_t r2 = f2_pack(rstd, rstd), m2 = f2_pack(-mean, -mean);
+        float mag = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            if (i < cnt) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    f[i][e] = f2_fma(f2_mul(f2_add(f[i][e], m2), r2), scale[i][e], shift[i][e]);
+                    mag = max_abs(f[i][e], mag);
+                }
+            }
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) mag = max_nan(mag, __shfl_xor_sync(0xffffffffu, mag, o));
+        if constexpr (T > 32) {
+            if (lane == 0) s_mag[warp] = mag;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < T / 32; ++w) mag = max_nan(mag, s_mag[w]);
+        }
+        const RowScale rs = row_scale(mag);
+        if (t == 0) q.scales[row] = rs.scale;
+        const uint64_t inv2 = f2_pack(rs.inv, rs.inv);
+        int8_t* out = q.codes + row * q.c_rs + 8 * t;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            if (i < cnt) {
+                uint32_t c[8];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {  // code_bits, two at a time
+                    f2_unpack(f2_add(f2_mul(f[i][e], inv2), magic), a, b);
+                    c[2 * e] = __float_as_uint(a);
+                    c[2 * e + 1] = __float_as_uint(b);
+                }
+                uint2 o = make_uint2(pack_codes(c[0], c[1], c[2], c[3]), pack_codes(c[4], c[5], c[6], c[7]));
+                if (!rs.live) o = make_uint2(0, 0);
+                *reinterpret_cast<uint2*>(out + 8 * i * T) = o;
+            }
+        }
+    };
+    int row = blockIdx.x * RPC + threadIdx.x / T;
+#pragma unroll
+    for (int k = 0; k < DEPTH; ++k) fetch(row + k * step, x[k], y[k]);
+    while (row < p.rows) {  // the same for all threads of a row
+#pragma unroll
+        for (int k = 0; k < DEPTH; ++k) {
+            if (row < p.rows) work(row, x[k], y[k]);
+            row += step;
         }
     }
-    const RowScale rs = row_scale(__uint_as_float(__reduce_max_sync(0xffffffffu, mag)));
-    if (lane == 0) q.scales[row] = rs.scale;
-    int8_t* out = q.codes + row * q.c_rs;
-#pragma unroll
-    for (int i = 0; i < kMaxVec; ++i) {
-        if (i < nv) {
-            float f[8];
-            modulated(i, f);
-            uint32_t c[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) c[e] = rs.live ? code_bits(f[e], rs.inv) : 0u;
-            *reinterpret_cast<uint2*>(out + 8 * (lane + 32 * i)) =
-                make_uint2(pack_codes(c[0], c[1], c[2], c[3]), pack_codes(c[4], c[5], c[6], c[7]));
-        }
-    }
+}
+
+template <bool BF16, bool RESIDUAL, int T, int NV>
+int launch_adaln_int8(const AdaInt8Params& p, int sms, cudaStream_t st) {
+    constexpr int DEPTH = RESIDUAL ? 1 : 2;  // the residual's second stream doubles what is in flight
+    constexpr int CTAS = RESIDUAL ? 3 : 4;   // per SM, by registers
+    const int64_t groups = ceil_div(p.a.rows, 128 / T);
+    const unsigned grid = (unsigned)std::min<int64_t>(groups, (int64_t)CTAS * sms);
+    k_adaln_int8<BF16, RESIDUAL, T, NV, DEPTH><<<grid, 128, 0, st>>>(p);
+    HB_LAUNCH_CHECK();
+    return HB_OK;
+}
+
+template <bool BF16, bool RESIDUAL>
+int launch_adaln_int8(const AdaInt8Params& p, cudaStream_t st) {
+    int dev = 0, sms = 0;
+    HB_CUDA_TRY(cudaGetDevice(&dev));
+    HB_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+    if (p.a.C <= 1024) return launch_adaln_int8<BF16, RESIDUAL, 32, 4>(p, sms, st);
+    if (p.a.C <= 3072) return launch_adaln_int8<BF16, RESIDUAL, 128, 3>(p, sms, st);
+    return launch_adaln_int8<BF16, RESIDUAL, 128, 4>(p, sms, st);
 }
 
 template <bool BF16>
@@ -334,19 +456,7 @@ extern "C" int hb_adaln_residual_int8(const void* x, int64_t x_rs, const void* y
     if (rows == 0) return HB_OK;
     const AdaInt8Params p{{x, y, gate, shift, scale, x_out, nullptr, x_rs, y_rs, xo_rs, 0, mod_bs, rows, rows_per_batch, C, eps},
                           codes, codes_rs, scales};
-    const dim3 grid((rows + 7) / 8), block(256);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (dtype == 1) {
-        if (y)
-            k_adaln_int8<true, true><<<grid, block, 0, st>>>(p);
-        else
-            k_adaln_int8<true, false><<<grid, block, 0, st>>>(p);
-    } else {
-        if (y)
-            k_adaln_int8<false, true><<<grid, block, 0, st>>>(p);
-        else
-            k_adaln_int8<false, false><<<grid, block, 0, st>>>(p);
-    }
-    HB_LAUNCH_CHECK();
-    return HB_OK;
+    if (dtype == 1) return y ? launch_adaln_int8<true, true>(p, st) : launch_adaln_int8<true, false>(p, st);
+    return y ? launch_adaln_int8<false, true>(p, st) : launch_adaln_int8<false, false>(p, st);
 }

@@ -83,91 +83,137 @@ struct QuantParams {
     float* scales;  // [rows]
 };
 
-// Eight values of a row from column c.  VEC: rows start on 16 bytes and ka and k
-// are multiples of 8; otherwise element by element (zeros past the end).
-template <bool VEC>
-__device__ __forceinline__ uint4 load8(const QuantParams& p, int64_t row, int c) {
+// Thread t of T's share i of a row: eight values, and where their codes go.  VEC
+// (rows start on 16 bytes, ka and k are multiples of 8): neighbours, in one 16-byte
+// load and one 8-byte store.  Otherwise every T-th value, so that a warp's 2-byte
+// loads and 1-byte stores are contiguous.  Zeros past the end of the row.
+template <bool VEC, int T>
+__device__ __forceinline__ uint4 load8(const QuantParams& p, int64_t row, int t, int i) {
     if constexpr (VEC) {
+        const int c = 8 * (t + i * T);
+        if (c >= p.k || row >= p.rows) return make_uint4(0, 0, 0, 0);
         const uint16_t* src = c < p.ka ? p.a + row * p.a_rs + c : p.b + row * p.b_rs + (c - p.ka);
         return *reinterpret_cast<const uint4*>(src);
     } else {
-        uint32_t w[4];
+        uint32_t w[8];
+        const uint16_t *a = p.a + row * p.a_rs, *b = p.b + row * p.b_rs;
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            uint32_t e[2];
-#pragma unroll
-            for (int j = 0; j < 2; j++) {
-                const int x = c + 2 * i + j;
-                e[j] = x < p.ka ? p.a[row * p.a_rs + x] : (x < p.k ? p.b[row * p.b_rs + (x - p.ka)] : 0);
-            }
-            w[i] = e[0] | (e[1] << 16);
+        for (int e = 0; e < 8; e++) {
+            const int c = 8 * i * T + e * T + t;
+            const uint16_t* src = c < p.ka ? a + c : b + (c - p.ka);
+            w[e] = 0;
+            if (c < p.k && row < p.rows) w[e] = __ldg(src);
         }
-        return make_uint4(w[0], w[1], w[2], w[3]);
+        return make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
+    }
+}
+template <bool VEC, int T>
+__device__ __forceinline__ void store8(const QuantParams& p, int64_t row, int t, int i, uint2 codes) {
+    int8_t* out = p.codes + row * p.c_rs;
+    if constexpr (VEC) {
+        const int c = 8 * (t + i * T);
+        if (c < p.k) *reinterpret_cast<uint2*>(out + c) = codes;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const int c = 8 * i * T + e * T + t;
+            if (c < p.k) out[c] = (int8_t)((e < 4 ? codes.x : codes.y) >> (8 * (e & 3)));
+        }
     }
 }
 
-// T threads per row (several rows per CTA when T = 32), the row read once and
-// held in registers between its maximum and its codes: up to 8 vectors of 8
-// values a thread; longer rows read the rest again.
+__device__ __forceinline__ uint32_t max_mag(uint32_t m, const uint4& v) {
+    return max_mag(max_mag(max_mag(max_mag(m, v.x), v.y), v.z), v.w);
+}
+template <bool BF16>
+__device__ __forceinline__ uint2 codes8(const uint4& v, const RowScale& s) {
+    if (!s.live) return make_uint2(0, 0);
+    return make_uint2(codes4<BF16>(v.x, v.y, s.inv), codes4<BF16>(v.z, v.w, s.inv));
+}
+
+// T threads per row (a warp, or the whole CTA), up to kQuantVec vectors of 8
+// values each: the row is read once and stays in registers between its maximum
+// and its codes.  Memory-bound (2 K bytes read, K written per row): CTAs are
+// persistent and each thread fetches its part of the next row before it works on
+// this one, so loads are in flight through the reduction and the stores.
+constexpr int kQuantVec = 4;
+
 template <bool BF16, bool VEC, int T>
 __global__ void __launch_bounds__(T < 128 ? 128 : T) k_quantize_rows(const __grid_constant__ QuantParams p) {
     constexpr int CTA = T < 128 ? 128 : T;
     constexpr int RPC = CTA / T;
-    constexpr int NV = 8;
-    __shared__ uint32_t s_max[CTA / 32];
+    constexpr int NV = kQuantVec;
+    __shared__ uint32_t s_max[2][CTA / 32];
     const int t = threadIdx.x % T;
-    const int64_t row = (int64_t)blockIdx.x * RPC + threadIdx.x / T;
-    if (row >= p.rows) return;  // whole warps; RPC > 1 has no block barrier
-    const int nv = (p.k + 7) / 8;
-    uint4 v[NV];
-    uint32_t m = 0;
+    const int64_t step = (int64_t)gridDim.x * RPC;
+    int64_t row = (int64_t)blockIdx.x * RPC + threadIdx.x / T;
+    uint4 next[NV];
+    auto fetch = [&](int64_t r) {
 #pragma unroll
-    for (int i = 0; i < NV; i++) {
-        const int j = t + i * T;
-        v[i] = j < nv ? load8<VEC>(p, row, 8 * j) : make_uint4(0, 0, 0, 0);
-        m = max_mag(max_mag(max_mag(max_mag(m, v[i].x), v[i].y), v[i].z), v[i].w);
-    }
-    for (int j = t + NV * T; j < nv; j += T) {
-        const uint4 u = load8<VEC>(p, row, 8 * j);
-        m = max_mag(max_mag(max_mag(max_mag(m, u.x), u.y), u.z), u.w);
-    }
+        for (int i = 0; i < NV; i++) next[i] = load8<VEC, T>(p, r, t, i);
+    };
+    fetch(row);
+    for (int parity = 0; row < p.rows; row += step, parity ^= 1) {  // the same for all threads of a row
+        uint4 v[NV];
+        uint32_t m = 0;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = __vmaxu2(m, __shfl_xor_sync(FULL, m, o));
-    if constexpr (T > 32) {
-        if ((threadIdx.x & 31) == 0) s_max[threadIdx.x / 32] = m;
-        __syncthreads();
+        for (int i = 0; i < NV; i++) v[i] = next[i];
+        fetch(row + step);
 #pragma unroll
-        for (int w = 0; w < T / 32; w++) m = __vmaxu2(m, s_max[w]);
-    }
-    const RowScale s = row_scale(mag_value<BF16>(m));
-    if (t == 0) p.scales[row] = s.scale;
-    int8_t* out = p.codes + row * p.c_rs;
+        for (int i = 0; i < NV; i++) m = max_mag(m, v[i]);
 #pragma unroll
-    for (int i = 0; i < NV; i++) {
-        const int j = t + i * T;
-        if (j < nv) {
-            uint2 c = make_uint2(codes4<BF16>(v[i].x, v[i].y, s.inv), codes4<BF16>(v[i].z, v[i].w, s.inv));
-            if (!s.live) c = make_uint2(0, 0);
-            *reinterpret_cast<uint2*>(out + 8 * j) = c;  // rows are padded to 16 bytes
+        for (int o = 16; o > 0; o >>= 1) m = __vmaxu2(m, __shfl_xor_sync(FULL, m, o));
+        if constexpr (T > 32) {  // two sets of words: a row's are read while the next row's are written
+            if ((threadIdx.x & 31) == 0) s_max[parity][threadIdx.x / 32] = m;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < T / 32; w++) m = __vmaxu2(m, s_max[parity][w]);
         }
-    }
-    for (int j = t + NV * T; j < nv; j += T) {
-        const uint4 u = load8<VEC>(p, row, 8 * j);
-        uint2 c = make_uint2(codes4<BF16>(u.x, u.y, s.inv), codes4<BF16>(u.z, u.w, s.inv));
-        if (!s.live) c = make_uint2(0, 0);
-        *reinterpret_cast<uint2*>(out + 8 * j) = c;
+        const RowScale s = row_scale(mag_value<BF16>(m));
+        if (t == 0) p.scales[row] = s.scale;
+#pragma unroll
+        for (int i = 0; i < NV; i++) store8<VEC, T>(p, row, t, i, codes8<BF16>(v[i], s));
     }
 }
 
+// Rows too long for a CTA's registers: one CTA per row, read twice.
 template <bool BF16, bool VEC>
-int launch_quantize(const QuantParams& p, cudaStream_t st) {
-    // threads per row: a warp up to 2048 columns (8 vectors a thread), then 4 and 16 warps
-    if (p.k <= 2048)
-        k_quantize_rows<BF16, VEC, 32><<<(unsigned)ceil_div(p.rows, 4), 128, 0, st>>>(p);
-    else if (p.k <= 8192)
-        k_quantize_rows<BF16, VEC, 128><<<p.rows, 128, 0, st>>>(p);
+__global__ void __launch_bounds__(512) k_quantize_long(const __grid_constant__ QuantParams p) {
+    __shared__ uint32_t s_max[16];
+    const int64_t row = blockIdx.x;
+    const int n = (p.k + 8 * 512 - 1) / (8 * 512);
+    uint32_t m = 0;
+#pragma unroll 4
+    for (int i = 0; i < n; i++) m = max_mag(m, load8<VEC, 512>(p, row, threadIdx.x, i));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = __vmaxu2(m, __shfl_xor_sync(FULL, m, o));
+    if ((threadIdx.x & 31) == 0) s_max[threadIdx.x / 32] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 16; w++) m = __vmaxu2(m, s_max[w]);
+    const RowScale s = row_scale(mag_value<BF16>(m));
+    if (threadIdx.x == 0) p.scales[row] = s.scale;
+#pragma unroll 4
+    for (int i = 0; i < n; i++)
+        store8<VEC, 512>(p, row, threadIdx.x, i, codes8<BF16>(load8<VEC, 512>(p, row, threadIdx.x, i), s));
+}
+
+template <bool BF16, bool VEC>
+int launch_quantize(const QuantParams& p, int sms, cudaStream_t st) {
+    // Threads per row: the fewest whose registers hold it (a warp up to 1024
+    // columns); persistent CTAs, as many as fill the SMs' 2048 threads.
+    const int64_t groups = p.k <= 8 * kQuantVec * 32 ? ceil_div(p.rows, 4) : p.rows;
+    auto grid = [&](int cta) { return (unsigned)std::min<int64_t>(groups, (int64_t)sms * (2048 / cta)); };
+    if (p.k <= 8 * kQuantVec * 32)
+        k_quantize_rows<BF16, VEC, 32><<<grid(128), 128, 0, st>>>(p);
+    else if (p.k <= 8 * kQuantVec * 128)
+        k_quantize_rows<BF16, VEC, 128><<<grid(128), 128, 0, st>>>(p);
+    else if (p.k <= 8 * kQuantVec * 256)
+        k_quantize_rows<BF16, VEC, 256><<<grid(256), 256, 0, st>>>(p);
+    else if (p.k <= 8 * kQuantVec * 512)
+        k_quantize_rows<BF16, VEC, 512><<<grid(512), 512, 0, st>>>(p);
     else
-        k_quantize_rows<BF16, VEC, 512><<<p.rows, 512, 0, st>>>(p);
+        k_quantize_long<BF16, VEC><<<p.rows, 512, 0, st>>>(p);
     HB_LAUNCH_CHECK();
     return HB_OK;
 }
@@ -285,7 +331,7 @@ __global__ void __launch_bounds__(256) k_int8_few(const __grid_constant__ FewPar
             mag[m] = 0;
             for (int c = 8 * threadIdx.x; c < p.K && m < p.M; c += 8 * 256) {
                 const uint4 v = load8(m, c);
-                mag[m] = max_mag(max_mag(max_mag(max_mag(mag[m], v.x), v.y), v.z), v.w);
+                mag[m] = max_mag(mag[m], v);
             }
         }
 #pragma unroll
@@ -304,9 +350,7 @@ __global__ void __launch_bounds__(256) k_int8_few(const __grid_constant__ FewPar
             if (threadIdx.x == 0) s_scale[m] = s.scale;
             for (int c = 8 * threadIdx.x; c < pitch && m < p.M; c += 8 * 256) {
                 const uint4 v = load8(m, c);
-                uint2 q = make_uint2(codes4<BF16>(v.x, v.y, s.inv), codes4<BF16>(v.z, v.w, s.inv));
-                if (!s.live) q = make_uint2(0, 0);
-                *reinterpret_cast<uint2*>(s_codes + m * pitch + c) = q;
+                *reinterpret_cast<uint2*>(s_codes + m * pitch + c) = codes8<BF16>(v, s);
             }
         }
         __syncthreads();
@@ -762,6 +806,11 @@ DeviceInfo g_dev[64];
 
 inline bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
+int current_device(int* dev) {
+    HB_CUDA_TRY(cudaGetDevice(dev));
+    return *dev < 64 ? HB_OK : HB_ERR_UNSUPPORTED;
+}
+
 int device_info(int dev, DeviceInfo* info) {
     std::lock_guard<std::mutex> lk(g_mu);
     DeviceInfo& di = g_dev[dev];
@@ -915,8 +964,11 @@ extern "C" int hb_quantize_rows(const void* a, int64_t a_rs, int ka, const void*
     QuantParams p{static_cast<const uint16_t*>(a), static_cast<const uint16_t*>(b), a_rs, b_rs, ka, k, rows, codes, codes_rs, scales};
     const bool vec = aligned(a, 16) && a_rs % 8 == 0 && ka % 8 == 0 && (!kb || (aligned(b, 16) && b_rs % 8 == 0 && kb % 8 == 0));
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (dtype == 1) return vec ? launch_quantize<true, true>(p, st) : launch_quantize<true, false>(p, st);
-    return vec ? launch_quantize<false, true>(p, st) : launch_quantize<false, false>(p, st);
+    int dev = 0, rc;
+    DeviceInfo di;
+    if ((rc = current_device(&dev)) || (rc = device_info(dev, &di))) return rc;
+    if (dtype == 1) return vec ? launch_quantize<true, true>(p, di.sms, st) : launch_quantize<true, false>(p, di.sms, st);
+    return vec ? launch_quantize<false, true>(p, di.sms, st) : launch_quantize<false, false>(p, di.sms, st);
 }
 
 namespace hb {
@@ -933,11 +985,6 @@ int check_linear(const void* x, const int8_t* w, int64_t w_rs, const float* w_sc
         return HB_ERR_ALIGN;
     if (ceil_div(M, 128) > 65535 || ceil_div(M, 128) * ceil_div(N, 128) > INT32_MAX / 8) return HB_ERR_UNSUPPORTED;
     return HB_OK;
-}
-
-int current_device(int* dev) {
-    HB_CUDA_TRY(cudaGetDevice(dev));
-    return *dev < 64 ? HB_OK : HB_ERR_UNSUPPORTED;
 }
 
 int linear_codes(const int8_t* x, int64_t x_rs, const float* x_scales, const int8_t* w, int64_t w_rs, const float* w_scales,
