@@ -218,6 +218,11 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 //   mean (ma + mb) / 2,  deviations da + db + (ma - mb)^2 n / 2,
 // which never subtracts large sums.  The lanes of a warp hold equally many
 // elements (C is a multiple of 256); warps are joined by their counts.
+//
+// 16384 x 3072: 63 us with the residual (5.6 TB/s), 39 us without (3.9 TB/s).  A warp
+// per row over vectors in L1 took 133 and 71 us, C / 8 threads per row 90 and 77 us
+// (the reductions' instructions per element), modulation kept in 16 bits for one
+// more CTA per SM 65 and 44 us (its unpacking).
 template <bool BF16, bool RESIDUAL, int T, int NV, int DEPTH>
 __global__ void __launch_bounds__(128) k_adaln_int8(const __grid_constant__ AdaInt8Params q) {
     using namespace ptx;
@@ -379,7 +384,7 @@ __global__ void __launch_bounds__(128) k_adaln_int8(const __grid_constant__ AdaI
 template <bool BF16, bool RESIDUAL, int T, int NV>
 int launch_adaln_int8(const AdaInt8Params& p, int sms, cudaStream_t st) {
     constexpr int DEPTH = RESIDUAL ? 1 : 2;  // the residual's second stream doubles what is in flight
-    constexpr int CTAS = RESIDUAL ? 3 : 4;   // per SM, by registers
+    constexpr int CTAS = RESIDUAL || NV > 3 ? 3 : 4;  // per SM, by registers
     const int64_t groups = ceil_div(p.a.rows, 128 / T);
     const unsigned grid = (unsigned)std::min<int64_t>(groups, (int64_t)CTAS * sms);
     k_adaln_int8<BF16, RESIDUAL, T, NV, DEPTH><<<grid, 128, 0, st>>>(p);
