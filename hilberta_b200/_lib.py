@@ -8,7 +8,6 @@ is missing.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import os
 from pathlib import Path
@@ -207,13 +206,26 @@ def ptr(t: torch.Tensor | None):
     return None if t is None else ctypes.c_void_p(t.data_ptr())
 
 
-# For ``with``: the current device is the launch's device already.
-SAME_DEVICE = contextlib.nullcontext()
+class on_device:
+    """``with on_device(device) as stream``: the device is current (the library
+    launches on the current one) and ``stream`` its current stream as an integer."""
 
+    __slots__ = ("index", "previous")
 
-def stream_handle(device) -> int:
-    """The current stream of ``device`` as an integer (no Stream object is made)."""
-    return torch._C._cuda_getCurrentRawStream(device.index)
+    def __init__(self, device):
+        self.index = device.index
+
+    def __enter__(self):
+        current = torch._C._cuda_getDevice()
+        self.previous = current if current != self.index else None
+        if self.previous is not None:
+            torch.cuda.set_device(self.index)
+        return torch._C._cuda_getCurrentRawStream(self.index)
+
+    def __exit__(self, *_):
+        if self.previous is not None:
+            torch.cuda.set_device(self.previous)
+        return False
 
 
 def stream_ptr(device) -> ctypes.c_void_p:

@@ -108,29 +108,31 @@ def _call_int8(x, y, gate, shift, scale, x_out, eps):
     if kind not in _DTYPES:
         raise ValueError("x must be float16 or bfloat16")
     x3, x_rs, B, S = _rows(x, "x")
-    C = x3.shape[-1]
+    C = x3.shape[2]
     mods = (shift, scale) if gate is None else (shift, scale, gate)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, y, *mods)):
         raise ValueError("Inference only; disable autograd")
-    mod_bs = _mod(shift, B, C, x, "shift")[1]
-    for name, m in zip(("scale", "gate"), mods[1:]):
-        if _mod(m, B, C, x, name)[1] != mod_bs:
+    mod_bs = None
+    for name, m in zip(("shift", "scale", "gate"), mods):
+        _, bs = _mod(m, B, C, x, name)
+        if mod_bs is not None and bs != mod_bs:
             raise ValueError("gate, shift and scale must share one batch stride")
+        mod_bs = bs
     y_rs = xo_rs = 0
+    y_ptr = gate_ptr = xo_ptr = None
     if y is not None:
         for name, t in (("y", y), ("x_out", x_out)):
             if t.shape != x.shape or t.dtype != kind or t.device != dev:
                 raise ValueError(f"{name} must match x's shape, dtype and device")
         y_rs, xo_rs = _rows(y, "y")[1], _rows(x_out, "x_out")[1]
+        y_ptr, gate_ptr, xo_ptr = y.data_ptr(), gate.data_ptr(), x_out.data_ptr()
         if x_out is not x:
             _check_apart(x_out, x, y, *mods)
     rows = _empty_rows(x.shape, kind, dev)
-    with torch.cuda.device(dev) if dev.index != torch.cuda.current_device() else _lib.SAME_DEVICE:
+    with _lib.on_device(dev) as stream:
         rc = _lib.lib().hb_adaln_residual_int8(
-            x.data_ptr(), x_rs, None if y is None else y.data_ptr(), y_rs, None if y is None else gate.data_ptr(),
-            shift.data_ptr(), scale.data_ptr(), mod_bs, None if y is None else x_out.data_ptr(), xo_rs,
-            rows.values.data_ptr(), rows.row_stride, rows.scales.data_ptr(), B * S, max(S, 1), C, eps, _DTYPES[kind],
-            _lib.stream_handle(dev))
+            x.data_ptr(), x_rs, y_ptr, y_rs, gate_ptr, shift.data_ptr(), scale.data_ptr(), mod_bs, xo_ptr, xo_rs,
+            rows.values.data_ptr(), rows.row_stride, rows.scales.data_ptr(), B * S, max(S, 1), C, eps, _DTYPES[kind], stream)
     if rc == _lib.HB_ERR_UNSUPPORTED:
         raise NotImplementedError("the channel count must be a multiple of 256 up to 4096")
     if rc == _lib.HB_ERR_ALIGN:

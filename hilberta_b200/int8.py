@@ -109,15 +109,10 @@ def _check_source(x, what):
         raise ValueError("CUDA tensors required")
     if x.dtype not in _DTYPES:
         raise TypeError(f"{what} must be float16 or bfloat16")
-    if x.shape[-1] < 1 or (x.shape[-1] > 1 and x.stride(-1) != 1):
+    if x.stride(-1) != 1 and x.shape[-1] > 1 or x.shape[-1] < 1:
         raise ValueError(f"{what} must have a nonempty contiguous last dimension")
-    if torch.is_grad_enabled() and x.requires_grad:
+    if x.requires_grad and torch.is_grad_enabled():
         raise ValueError("Inference only; disable autograd")
-
-
-def _on(device):
-    """The launches of the library go to the current device."""
-    return torch.cuda.device(device) if device.index != torch.cuda.current_device() else _lib.SAME_DEVICE
 
 
 def quantize_rows(x, *, joined=None):
@@ -140,10 +135,10 @@ def quantize_rows(x, *, joined=None):
     rows = out.scales.numel()
     if rows >= 1 << 31:
         raise NotImplementedError("2^31 rows or more are not supported")
-    with _on(x.device):
+    with _lib.on_device(x.device) as stream:
         rc = _lib.lib().hb_quantize_rows(
             x.data_ptr(), x_rs, ka, None if joined is None else joined.data_ptr(), j_rs, kb, rows, out.values.data_ptr(),
-            out.row_stride, out.scales.data_ptr(), _DTYPES[x.dtype], _lib.stream_handle(x.device))
+            out.row_stride, out.scales.data_ptr(), _DTYPES[x.dtype], stream)
     _lib.check(rc, "hb_quantize_rows")
     return out
 
@@ -158,32 +153,38 @@ def int8_linear(x, weight, bias=None, *, activation=None, out=None):
     spaced (a slice of a wider buffer), a leading dimension whose rows are not
     equally spaced takes one launch per index.  Integer sums are exact, so equal
     inputs give equal outputs whatever the number of tokens."""
-    if not isinstance(weight, Int8Rows) or weight.ndim != 2:
+    if not isinstance(weight, Int8Rows) or weight.values.ndim != 2:
         raise TypeError("weight must be 2-D Int8Rows [N, K] (quantize_rows of a weight matrix)")
-    if not isinstance(x, Int8Rows):
-        _check_source(x, "x")
-    if x.ndim < 1 or x.shape[-1] != weight.shape[1]:
-        raise ValueError("x and weight must have the same inner size")
-    if x.device != weight.device:
-        raise ValueError("x and weight must be on the same CUDA device")
-    if activation not in _ACTIVATIONS:
-        raise ValueError('activation must be None or "gelu_tanh"')
-    N = weight.shape[0]
-    if bias is not None:
-        if bias.shape != (N,) or bias.dtype != x.dtype or bias.device != x.device or not bias.is_contiguous():
-            raise ValueError("bias must be a contiguous [N] tensor of x's type and device")
-        if torch.is_grad_enabled() and bias.requires_grad:
-            raise ValueError("Inference only; disable autograd")
-    shape = (*x.shape[:-1], N)
-    if out is None:
-        out = torch.empty(shape, dtype=x.dtype, device=x.device)
+    coded = isinstance(x, Int8Rows)
+    if coded:
+        x_shape = x.values.shape
     else:
-        if out.shape != shape or out.dtype != x.dtype or out.device != x.device or (N > 1 and out.stride(-1) != 1):
+        _check_source(x, "x")
+        x_shape = x.shape
+    N, K = weight.values.shape
+    kind, dev = x.dtype, x.device
+    if x_shape[-1] != K:
+        raise ValueError("x and weight must have the same inner size")
+    if weight.values.device != dev:
+        raise ValueError("x and weight must be on the same CUDA device")
+    act = _ACTIVATIONS.get(activation)
+    if act is None:
+        raise ValueError('activation must be None or "gelu_tanh"')
+    if bias is not None:
+        if bias.shape != (N,) or bias.dtype != kind or bias.device != dev or not bias.is_contiguous():
+            raise ValueError("bias must be a contiguous [N] tensor of x's type and device")
+        if bias.requires_grad and torch.is_grad_enabled():
+            raise ValueError("Inference only; disable autograd")
+    shape = (*x_shape[:-1], N)
+    if out is None:
+        out = torch.empty(shape, dtype=kind, device=dev) if coded else x.new_empty(shape)
+    else:
+        if out.shape != shape or out.dtype != kind or out.device != dev or (N > 1 and out.stride(-1) != 1):
             raise ValueError("out must be [..., N] of x's type and device with a contiguous last dimension")
-        if torch.is_grad_enabled() and out.requires_grad:
+        if out.requires_grad and torch.is_grad_enabled():
             raise ValueError("Inference output cannot require gradients")
         _check_out(out, x, weight, bias)
-    _product(x, weight, bias, _ACTIVATIONS[activation], out)
+    _product(x, coded, weight, bias, act, out, dev)
     return out
 
 
@@ -210,29 +211,28 @@ def _span(t):
     return t.data_ptr(), t.data_ptr() + extent * t.element_size()
 
 
-def _product(x, weight, bias, act, out):
-    coded = isinstance(x, Int8Rows)
+def _product(x, coded, weight, bias, act, out, dev):
     out_rs = _row_stride(out)
     x_rs = x.row_stride if coded else _row_stride(x)
     if out_rs is None or x_rs is None:  # a leading index at a time
         for i in range(out.shape[0]):
             part = Int8Rows(x.values[i], x.scales[i], x.dtype) if coded else x[i]
-            _product(part, weight, bias, act, out[i])
+            _product(part, coded, weight, bias, act, out[i], dev)
         return
-    dev = x.device
     lib = _lib.lib()
-    N, K = weight.values.shape
+    w = weight.values
+    N, K = w.shape
     M = x.scales.numel() if coded else x.numel() // K
-    tail = (weight.values.data_ptr(), weight.row_stride, weight.scales.data_ptr(), None if bias is None else bias.data_ptr(),
-            out.data_ptr(), out_rs, M, N, K, act, _DTYPES[x.dtype])
-    with _on(dev):
-        stream = _lib.stream_handle(dev)
+    tail = (w.data_ptr(), weight.row_stride, weight.scales.data_ptr(), None if bias is None else bias.data_ptr(),
+            out.data_ptr(), out_rs, M, N, K, act, _DTYPES[out.dtype])
+    with _lib.on_device(dev) as stream:
         if coded:
             rc = lib.hb_int8_linear(x.values.data_ptr(), x_rs, x.scales.data_ptr(), *tail, stream)
+        elif nbytes := lib.hb_int8_linear16_workspace_bytes(M, K):
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            rc = lib.hb_int8_linear16(x.data_ptr(), x_rs, *tail, ws.data_ptr(), nbytes, stream)
         else:
-            nbytes = lib.hb_int8_linear16_workspace_bytes(M, K)
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-            rc = lib.hb_int8_linear16(x.data_ptr(), x_rs, *tail, None if ws is None else ws.data_ptr(), nbytes, stream)
+            rc = lib.hb_int8_linear16(x.data_ptr(), x_rs, *tail, None, 0, stream)
     if rc == _lib.HB_ERR_UNSUPPORTED:
         raise NotImplementedError(f"int8_linear: {_lib.status_text(rc)}")
     _lib.check(rc, "hb_int8_linear")

@@ -153,18 +153,17 @@ def norm_rope_qk(q, k, *, weight_q, weight_k, cos, sin, text_tokens=0, weight_tx
     if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, cos, sin, *weights)):
         raise ValueError("Inference only; disable autograd")
     if out is None:
-        q_out = torch.empty((B, S, Hq, D), dtype=kind, device=dev)
-        k_out = torch.empty((B, S, Hk, D), dtype=kind, device=dev)
+        q_out, k_out = q.new_empty((B, S, Hq, D)), k.new_empty((B, S, Hk, D))
     else:
         _check_qk_out(q, k, out, (cos, sin, *weights))
         q_out, k_out = out
     strides = _Strides(*q.stride()[:3], *k.stride()[:3], *q_out.stride()[:3], *k_out.stride()[:3])
-    with torch.cuda.device(dev) if dev.index != torch.cuda.current_device() else _lib.SAME_DEVICE:
+    with _lib.on_device(dev) as stream:
         rc = _lib.lib().hb_norm_rope_qk(
             q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr(), strides, B, S, T, Hq, Hk, D,
             weight_q.data_ptr(), weight_k.data_ptr(), None if weight_txt_q is None else weight_txt_q.data_ptr(),
             None if weight_txt_k is None else weight_txt_k.data_ptr(), eps, cos.data_ptr(), sin.data_ptr(), dtype,
-            _lib.stream_handle(dev))
+            stream)
     if rc == _lib.HB_ERR_ALIGN:
         raise ValueError("hb_norm_rope_qk needs 16-byte aligned rows (strides multiples of 8 elements)")
     if rc == _lib.HB_ERR_UNSUPPORTED:
