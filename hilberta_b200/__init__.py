@@ -15,11 +15,14 @@ built from them (``HilbertAProcessor``), the reference adapter's entry
 (``persistent_flux_attention``) and sampling wrapper (``sample_flux_persistent``),
 and a FLUX.1-architecture transformer with
 random weights and diffusers' interface to run it on
-(``hilberta_b200.flux_model.FluxTransformer``).
+(``hilberta_b200.flux_model.FluxTransformer``).  Linear layers in 8-bit
+integers (``int8_linear``, ``Int8Linear``, ``quantize_rows``), query/key norms and
+rotation in one pass (``norm_rope_qk``), and that transformer made of them
+(``hilberta_b200.flux_int8.quantize_flux_model``).
 """
 
 from .bridge_k import bridge_k_plan
-from .int8 import Int8Rows, int8_linear, quantize_rows
+from .int8 import Int8Linear, Int8Rows, int8_linear, quantize_rows
 from .head_parallel import PeerAllGather, all_gather_heads, head_parallel_attention
 from .paired_kernel import RasterOrder, device_status, paired_attention, raster_order, token_order_map
 from .paired_metadata import PairedMetadata, pair_metadata, unpair_metadata
@@ -59,6 +62,7 @@ __all__ = [
     "norm_rope_pack",
     "norm_rope_qk",
     "Int8Rows",
+    "Int8Linear",
     "quantize_rows",
     "int8_linear",
     "PeerAllGather",

@@ -85,7 +85,9 @@ class DenseProcessor:
             raise ValueError("External attention masks are not supported")
         cos, sin = image_rotary_emb
         h = attn.heads
-        if encoder_hidden_states is not None:
+        if hasattr(attn, "joint_qkv"):  # 8-bit attention modules prepare q, k and v themselves
+            q, k, v = (x.transpose(1, 2) for x in attn.joint_qkv(hidden_states, encoder_hidden_states, image_rotary_emb))
+        elif encoder_hidden_states is not None:
             q = norm_rope_pack(attn.add_q_proj(encoder_hidden_states), attn.to_q(hidden_states), heads=h,
                                weight_txt=attn.norm_added_q.weight, weight_img=attn.norm_q.weight, cos=cos, sin=sin)
             k = norm_rope_pack(attn.add_k_proj(encoder_hidden_states), attn.to_k(hidden_states), heads=h,

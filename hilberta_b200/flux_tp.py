@@ -197,6 +197,8 @@ def shard_flux_model(model, group=None, *, chunks=1, carveout=None, min_rows=204
     of the GEMMs meanwhile (``chunks=1``: one GEMM, then one all-reduce).
     ``sequence_parallel``: the image and joined streams split by tokens (see the
     module docstring)."""
+    if getattr(model, "int8", False):
+        raise ValueError("a model in 8 bits cannot be sharded")
     world = dist.get_world_size(group)
     rank = dist.get_rank(group)
     ov = _Overlap(chunks, carveout, min_rows)

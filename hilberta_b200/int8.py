@@ -5,6 +5,7 @@ per token), products summed exactly in 32-bit integers.
 ``quantize_rows(x)``                  16-bit rows -> ``Int8Rows`` (weights and activations alike)
 ``quantize_rows(a, joined=b)``        the rows [a | b] without the concatenation
 ``int8_linear(x, weight, bias, ...)`` act((x @ weight^T) + bias) in 16 bits
+``Int8Linear(linear)``                a ``torch.nn.Linear`` with 8-bit weights
 
 A row's scale is max|x| / 127 and its codes round(x * (127 / max|x|)), ties to
 even.  A row holding an infinity or NaN gets the scale NaN: every output made
@@ -239,4 +240,48 @@ def _product(x, coded, weight, bias, act, out, dev):
     _used.add(dev.index)
 
 
-__all__ = ["Int8Rows", "quantize_rows", "int8_linear"]
+class Int8Linear(torch.nn.Module):
+    """``torch.nn.Linear`` with 8-bit weights, quantised once from ``linear`` (a
+    CUDA layer in float16 or bfloat16): y = int8_linear(x, weight, bias).
+
+    ``forward`` takes 16-bit tensors or ``Int8Rows``.  ``weight`` is the layer's
+    ``Int8Rows``; its parts are the buffers ``values`` and ``scales``."""
+
+    def __init__(self, linear):
+        super().__init__()
+        self._set(quantize_rows(linear.weight.detach()), None if linear.bias is None else linear.bias.detach())
+
+    def _set(self, rows, bias):
+        self.dtype = rows.dtype
+        self.register_buffer("values", rows.values)
+        self.register_buffer("scales", rows.scales)
+        self.register_buffer("bias", bias)
+
+    @classmethod
+    def joined(cls, linears):
+        """One layer of several that read the same input: their outputs side by side."""
+        self = cls.__new__(cls)
+        torch.nn.Module.__init__(self)
+        weight = torch.cat([m.weight.detach() for m in linears])
+        bias = None
+        if any(m.bias is not None for m in linears):
+            bias = torch.cat([weight.new_zeros(m.weight.shape[0]) if m.bias is None else m.bias.detach() for m in linears])
+        self._set(quantize_rows(weight), bias)
+        return self
+
+    def outputs(self, start, stop):
+        """The layer of output channels [start, stop), sharing this one's storage."""
+        part = Int8Linear.__new__(Int8Linear)
+        torch.nn.Module.__init__(part)
+        part._set(self.weight.row_slice(start, stop), None if self.bias is None else self.bias[start:stop])
+        return part
+
+    @property
+    def weight(self):
+        return Int8Rows(self.values, self.scales, self.dtype)
+
+    def forward(self, x, *, activation=None, out=None):
+        return int8_linear(x, self.weight, self.bias, activation=activation, out=out)
+
+
+__all__ = ["Int8Rows", "Int8Linear", "quantize_rows", "int8_linear"]

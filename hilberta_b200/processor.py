@@ -44,6 +44,16 @@ class HilbertAProcessor:
         output projections."""
         if torch.is_grad_enabled():
             raise RuntimeError("HilbertA attention is inference-only; use torch.no_grad or inference_mode")
+        if hasattr(attn, "joint_qkv"):  # 8-bit attention modules prepare q, k and v themselves
+            q, k, v = attn.joint_qkv(hidden_states, encoder_hidden_states, image_rotary_emb)
+        else:
+            q, k, v = self._prepare(attn, hidden_states, encoder_hidden_states, image_rotary_emb)
+        if q.shape[2] != self.bank.total_tokens:
+            raise ValueError("Native attention sequence length does not match the plan")
+        return self._attend(q, k, v).transpose(1, 2).flatten(2, 3)
+
+    def _prepare(self, attn, hidden_states, encoder_hidden_states, image_rotary_emb):
+        """q, k, v as [B, H, S, D] views of [B, S, H, D]."""
         heads = attn.heads
         cos, sin = (None, None) if image_rotary_emb is None else image_rotary_emb
         if encoder_hidden_states is not None and getattr(attn, "added_kv_proj_dim", None) is not None:
@@ -73,10 +83,7 @@ class HilbertAProcessor:
                     sin=rot[1],
                 )
             )
-        q, k, v = (x.transpose(1, 2) for x in packed)  # [B, H, S, D] views of [B, S, H, D]
-        if q.shape[2] != self.bank.total_tokens:
-            raise ValueError("Native attention sequence length does not match the plan")
-        return self._attend(q, k, v).transpose(1, 2).flatten(2, 3)
+        return tuple(x.transpose(1, 2) for x in packed)
 
     def _attend(self, q, k, v):
         """The attention of the layer's phase on the prepared [B, H, S, D] views."""
