@@ -1,0 +1,616 @@
+// 8-bit products on the tensor cores (tcgen05 kind::i8, 32-bit integer sums in TMEM):
+// 256 x 256 or 256 x 128 tiles by CTA pairs for many tokens, 128 channels x up to 128
+// tokens by single CTAs, which may split K, for few.
+#include <algorithm>
+#include <climits>
+#include <mutex>
+
+#include "int8_common.cuh"
+
+namespace hb {
+namespace {
+
+using namespace ptx;
+constexpr unsigned FULL = 0xffffffffu;
+
+// HB_DEV_* bits of the launches on this device (read by hb_int8_status).
+__device__ int32_t g_int8_status;
+
+struct GemmParams {
+    CUtensorMap tmap_x;    // int8 [M][K], boxes of 128 bytes
+    CUtensorMap tmap_w;    // int8 [N][K]
+    CUtensorMap tmap_out;  // 16-bit [M][N], box 32 x 128 bytes (pair kernel, tma_out)
+    const float* x_scales;
+    const float* w_scales;
+    const uint16_t* bias;  // [N] or null
+    uint16_t* out;
+    int64_t out_rs;
+    int M, N, K, act;
+    int tma_out;  // out rows start on 16 bytes: TMA stores
+    int tiles_m, tiles_n;
+    long long timeout;
+};
+
+// Up to 128 tokens x 128 channels per CTA, the weights as the product's first
+// operand: its 128 rows are then always full, the tokens' side is as narrow as there
+// are tokens (BT), and the weights' bytes, which bound it, pass shared memory once.
+// The CTAs of a cluster split K and exchange their 32-bit sums through distributed
+// shared memory.  A thread holds one channel and half of the tokens, so a warp's
+// stores of a token are 64 contiguous bytes.
+template <int BT>
+struct TileCfg {
+    static constexpr int BC = 128, BK = 128;
+    static constexpr int W_BYTES = BC * BK, X_BYTES = BT * BK, STAGE = W_BYTES + X_BYTES;
+    static constexpr int STAGES = 104 * 1024 / STAGE;  // two CTAs per SM
+    static constexpr int PITCH = BC;                   // words between tokens' partial sums
+    static constexpr int HALF = BT / 2;                // tokens per warp in the epilogue: two warps share a channel
+    static constexpr int TMEM_COLS = BT < 64 ? 64 : BT;  // loads of 32 columns from the second half on stay inside
+    struct Ctl {
+        uint64_t full[STAGES], empty[STAGES], done;
+        uint32_t tmem_base;
+        int abort;
+        float scales[BT + 8];  // of the tokens, read eight at a time
+    };
+    static constexpr int CTL_OFF = STAGES * STAGE;
+    static constexpr int SMEM = CTL_OFF + (int)((sizeof(Ctl) + 15) / 16 * 16);
+    static_assert(BT * PITCH * 4 <= CTL_OFF, "partial sums reuse the stages");
+};
+
+template <bool BF16, int BT>
+__global__ void __launch_bounds__(256, 2) k_int8_tile(const __grid_constant__ GemmParams p, int split) {
+    using C = TileCfg<BT>;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    auto* ctl = reinterpret_cast<typename C::Ctl*>(smem + C::CTL_OFF);
+    constexpr int U = 8;  // tokens finished together
+    volatile int* abort_flag = &ctl->abort;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = blockIdx.x % split;
+    const int n0 = blockIdx.x / split * C::BC, m0 = blockIdx.y * BT;
+    const int nkb = (p.K + C::BK - 1) / C::BK;
+    const int kb0 = (int)((int64_t)nkb * rank / split), kb1 = (int)((int64_t)nkb * (rank + 1) / split);
+
+    if (smem_u32(smem) & 1023) {  // uniform over the cluster
+        if (threadIdx.x == 0) atomicOr(&g_int8_status, HB_DEV_SMEM_ALIGN);
+        return;
+    }
+    if (warp == 0 && lane == 0) {
+        prefetch_tmap(&p.tmap_x);
+        prefetch_tmap(&p.tmap_w);
+        for (int i = 0; i < C::STAGES; i++) {
+            mbar_init(&ctl->full[i], 1);
+            mbar_init(&ctl->empty[i], 1);
+        }
+        mbar_init(&ctl->done, 1);
+        ctl->abort = 0;
+        fence_barrier_init();
+    }
+    if (warp == 2) {
+        tmem_alloc(&ctl->tmem_base, C::TMEM_COLS);
+        tmem_relinquish();
+        tc_fence_before();
+    }
+    const int channel = threadIdx.x & 127, n = n0 + channel;  // this thread's channel
+    const int t0 = (warp >> 2) * C::HALF;                     // and the first of its tokens
+    const float sw = n < p.N ? p.w_scales[n] : 0.f, bias = n < p.N && p.bias ? load16<BF16>(p.bias + n) : 0.f;
+    if (threadIdx.x < BT) ctl->scales[threadIdx.x] = m0 + (int)threadIdx.x < p.M ? p.x_scales[m0 + threadIdx.x] : 0.f;
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = ctl->tmem_base;
+
+    if (warp == 0 && lane == 0) {
+        int it = 0;
+        bool ok = true;
+        for (int kb = kb0; kb < kb1; kb++, it++) {
+            const int s = it % C::STAGES;
+            if (it >= C::STAGES && !mbar_wait(&ctl->empty[s], (it / C::STAGES - 1) & 1, abort_flag, p.timeout)) {
+                ok = false;
+                break;
+            }
+            uint8_t* st = smem + s * C::STAGE;
+            mbar_arrive_expect_tx(&ctl->full[s], C::STAGE);
+            tma_load_2d(st, &p.tmap_w, &ctl->full[s], kb * C::BK, n0);
+            tma_load_2d(st + C::W_BYTES, &p.tmap_x, &ctl->full[s], kb * C::BK, m0);
+        }
+        if (!ok) {  // let the copies in flight land before the CTA gives up its memory
+            volatile int ignore = 0;
+            for (int j = max(0, it - C::STAGES); j < it; j++)
+                mbar_wait(&ctl->full[j % C::STAGES], (j / C::STAGES) & 1, &ignore, p.timeout);
+        }
+    } else if (warp == 1 && lane == 0) {
+        constexpr uint32_t idesc = idesc_i8(C::BC, BT);
+        bool ok = true;
+        int it = 0;
+        for (int kb = kb0; kb < kb1; kb++, it++) {
+            const int s = it % C::STAGES;
+            if (!mbar_wait(&ctl->full[s], (it / C::STAGES) & 1, abort_flag, p.timeout)) {
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+            const uint32_t w = smem_u32(smem + s * C::STAGE), x = w + C::W_BYTES;
+#pragma unroll
+            for (int k = 0; k < C::BK; k += 32)
+                mma_i8_ss(tmem, desc_sw128(w + k, 16, 1024), desc_sw128(x + k, 16, 1024), idesc, it > 0 || k > 0);
+            tc_commit(&ctl->empty[s]);
+        }
+        if (ok) tc_commit(&ctl->done);
+    }
+    __syncwarp();
+    bool ok = __all_sync(FULL, mbar_wait(&ctl->done, 0, abort_flag, p.timeout));
+    if (!ok && lane == 0) atomicOr(&g_int8_status, HB_DEV_TIMEOUT);
+    // Finishes U tokens from j on: straight-line code, so that their latencies overlap.
+    auto finish_tokens = [&](int j, int end, const int (&acc)[U]) {
+        float y[U];
+#pragma unroll
+        for (int i = 0; i < U; i++) y[i] = finish<0>(acc[i], ctl->scales[j + i], sw, bias);
+        if (p.act) {
+#pragma unroll
+            for (int i = 0; i < U; i++) y[i] = gelu_tanh(y[i]);
+        }
+        if (n >= p.N) return;
+        uint16_t* dst = p.out + (int64_t)(m0 + j) * p.out_rs + n;
+#pragma unroll
+        for (int i = 0; i < U; i++)
+            if (j + i < end) dst[i * p.out_rs] = (uint16_t)pack2<BF16>(y[i], 0.f);
+    };
+    const int tokens = min(BT, p.M - m0);
+    const uint32_t acc0 = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + t0;
+    if (split == 1) {
+        if (ok) {
+            tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < C::HALF; c += 32) {
+                uint32_t r[32];
+                tmem_ld32(acc0 + c, r);
+#pragma unroll
+                for (int i = 0; i < (C::HALF < 32 ? C::HALF : 32); i += U) {
+                    int acc[U];
+#pragma unroll
+                    for (int e = 0; e < U; e++) acc[e] = (int)r[i + e];
+                    if (t0 + c + i < tokens) finish_tokens(t0 + c + i, tokens, acc);
+                }
+            }
+            tc_fence_before();
+        }
+        __syncthreads();
+        if (warp == 2) {
+            tc_fence_after();
+            tmem_dealloc(tmem, C::TMEM_COLS);
+        }
+        return;
+    }
+    // Every CTA of the cluster sends each peer the sums of that peer's share of the
+    // tokens ([source][token][channel], in the stages, which every MMA has read by
+    // the first barrier) and adds up its own share.
+    const int log_share = __ffs(BT) - __ffs(split), share = 1 << log_share;  // both powers of two
+    int* part = reinterpret_cast<int*>(smem);
+    const uint32_t mine = smem_u32(part + rank * share * C::PITCH + channel);
+    ok = __syncthreads_and(ok);
+    cluster_sync();  // every CTA arrives at both barriers, whatever happened before
+    if (ok) {
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < C::HALF; c += 32) {
+            uint32_t r[32];
+            tmem_ld32(acc0 + c, r);
+#pragma unroll
+            for (int i = 0; i < (C::HALF < 32 ? C::HALF : 32); i++) {
+                const int j = t0 + c + i;
+                const uint32_t at = mine + (j & (share - 1)) * (C::PITCH * 4);
+                st_cluster_s32(cluster_map(at, j >> log_share), (int)r[i]);
+            }
+        }
+        tc_fence_before();
+    }
+    __syncthreads();
+    cluster_sync();
+    if (warp == 2) {
+        tc_fence_after();
+        tmem_dealloc(tmem, C::TMEM_COLS);
+    }
+    if (!ok) return;
+    for (int j = U * (warp >> 2); j < share && rank * share + j < tokens; j += 2 * U) {
+        int acc[U] = {};
+        for (int q = 0; q < split; q++) {
+#pragma unroll
+            for (int i = 0; i < U; i++)
+                if (j + i < share) acc[i] += part[(q * share + j + i) * C::PITCH + channel];
+        }
+        finish_tokens(rank * share + j, min(tokens, (rank + 1) * share), acc);
+    }
+}
+
+// 256 x BN (256 or 128) output tiles by CTA pairs, persistent.  One MMA of a pair
+// covers 256 x BN x 32: each CTA stages 128 rows of the tokens and BN / 2 of the
+// weights, so it reads half of the weight tile's bytes that it would need alone, and
+// both keep 128 rows of the accumulator.  Two accumulators (all of the TMEM at BN
+// 256): the epilogue of a tile runs under the products of the next.
+template <int BN_>
+struct PairCfg {
+    static constexpr int BM = 256, BN = BN_, BK = 128;
+    static constexpr int A_BYTES = 128 * BK, B_BYTES = BN / 2 * BK, STAGE = A_BYTES + B_BYTES;
+    static constexpr int STAGES = 192 * 1024 / STAGE;
+    static constexpr int EPI_WARPS = 8;         // two per TMEM lane quarter, half of the columns each
+    static constexpr int STAGING = 32 * 128;    // per warp: 32 rows x 64 columns of the output
+    static constexpr int THREADS = 128 + 32 * EPI_WARPS;
+    struct Ctl {
+        uint64_t full[STAGES], empty[STAGES], acc_full[2], acc_empty[2];
+        uint32_t tmem_base;
+        int abort;
+        alignas(16) float2 cols[BN];  // weight scale and bias of the tile's columns, read two at a time
+    };
+    static constexpr int STG_OFF = STAGES * STAGE;
+    static constexpr int CTL_OFF = STG_OFF + EPI_WARPS * STAGING;
+    static constexpr int SMEM = CTL_OFF + (int)((sizeof(Ctl) + 15) / 16 * 16);
+    static_assert(SMEM <= 227 * 1024, "shared memory of one CTA");
+    // Tiles are walked down columns of GROUP row tiles, so the tiles in flight at
+    // one time share few rows of both operands (both stay in L2).
+    static constexpr int GROUP = 8;
+};
+
+template <class C>
+__device__ __forceinline__ void pair_tile(const GemmParams& p, int t, int& m0, int& n0) {
+    const int per = C::GROUP * p.tiles_n;
+    const int g = t / per, r = t - g * per;
+    const int gm = min(C::GROUP, p.tiles_m - g * C::GROUP);
+    m0 = (g * C::GROUP + r % gm) * C::BM;
+    n0 = r / gm * C::BN;
+}
+
+template <bool BF16, int ACT, int BN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<BN>::THREADS, 1)
+    k_int8_pair(const __grid_constant__ GemmParams p) {
+    using C = PairCfg<BN>;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    auto* ctl = reinterpret_cast<typename C::Ctl*>(smem + C::CTL_OFF);
+    volatile int* abort_flag = &ctl->abort;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = (int)cluster_rank();
+    const int first = blockIdx.x >> 1, step = gridDim.x >> 1, tiles = p.tiles_m * p.tiles_n;
+    const int nkb = (p.K + C::BK - 1) / C::BK;
+
+    if (smem_u32(smem) & 1023) {  // the same in both CTAs
+        if (threadIdx.x == 0) atomicOr(&g_int8_status, HB_DEV_SMEM_ALIGN);
+        return;
+    }
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < C::STAGES; i++) {
+            mbar_init(&ctl->full[i], 1);
+            mbar_init(&ctl->empty[i], 1);
+        }
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&ctl->acc_full[i], 1);
+            mbar_init(&ctl->acc_empty[i], 2 * C::EPI_WARPS);
+        }
+        ctl->abort = 0;
+        fence_barrier_init();
+        prefetch_tmap(&p.tmap_x);
+        prefetch_tmap(&p.tmap_w);
+        if (p.tma_out) prefetch_tmap(&p.tmap_out);
+    }
+    if (warp == 2) {
+        tmem_alloc_pair(&ctl->tmem_base, 2 * BN);
+        tc_fence_before();
+    }
+    __syncthreads();
+    cluster_sync();
+    tc_fence_after();
+    const uint32_t tmem = ctl->tmem_base;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int it = 0;
+            bool ok = true;
+            for (int t = first; t < tiles && ok; t += step) {
+                int m0, n0;
+                pair_tile<C>(p, t, m0, n0);
+                for (int kb = 0; kb < nkb; kb++, it++) {
+                    const int s = it % C::STAGES;
+                    if (it >= C::STAGES &&
+                        !mbar_wait_cluster(&ctl->empty[s], (it / C::STAGES - 1) & 1, abort_flag, p.timeout)) {
+                        ok = false;
+                        break;
+                    }
+                    uint8_t* st = smem + s * C::STAGE;
+                    if (rank == 0) mbar_arrive_expect_tx(&ctl->full[s], 2 * C::STAGE);
+                    const uint32_t bar = cluster_map(smem_u32(&ctl->full[s]), 0);
+                    tma_load_2d_pair(st, &p.tmap_x, bar, kb * C::BK, m0 + 128 * rank);
+                    tma_load_2d_pair(st + C::A_BYTES, &p.tmap_w, bar, kb * C::BK, n0 + BN / 2 * rank);
+                }
+            }
+            if (!ok) {  // gave up: time for the copies and MMAs in flight to end before the memory is given back
+                const long long t0 = clock64();
+                while (clock64() - t0 < p.timeout / 1000) {
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            constexpr uint32_t idesc = idesc_i8(C::BM, C::BN);
+            int it = 0, i = 0;
+            bool ok = true;
+            for (int t = first; t < tiles && ok; t += step, i++) {
+                const uint32_t d = tmem + (i & 1) * BN;
+                if (i >= 2 && !mbar_wait_cluster(&ctl->acc_empty[i & 1], (i / 2 - 1) & 1, abort_flag, p.timeout)) break;
+                tc_fence_after();
+                for (int kb = 0; kb < nkb; kb++, it++) {
+                    const int s = it % C::STAGES;
+                    if (!mbar_wait_cluster(&ctl->full[s], (it / C::STAGES) & 1, abort_flag, p.timeout)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t a = smem_u32(smem + s * C::STAGE), b = a + C::A_BYTES;
+#pragma unroll
+                    for (int k = 0; k < C::BK; k += 32)
+                        mma_i8_ss_pair(d, desc_sw128(a + k, 16, 1024), desc_sw128(b + k, 16, 1024), idesc, kb > 0 || k > 0);
+                    tc_commit_pair(&ctl->empty[s], 3);
+                }
+                if (ok) tc_commit_pair(&ctl->acc_full[i & 1], 3);
+            }
+        }
+    } else if (warp >= 4) {
+        const int ew = warp - 4, quarter = warp & 3, half = ew >> 2;
+        uint8_t* stg = smem + C::STG_OFF + ew * C::STAGING;
+        float2* cols = ctl->cols + BN / 2 * half;
+        int i = 0;
+        bool dead = false;  // a wait ran out: only the barriers of the remaining tiles are kept, so that no warp is left at one
+        for (int t = first; t < tiles; t += step, i++) {
+            int m0, n0;
+            pair_tile<C>(p, t, m0, n0);
+            const int row0 = m0 + 128 * rank + 32 * quarter, col0 = n0 + BN / 2 * half;
+            {  // this half's column scales and biases (its four warps only)
+                const int c = threadIdx.x & 127;
+                float2 v = make_float2(0.f, 0.f);
+                if (c < BN / 2 && col0 + c < p.N) {
+                    v.x = p.w_scales[col0 + c];
+                    if (p.bias) v.y = load16<BF16>(p.bias + col0 + c);
+                }
+                asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");
+                if (c < BN / 2) cols[c] = v;
+                asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");
+            }
+            if (dead) continue;
+            const float sx = row0 + lane < p.M ? p.x_scales[row0 + lane] : 0.f;
+            const bool ok = mbar_wait_cluster(&ctl->acc_full[i & 1], (i >> 1) & 1, abort_flag, p.timeout);
+            if (!__all_sync(FULL, ok)) {
+                if (lane == 0) atomicOr(&g_int8_status, HB_DEV_TIMEOUT);
+                dead = true;
+                continue;
+            }
+            tc_fence_after();
+            const uint32_t acc = tmem + ((uint32_t)(32 * quarter) << 16) + (i & 1) * BN + BN / 2 * half;
+#pragma unroll
+            for (int c = 0; c < BN / 2; c += 64) {
+                uint32_t lo[32], hi[32];
+                tmem_ld32_async(acc + c, lo);
+                tmem_ld32_async(acc + c + 32, hi);
+                tmem_wait_ld(lo);
+                tmem_wait_ld(hi);
+                if (c + 64 == BN / 2) {  // the accumulator is in registers: the next tile but one may take its place
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster(cluster_map(smem_u32(&ctl->acc_empty[i & 1]), 0));
+                }
+                if (lane == 0) bulk_wait_read<0>();
+                __syncwarp();
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    uint32_t o[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int x = 8 * j + 2 * e;
+                        const float4 sb = *reinterpret_cast<const float4*>(cols + c + x);
+                        const int u = (int)(x < 32 ? lo[x & 31] : hi[x & 31]);
+                        const int v = (int)(x < 32 ? lo[(x + 1) & 31] : hi[(x + 1) & 31]);
+                        o[e] = pack2<BF16>(finish<ACT>(u, sx, sb.x, sb.y), finish<ACT>(v, sx, sb.z, sb.w));
+                    }
+                    // 128-byte rows with the map's swizzle: conflict-free 16-byte stores
+                    *reinterpret_cast<uint4*>(stg + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+                }
+                if (p.tma_out) {
+                    fence_async_smem();
+                    __syncwarp();
+                    if (lane == 0 && row0 < p.M && col0 + c < p.N) {
+                        tma_store_2d(&p.tmap_out, stg, col0 + c, row0);
+                        bulk_commit();
+                    }
+                } else {
+                    __syncwarp();
+                    for (int r = 0; r < 32 && row0 + r < p.M; r++)
+#pragma unroll
+                        for (int k = 0; k < 64; k += 32) {
+                            const int x = k + lane;
+                            if (col0 + c + x < p.N)
+                                p.out[(int64_t)(row0 + r) * p.out_rs + col0 + c + x] = *reinterpret_cast<const uint16_t*>(
+                                    stg + r * 128 + (((x >> 3) ^ (r & 7)) << 4) + (x & 7) * 2);
+                        }
+                    __syncwarp();
+                }
+            }
+        }
+        if (lane == 0) bulk_wait<0>();
+    }
+    __syncwarp();
+    __syncthreads();
+    cluster_sync();  // no CTA leaves while the other's MMAs read its memory or arrivals are on the way
+    if (warp == 2) {
+        tc_fence_after();
+        tmem_dealloc_pair(tmem, 2 * BN);
+    }
+}
+
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_fn() {
+    static EncodeTiledFn fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void* ptr = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<EncodeTiledFn>(ptr);
+    });
+    return fn;
+}
+
+// [rows][cols] matrix of `type` (elements of `size` bytes, row stride rs bytes)
+// as a 2-D map with 128-byte swizzle and a box of 128 bytes x box_rows.
+int make_tmap_2d(CUtensorMap* map, CUtensorMapDataType type, int size, const void* base, int64_t rows, int64_t cols,
+                 int64_t rs, int box_rows) {
+    EncodeTiledFn enc = encode_fn();
+    if (!enc) return HB_ERR_CUDA;
+    if (rows == 1) rs = (cols * size + 15) / 16 * 16;  // never used for addressing
+    cuuint64_t gdim[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    cuuint64_t gstride[1] = {(cuuint64_t)rs};
+    cuuint32_t box[2] = {(cuuint32_t)(128 / size), (cuuint32_t)box_rows}, estride[2] = {1, 1};
+    const CUresult r = enc(map, type, 2, const_cast<void*>(base), gdim, gstride, box, estride,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? HB_OK : HB_ERR_TMA;
+}
+
+std::mutex g_mu;
+unsigned g_configured[64];  // per device: kernels whose shared-memory limit is set
+
+template <class Kernel>
+int configure(Kernel kern, int dev, int slot, int smem) {
+    std::lock_guard<std::mutex> lk(g_mu);
+    if (!(g_configured[dev] >> slot & 1u)) {
+        HB_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        g_configured[dev] |= 1u << slot;
+    }
+    return HB_OK;
+}
+
+template <bool BF16, int BT>
+int launch_tile(const Int8Problem& q, GemmParams& p, int dev, const DeviceInfo& di, cudaStream_t st) {
+    using C = TileCfg<BT>;
+    auto kern = k_int8_tile<BF16, BT>;
+    constexpr int slot = 8 + BF16 * 4 + (BT == 16 ? 0 : BT == 32 ? 1 : BT == 64 ? 2 : 3);
+    int rc;
+    if ((rc = configure(kern, dev, slot, C::SMEM))) return rc;
+    if ((rc = make_tmap_2d(&p.tmap_x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, q.x, p.M, p.K, q.x_rs, BT))) return rc;
+    if ((rc = make_tmap_2d(&p.tmap_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, q.w, p.N, p.K, q.w_rs, C::BC))) return rc;
+    const int64_t tn = ceil_div(p.N, C::BC), tm = ceil_div(p.M, BT);
+    if (tm > 65535) return HB_ERR_UNSUPPORTED;
+    const int nkb = (int)ceil_div(p.K, C::BK);
+    int split = 1;  // fill the SMs: double while half of them would be idle (clusters of two CTAs per SM do not all fit at once)
+    while (split < 8 && tn * tm * split * 2 <= di.sms && nkb >= 4 * split) split *= 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(tn * split), (unsigned)tm);
+    cfg.blockDim = dim3(256);
+    cfg.dynamicSmemBytes = C::SMEM;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = split;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = split > 1;
+    HB_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, p, split));
+    return HB_OK;
+}
+
+// CTA pairs that can be resident at once (every SM, unless pairs do not fit some).
+template <class C, class Kernel>
+int max_pairs(Kernel kern, int dev, int* pairs) {
+    static int known[64];
+    std::lock_guard<std::mutex> lk(g_mu);
+    int& n = known[dev];
+    if (!n) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(2);
+        cfg.blockDim = dim3(C::THREADS);
+        cfg.dynamicSmemBytes = C::SMEM;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = 2;
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        HB_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, kern, &cfg));
+        if (n <= 0) {
+            n = 0;
+            return HB_ERR_UNSUPPORTED;
+        }
+    }
+    *pairs = n;
+    return HB_OK;
+}
+
+template <bool BF16, int ACT, int BN>
+int launch_pair(const Int8Problem& q, GemmParams& p, int dev, cudaStream_t st) {
+    using C = PairCfg<BN>;
+    auto kern = k_int8_pair<BF16, ACT, BN>;
+    int pairs = 0, rc;
+    if ((rc = configure(kern, dev, BF16 * 4 + ACT * 2 + (BN == 256), C::SMEM))) return rc;
+    if ((rc = max_pairs<C>(kern, dev, &pairs))) return rc;
+    if ((rc = make_tmap_2d(&p.tmap_x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, q.x, p.M, p.K, q.x_rs, 128))) return rc;
+    if ((rc = make_tmap_2d(&p.tmap_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, q.w, p.N, p.K, q.w_rs, BN / 2))) return rc;
+    p.tiles_m = (int)ceil_div(p.M, C::BM);
+    p.tiles_n = (int)ceil_div(p.N, BN);
+    p.tma_out = aligned(p.out, 16) && (p.M == 1 || p.out_rs % 8 == 0);
+    if (p.tma_out &&
+        (rc = make_tmap_2d(&p.tmap_out, BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, p.out,
+                           p.M, p.N, p.out_rs * 2, 32)))
+        return rc;
+    const int tiles = p.tiles_m * p.tiles_n;
+    kern<<<2 * std::min(tiles, pairs), C::THREADS, C::SMEM, st>>>(p);
+    HB_LAUNCH_CHECK();
+    return HB_OK;
+}
+
+template <bool BF16, int BN>
+int launch_pair(const Int8Problem& q, GemmParams& p, int dev, cudaStream_t st) {
+    return p.act ? launch_pair<BF16, 1, BN>(q, p, dev, st) : launch_pair<BF16, 0, BN>(q, p, dev, st);
+}
+
+template <bool BF16>
+int launch_gemm(const Int8Problem& q, GemmParams& p, int dev, const DeviceInfo& di, cudaStream_t st) {
+    if (p.M <= 16) return launch_tile<BF16, 16>(q, p, dev, di, st);
+    if (p.M <= 32) return launch_tile<BF16, 32>(q, p, dev, di, st);
+    if (p.M <= 64) return launch_tile<BF16, 64>(q, p, dev, di, st);
+    if (p.M > 128 && ceil_div(p.M, 256) * ceil_div(p.N, 256) >= 37) return launch_pair<BF16, 256>(q, p, dev, st);
+    if (p.M > 128 && ceil_div(p.M, 256) * ceil_div(p.N, 128) >= 37) return launch_pair<BF16, 128>(q, p, dev, st);
+    return launch_tile<BF16, 128>(q, p, dev, di, st);
+}
+
+}  // namespace
+
+int launch_int8_gemm(const Int8Problem& q, int dev, const DeviceInfo& di, cudaStream_t st) {
+    GemmParams p;
+    p.x_scales = q.x_scales;
+    p.w_scales = q.w_scales;
+    p.bias = q.bias;
+    p.out = q.out;
+    p.out_rs = q.out_rs;
+    p.M = q.M;
+    p.N = q.N;
+    p.K = q.K;
+    p.act = q.act;
+    p.timeout = 2000LL * di.clock_khz;
+    return q.dtype == 1 ? launch_gemm<true>(q, p, dev, di, st) : launch_gemm<false>(q, p, dev, di, st);
+}
+
+}  // namespace hb
+
+using namespace hb;
+
+extern "C" int hb_int8_status(int clear, int32_t* bits, void* stream) {
+    if (!bits) return HB_ERR_ARG;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    HB_CUDA_TRY(cudaMemcpyFromSymbolAsync(bits, g_int8_status, sizeof(int32_t), 0, cudaMemcpyDeviceToHost, st));
+    HB_CUDA_TRY(cudaStreamSynchronize(st));
+    if (clear && *bits) {
+        static const int32_t zero = 0;
+        HB_CUDA_TRY(cudaMemcpyToSymbolAsync(g_int8_status, &zero, sizeof(int32_t), 0, cudaMemcpyHostToDevice, st));
+        HB_CUDA_TRY(cudaStreamSynchronize(st));
+    }
+    return HB_OK;
+}
