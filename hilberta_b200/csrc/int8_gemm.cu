@@ -1,6 +1,6 @@
 // 8-bit products on the tensor cores (tcgen05 kind::i8, 32-bit integer sums in TMEM):
-// 256 x 256 or 256 x 128 tiles by CTA pairs for many tokens, 128 channels x up to 128
-// tokens by single CTAs, which may split K, for few.
+// 256 x 256 tiles by CTA pairs for large products, 128 channels x up to 128 tokens by
+// single CTAs, which may split K, for small ones.
 #include <algorithm>
 #include <climits>
 #include <mutex>
@@ -41,26 +41,28 @@ template <int BT>
 struct TileCfg {
     static constexpr int BC = 128, BK = 128;
     static constexpr int W_BYTES = BC * BK, X_BYTES = BT * BK, STAGE = W_BYTES + X_BYTES;
-    static constexpr int STAGES = 104 * 1024 / STAGE;  // two CTAs per SM
+    // Copies take over a microsecond: a CTA that has an SM to itself keeps twice the
+    // bytes in flight of one that shares it.
+    static constexpr int STAGES = 104 * 1024 / STAGE, STAGES_ALONE = 208 * 1024 / STAGE;
     static constexpr int PITCH = BC;                   // words between tokens' partial sums
     static constexpr int HALF = BT / 2;                // tokens per warp in the epilogue: two warps share a channel
     static constexpr int TMEM_COLS = BT < 64 ? 64 : BT;  // loads of 32 columns from the second half on stay inside
     struct Ctl {
-        uint64_t full[STAGES], empty[STAGES], done;
+        uint64_t full[STAGES_ALONE], empty[STAGES_ALONE], done;
         uint32_t tmem_base;
         int abort;
         float scales[BT + 8];  // of the tokens, read eight at a time
     };
-    static constexpr int CTL_OFF = STAGES * STAGE;
-    static constexpr int SMEM = CTL_OFF + (int)((sizeof(Ctl) + 15) / 16 * 16);
-    static_assert(BT * PITCH * 4 <= CTL_OFF, "partial sums reuse the stages");
+    static constexpr int smem(int stages) { return stages * STAGE + (int)((sizeof(Ctl) + 15) / 16 * 16); }
+    static_assert((BT + 8) * PITCH * 4 <= STAGES * STAGE, "partial sums reuse the stages");
+    static_assert(STAGES_ALONE * STAGE + (int)sizeof(Ctl) + 16 <= 227 * 1024, "shared memory of one CTA");
 };
 
 template <bool BF16, int BT>
-__global__ void __launch_bounds__(256, 2) k_int8_tile(const __grid_constant__ GemmParams p, int split) {
+__global__ void __launch_bounds__(256, 2) k_int8_tile(const __grid_constant__ GemmParams p, int split, int stages) {
     using C = TileCfg<BT>;
     extern __shared__ __align__(1024) uint8_t smem[];
-    auto* ctl = reinterpret_cast<typename C::Ctl*>(smem + C::CTL_OFF);
+    auto* ctl = reinterpret_cast<typename C::Ctl*>(smem + stages * C::STAGE);
     constexpr int U = 8;  // tokens finished together
     volatile int* abort_flag = &ctl->abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -76,7 +78,7 @@ __global__ void __launch_bounds__(256, 2) k_int8_tile(const __grid_constant__ Ge
     if (warp == 0 && lane == 0) {
         prefetch_tmap(&p.tmap_x);
         prefetch_tmap(&p.tmap_w);
-        for (int i = 0; i < C::STAGES; i++) {
+        for (int i = 0; i < stages; i++) {
             mbar_init(&ctl->full[i], 1);
             mbar_init(&ctl->empty[i], 1);
         }
@@ -98,11 +100,10 @@ __global__ void __launch_bounds__(256, 2) k_int8_tile(const __grid_constant__ Ge
     const uint32_t tmem = ctl->tmem_base;
 
     if (warp == 0 && lane == 0) {
-        int it = 0;
         bool ok = true;
+        int s = 0, round = 0, it = 0;
         for (int kb = kb0; kb < kb1; kb++, it++) {
-            const int s = it % C::STAGES;
-            if (it >= C::STAGES && !mbar_wait(&ctl->empty[s], (it / C::STAGES - 1) & 1, abort_flag, p.timeout)) {
+            if (round > 0 && !mbar_wait(&ctl->empty[s], (round - 1) & 1, abort_flag, p.timeout)) {
                 ok = false;
                 break;
             }
@@ -110,19 +111,19 @@ __global__ void __launch_bounds__(256, 2) k_int8_tile(const __grid_constant__ Ge
             mbar_arrive_expect_tx(&ctl->full[s], C::STAGE);
             tma_load_2d(st, &p.tmap_w, &ctl->full[s], kb * C::BK, n0);
             tma_load_2d(st + C::W_BYTES, &p.tmap_x, &ctl->full[s], kb * C::BK, m0);
+            if (++s == stages) s = 0, round++;
         }
         if (!ok) {  // let the copies in flight land before the CTA gives up its memory
             volatile int ignore = 0;
-            for (int j = max(0, it - C::STAGES); j < it; j++)
-                mbar_wait(&ctl->full[j % C::STAGES], (j / C::STAGES) & 1, &ignore, p.timeout);
+            for (int j = max(0, it - stages); j < it; j++)
+                mbar_wait(&ctl->full[j % stages], (j / stages) & 1, &ignore, p.timeout);
         }
     } else if (warp == 1 && lane == 0) {
         constexpr uint32_t idesc = idesc_i8(C::BC, BT);
         bool ok = true;
-        int it = 0;
-        for (int kb = kb0; kb < kb1; kb++, it++) {
-            const int s = it % C::STAGES;
-            if (!mbar_wait(&ctl->full[s], (it / C::STAGES) & 1, abort_flag, p.timeout)) {
+        int s = 0, round = 0;
+        for (int kb = kb0; kb < kb1; kb++) {
+            if (!mbar_wait(&ctl->full[s], round & 1, abort_flag, p.timeout)) {
                 ok = false;
                 break;
             }
@@ -130,8 +131,9 @@ __global__ void __launch_bounds__(256, 2) k_int8_tile(const __grid_constant__ Ge
             const uint32_t w = smem_u32(smem + s * C::STAGE), x = w + C::W_BYTES;
 #pragma unroll
             for (int k = 0; k < C::BK; k += 32)
-                mma_i8_ss(tmem, desc_sw128(w + k, 16, 1024), desc_sw128(x + k, 16, 1024), idesc, it > 0 || k > 0);
+                mma_i8_ss(tmem, desc_sw128(w + k, 16, 1024), desc_sw128(x + k, 16, 1024), idesc, kb > kb0 || k > 0);
             tc_commit(&ctl->empty[s]);
+            if (++s == stages) s = 0, round++;
         }
         if (ok) tc_commit(&ctl->done);
     }
@@ -220,16 +222,15 @@ __global__ void __launch_bounds__(256, 2) k_int8_tile(const __grid_constant__ Ge
     }
 }
 
-// 256 x BN (256 or 128) output tiles by CTA pairs, persistent.  One MMA of a pair
-// covers 256 x BN x 32: each CTA stages 128 rows of the tokens and BN / 2 of the
-// weights, so it reads half of the weight tile's bytes that it would need alone, and
-// both keep 128 rows of the accumulator.  Two accumulators (all of the TMEM at BN
-// 256): the epilogue of a tile runs under the products of the next.
-template <int BN_>
+// 256 x 256 output tiles by CTA pairs, persistent.  One MMA of a pair covers 256
+// x 256 x 32: each CTA stages 128 rows of both operands, so a CTA reads half of
+// the weight tile's bytes that it would need alone, and both keep 128 rows of the
+// accumulator.  Two accumulators fill the TMEM: the epilogue of a tile runs under
+// the products of the next.
 struct PairCfg {
-    static constexpr int BM = 256, BN = BN_, BK = 128;
-    static constexpr int A_BYTES = 128 * BK, B_BYTES = BN / 2 * BK, STAGE = A_BYTES + B_BYTES;
-    static constexpr int STAGES = 192 * 1024 / STAGE;
+    static constexpr int BM = 256, BN = 256, BK = 128;
+    static constexpr int A_BYTES = 128 * BK, B_BYTES = 128 * BK, STAGE = A_BYTES + B_BYTES;
+    static constexpr int STAGES = 6;
     static constexpr int EPI_WARPS = 8;         // two per TMEM lane quarter, half of the columns each
     static constexpr int STAGING = 32 * 128;    // per warp: 32 rows x 64 columns of the output
     static constexpr int THREADS = 128 + 32 * EPI_WARPS;
@@ -248,21 +249,20 @@ struct PairCfg {
     static constexpr int GROUP = 8;
 };
 
-template <class C>
 __device__ __forceinline__ void pair_tile(const GemmParams& p, int t, int& m0, int& n0) {
-    const int per = C::GROUP * p.tiles_n;
+    const int per = PairCfg::GROUP * p.tiles_n;
     const int g = t / per, r = t - g * per;
-    const int gm = min(C::GROUP, p.tiles_m - g * C::GROUP);
-    m0 = (g * C::GROUP + r % gm) * C::BM;
-    n0 = r / gm * C::BN;
+    const int gm = min(PairCfg::GROUP, p.tiles_m - g * PairCfg::GROUP);
+    m0 = (g * PairCfg::GROUP + r % gm) * PairCfg::BM;
+    n0 = r / gm * PairCfg::BN;
 }
 
-template <bool BF16, int ACT, int BN>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<BN>::THREADS, 1)
+template <bool BF16, int ACT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::THREADS, 1)
     k_int8_pair(const __grid_constant__ GemmParams p) {
-    using C = PairCfg<BN>;
+    using C = PairCfg;
     extern __shared__ __align__(1024) uint8_t smem[];
-    auto* ctl = reinterpret_cast<typename C::Ctl*>(smem + C::CTL_OFF);
+    auto* ctl = reinterpret_cast<C::Ctl*>(smem + C::CTL_OFF);
     volatile int* abort_flag = &ctl->abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = (int)cluster_rank();
@@ -289,7 +289,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<BN>::THREADS
         if (p.tma_out) prefetch_tmap(&p.tmap_out);
     }
     if (warp == 2) {
-        tmem_alloc_pair(&ctl->tmem_base, 2 * BN);
+        tmem_alloc_pair(&ctl->tmem_base, 512);
         tc_fence_before();
     }
     __syncthreads();
@@ -303,7 +303,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<BN>::THREADS
             bool ok = true;
             for (int t = first; t < tiles && ok; t += step) {
                 int m0, n0;
-                pair_tile<C>(p, t, m0, n0);
+                pair_tile(p, t, m0, n0);
                 for (int kb = 0; kb < nkb; kb++, it++) {
                     const int s = it % C::STAGES;
                     if (it >= C::STAGES &&
@@ -315,7 +315,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<BN>::THREADS
                     if (rank == 0) mbar_arrive_expect_tx(&ctl->full[s], 2 * C::STAGE);
                     const uint32_t bar = cluster_map(smem_u32(&ctl->full[s]), 0);
                     tma_load_2d_pair(st, &p.tmap_x, bar, kb * C::BK, m0 + 128 * rank);
-                    tma_load_2d_pair(st + C::A_BYTES, &p.tmap_w, bar, kb * C::BK, n0 + BN / 2 * rank);
+                    tma_load_2d_pair(st + C::A_BYTES, &p.tmap_w, bar, kb * C::BK, n0 + 128 * rank);
                 }
             }
             if (!ok) {  // gave up: time for the copies and MMAs in flight to end before the memory is given back
@@ -330,7 +330,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<BN>::THREADS
             int it = 0, i = 0;
             bool ok = true;
             for (int t = first; t < tiles && ok; t += step, i++) {
-                const uint32_t d = tmem + (i & 1) * BN;
+                const uint32_t d = tmem + (i & 1) * C::BN;
                 if (i >= 2 && !mbar_wait_cluster(&ctl->acc_empty[i & 1], (i / 2 - 1) & 1, abort_flag, p.timeout)) break;
                 tc_fence_after();
                 for (int kb = 0; kb < nkb; kb++, it++) {
@@ -352,22 +352,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<BN>::THREADS
     } else if (warp >= 4) {
         const int ew = warp - 4, quarter = warp & 3, half = ew >> 2;
         uint8_t* stg = smem + C::STG_OFF + ew * C::STAGING;
-        float2* cols = ctl->cols + BN / 2 * half;
+        float2* cols = ctl->cols + 128 * half;
         int i = 0;
         bool dead = false;  // a wait ran out: only the barriers of the remaining tiles are kept, so that no warp is left at one
         for (int t = first; t < tiles; t += step, i++) {
             int m0, n0;
-            pair_tile<C>(p, t, m0, n0);
-            const int row0 = m0 + 128 * rank + 32 * quarter, col0 = n0 + BN / 2 * half;
+            pair_tile(p, t, m0, n0);
+            const int row0 = m0 + 128 * rank + 32 * quarter, col0 = n0 + 128 * half;
             {  // this half's column scales and biases (its four warps only)
                 const int c = threadIdx.x & 127;
                 float2 v = make_float2(0.f, 0.f);
-                if (c < BN / 2 && col0 + c < p.N) {
+                if (col0 + c < p.N) {
                     v.x = p.w_scales[col0 + c];
                     if (p.bias) v.y = load16<BF16>(p.bias + col0 + c);
                 }
                 asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");
-                if (c < BN / 2) cols[c] = v;
+                cols[c] = v;
                 asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");
             }
             if (dead) continue;
@@ -379,15 +379,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<BN>::THREADS
                 continue;
             }
             tc_fence_after();
-            const uint32_t acc = tmem + ((uint32_t)(32 * quarter) << 16) + (i & 1) * BN + BN / 2 * half;
+            const uint32_t acc = tmem + ((uint32_t)(32 * quarter) << 16) + (i & 1) * C::BN + 128 * half;
 #pragma unroll
-            for (int c = 0; c < BN / 2; c += 64) {
+            for (int c = 0; c < 128; c += 64) {
                 uint32_t lo[32], hi[32];
                 tmem_ld32_async(acc + c, lo);
                 tmem_ld32_async(acc + c + 32, hi);
                 tmem_wait_ld(lo);
                 tmem_wait_ld(hi);
-                if (c + 64 == BN / 2) {  // the accumulator is in registers: the next tile but one may take its place
+                if (c == 64) {  // the accumulator is in registers: the next tile but one may take its place
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive_cluster(cluster_map(smem_u32(&ctl->acc_empty[i & 1]), 0));
@@ -417,14 +417,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<BN>::THREADS
                     }
                 } else {
                     __syncwarp();
-                    for (int r = 0; r < 32 && row0 + r < p.M; r++)
+                    // a lane per column and the next but 31, eight rows' values at a time
+                    uint16_t* dst = p.out + (int64_t)row0 * p.out_rs + col0 + c + lane;
+                    const bool in0 = col0 + c + lane < p.N, in1 = col0 + c + lane + 32 < p.N;
+                    for (int r = 0; r < 32 && row0 + r < p.M; r += 8, dst += 8 * p.out_rs) {
+                        uint16_t v[16];
 #pragma unroll
-                        for (int k = 0; k < 64; k += 32) {
-                            const int x = k + lane;
-                            if (col0 + c + x < p.N)
-                                p.out[(int64_t)(row0 + r) * p.out_rs + col0 + c + x] = *reinterpret_cast<const uint16_t*>(
-                                    stg + r * 128 + (((x >> 3) ^ (r & 7)) << 4) + (x & 7) * 2);
+                        for (int e = 0; e < 8; e++) {
+                            const uint8_t* line = stg + (r + e) * 128 + (lane & 7) * 2;
+                            v[2 * e] = *reinterpret_cast<const uint16_t*>(line + (((lane >> 3) ^ e) << 4));
+                            v[2 * e + 1] = *reinterpret_cast<const uint16_t*>(line + (((lane >> 3) + 4 ^ e) << 4));
                         }
+#pragma unroll
+                        for (int e = 0; e < 8; e++) {
+                            if (row0 + r + e < p.M) {
+                                if (in0) dst[e * p.out_rs] = v[2 * e];
+                                if (in1) dst[e * p.out_rs + 32] = v[2 * e + 1];
+                            }
+                        }
+                    }
                     __syncwarp();
                 }
             }
@@ -436,7 +447,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<BN>::THREADS
     cluster_sync();  // no CTA leaves while the other's MMAs read its memory or arrivals are on the way
     if (warp == 2) {
         tc_fence_after();
-        tmem_dealloc_pair(tmem, 2 * BN);
+        tmem_dealloc_pair(tmem, 512);
     }
 }
 
@@ -486,24 +497,35 @@ int configure(Kernel kern, int dev, int slot, int smem) {
     return HB_OK;
 }
 
+// CTAs that split K: doubled while each has an SM to itself, with two blocks of K at
+// least.  Clusters of four and more count 16 SMs of each of the eight processing
+// clusters only: the others cannot hold a whole one, and a second wave of a few
+// clusters costs as much as the first (128 x 3072, K 3072: 8.9 us with 2 CTAs for K,
+// 14.9 us with 3 on 144 SMs).
+int tile_split(const GemmParams& p, int bt, int sms) {
+    const int64_t tiles = ceil_div(p.N, 128) * ceil_div(p.M, bt), nkb = ceil_div(p.K, 128);
+    int split = 1;
+    while (split < 8 && tiles * split * 2 <= (split == 1 ? sms : std::min(sms, 128)) && nkb >= 4 * split) split *= 2;
+    return split;
+}
+
 template <bool BF16, int BT>
 int launch_tile(const Int8Problem& q, GemmParams& p, int dev, const DeviceInfo& di, cudaStream_t st) {
     using C = TileCfg<BT>;
     auto kern = k_int8_tile<BF16, BT>;
     constexpr int slot = 8 + BF16 * 4 + (BT == 16 ? 0 : BT == 32 ? 1 : BT == 64 ? 2 : 3);
     int rc;
-    if ((rc = configure(kern, dev, slot, C::SMEM))) return rc;
+    if ((rc = configure(kern, dev, slot, C::smem(C::STAGES_ALONE)))) return rc;
     if ((rc = make_tmap_2d(&p.tmap_x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, q.x, p.M, p.K, q.x_rs, BT))) return rc;
     if ((rc = make_tmap_2d(&p.tmap_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, q.w, p.N, p.K, q.w_rs, C::BC))) return rc;
     const int64_t tn = ceil_div(p.N, C::BC), tm = ceil_div(p.M, BT);
     if (tm > 65535) return HB_ERR_UNSUPPORTED;
-    const int nkb = (int)ceil_div(p.K, C::BK);
-    int split = 1;  // fill the SMs: double while half of them would be idle (clusters of two CTAs per SM do not all fit at once)
-    while (split < 8 && tn * tm * split * 2 <= di.sms && nkb >= 4 * split) split *= 2;
+    const int split = tile_split(p, BT, di.sms);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(tn * split), (unsigned)tm);
     cfg.blockDim = dim3(256);
-    cfg.dynamicSmemBytes = C::SMEM;
+    const int stages = tn * tm * split <= di.sms ? C::STAGES_ALONE : C::STAGES;
+    cfg.dynamicSmemBytes = C::smem(stages);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -512,12 +534,12 @@ int launch_tile(const Int8Problem& q, GemmParams& p, int dev, const DeviceInfo& 
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = split > 1;
-    HB_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, p, split));
+    HB_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, p, split, stages));
     return HB_OK;
 }
 
 // CTA pairs that can be resident at once (every SM, unless pairs do not fit some).
-template <class C, class Kernel>
+template <class Kernel>
 int max_pairs(Kernel kern, int dev, int* pairs) {
     static int known[64];
     std::lock_guard<std::mutex> lk(g_mu);
@@ -525,8 +547,8 @@ int max_pairs(Kernel kern, int dev, int* pairs) {
     if (!n) {
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(2);
-        cfg.blockDim = dim3(C::THREADS);
-        cfg.dynamicSmemBytes = C::SMEM;
+        cfg.blockDim = dim3(PairCfg::THREADS);
+        cfg.dynamicSmemBytes = PairCfg::SMEM;
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeClusterDimension;
         attr[0].val.clusterDim.x = 2;
@@ -544,17 +566,17 @@ int max_pairs(Kernel kern, int dev, int* pairs) {
     return HB_OK;
 }
 
-template <bool BF16, int ACT, int BN>
+template <bool BF16, int ACT>
 int launch_pair(const Int8Problem& q, GemmParams& p, int dev, cudaStream_t st) {
-    using C = PairCfg<BN>;
-    auto kern = k_int8_pair<BF16, ACT, BN>;
+    using C = PairCfg;
+    auto kern = k_int8_pair<BF16, ACT>;
     int pairs = 0, rc;
-    if ((rc = configure(kern, dev, BF16 * 4 + ACT * 2 + (BN == 256), C::SMEM))) return rc;
-    if ((rc = max_pairs<C>(kern, dev, &pairs))) return rc;
+    if ((rc = configure(kern, dev, BF16 * 2 + ACT, C::SMEM))) return rc;
+    if ((rc = max_pairs(kern, dev, &pairs))) return rc;
     if ((rc = make_tmap_2d(&p.tmap_x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, q.x, p.M, p.K, q.x_rs, 128))) return rc;
-    if ((rc = make_tmap_2d(&p.tmap_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, q.w, p.N, p.K, q.w_rs, BN / 2))) return rc;
+    if ((rc = make_tmap_2d(&p.tmap_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, q.w, p.N, p.K, q.w_rs, 128))) return rc;
     p.tiles_m = (int)ceil_div(p.M, C::BM);
-    p.tiles_n = (int)ceil_div(p.N, BN);
+    p.tiles_n = (int)ceil_div(p.N, C::BN);
     p.tma_out = aligned(p.out, 16) && (p.M == 1 || p.out_rs % 8 == 0);
     if (p.tma_out &&
         (rc = make_tmap_2d(&p.tmap_out, BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, p.out,
@@ -566,18 +588,30 @@ int launch_pair(const Int8Problem& q, GemmParams& p, int dev, cudaStream_t st) {
     return HB_OK;
 }
 
-template <bool BF16, int BN>
-int launch_pair(const Int8Problem& q, GemmParams& p, int dev, cudaStream_t st) {
-    return p.act ? launch_pair<BF16, 1, BN>(q, p, dev, st) : launch_pair<BF16, 0, BN>(q, p, dev, st);
+// Expected times in hundredths of a microsecond, from 70 shapes (65 to 4096 tokens, 640
+// to 12288 channels, K 256 to 12288) timed with every kernel.  A k-block of 128 bytes
+// takes a CTA (or a pair) about 0.28 us, two CTAs of an SM together 0.47 us; the fixed
+// parts are the launch, the first copies and a tile's way out.  At the crossings: 768 x
+// 3072, K 3072 12.5 us in tiles of 128 tokens and 13.7 us in pairs, 1024 tokens 15.5
+// and 14.2 us; 512 x 3072 12.6 us in tiles of 64 and 12.2 us of 128, 192 tokens 9.1
+// and 10.6 us.
+int64_t tile_cost(const GemmParams& p, int bt, int sms) {
+    const int64_t split = tile_split(p, bt, sms);
+    const int64_t waves = ceil_div(ceil_div(p.N, 128) * ceil_div(p.M, bt) * split, sms), kb = ceil_div(ceil_div(p.K, 128), split);
+    return (bt == 128 ? 550 : 430) + (split > 1 ? 100 : 0) + (waves - 1) * 130 + kb * (waves == 1 ? 28 : waves * 47 / 2);
+}
+int64_t pair_cost(const GemmParams& p, int sms) {
+    return 700 + ceil_div(p.K, 128) * 29 * ceil_div(ceil_div(p.M, 256) * ceil_div(p.N, 256), sms / 2);
 }
 
 template <bool BF16>
 int launch_gemm(const Int8Problem& q, GemmParams& p, int dev, const DeviceInfo& di, cudaStream_t st) {
     if (p.M <= 16) return launch_tile<BF16, 16>(q, p, dev, di, st);
     if (p.M <= 32) return launch_tile<BF16, 32>(q, p, dev, di, st);
-    if (p.M <= 64) return launch_tile<BF16, 64>(q, p, dev, di, st);
-    if (p.M > 128 && ceil_div(p.M, 256) * ceil_div(p.N, 256) >= 37) return launch_pair<BF16, 256>(q, p, dev, st);
-    if (p.M > 128 && ceil_div(p.M, 256) * ceil_div(p.N, 128) >= 37) return launch_pair<BF16, 128>(q, p, dev, st);
+    const int64_t narrow = tile_cost(p, 64, di.sms), wide = tile_cost(p, 128, di.sms);
+    if (p.M > 64 && pair_cost(p, di.sms) < std::min(narrow, wide))
+        return p.act ? launch_pair<BF16, 1>(q, p, dev, st) : launch_pair<BF16, 0>(q, p, dev, st);
+    if (p.M <= 64 || narrow <= wide) return launch_tile<BF16, 64>(q, p, dev, di, st);
     return launch_tile<BF16, 128>(q, p, dev, di, st);
 }
 
