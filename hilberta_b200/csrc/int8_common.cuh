@@ -62,17 +62,35 @@ __device__ __forceinline__ uint2 codes8(const uint4& v, const RowScale& s) {
 
 // tanh-GELU(v) = v / (1 + exp(-2u)), u = sqrt(2/pi) (v + 0.044715 v^3), the
 // exponential taken in base 2.
-__device__ __forceinline__ float gelu_tanh(float v) {
-    const float k0 = -2.f * 1.4426950408889634f * 0.7978845608028654f;
-    const float e = ptx::ex2(v * fmaf(k0 * 0.044715f, v * v, k0));
+constexpr float kGelu0 = -2.f * 1.4426950408889634f * 0.7978845608028654f, kGelu1 = kGelu0 * 0.044715f;
+__device__ __forceinline__ float rcp(float x) {
     float r;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
-    return v * r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float gelu_tanh(float v) {
+    return v * rcp(1.f + ptx::ex2(v * fmaf(kGelu1, v * v, kGelu0)));
 }
 template <int ACT>
 __device__ __forceinline__ float finish(int acc, float sx, float sw, float b) {
     const float v = fmaf(__int2float_rn(acc) * sx, sw, b);
     return ACT ? gelu_tanh(v) : v;
+}
+// Two neighbouring columns at once, the same operations in packed fp32: sx the row's
+// scale twice, sw and b the columns' scales and biases; packed to 16 bits.
+template <bool BF16, int ACT>
+__device__ __forceinline__ uint32_t finish2(int acc0, int acc1, uint64_t sx, uint64_t sw, uint64_t b) {
+    using namespace ptx;
+    uint64_t v = f2_fma(f2_mul(f2_pack(__int2float_rn(acc0), __int2float_rn(acc1)), sx), sw, b);
+    float lo, hi;
+    if constexpr (ACT) {
+        const uint64_t k0 = f2_pack(kGelu0, kGelu0), k1 = f2_pack(kGelu1, kGelu1), one = f2_pack(1.f, 1.f);
+        f2_unpack(f2_mul(v, f2_fma(k1, f2_mul(v, v), k0)), lo, hi);
+        f2_unpack(f2_add(f2_pack(ex2(lo), ex2(hi)), one), lo, hi);
+        v = f2_mul(v, f2_pack(rcp(lo), rcp(hi)));
+    }
+    f2_unpack(v, lo, hi);
+    return pack2<BF16>(lo, hi);
 }
 
 struct DeviceInfo {

@@ -238,7 +238,8 @@ struct PairCfg {
         uint64_t full[STAGES], empty[STAGES], acc_full[2], acc_empty[2];
         uint32_t tmem_base;
         int abort;
-        alignas(16) float2 cols[BN];  // weight scale and bias of the tile's columns, read two at a time
+        alignas(16) float col_scale[BN];  // of the tile's columns
+        alignas(16) float col_bias[BN];
     };
     static constexpr int STG_OFF = STAGES * STAGE;
     static constexpr int CTL_OFF = STG_OFF + EPI_WARPS * STAGING;
@@ -352,7 +353,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::THREADS, 1)
     } else if (warp >= 4) {
         const int ew = warp - 4, quarter = warp & 3, half = ew >> 2;
         uint8_t* stg = smem + C::STG_OFF + ew * C::STAGING;
-        float2* cols = ctl->cols + 128 * half;
+        float *col_scale = ctl->col_scale + 128 * half, *col_bias = ctl->col_bias + 128 * half;
         int i = 0;
         bool dead = false;  // a wait ran out: only the barriers of the remaining tiles are kept, so that no warp is left at one
         for (int t = first; t < tiles; t += step, i++) {
@@ -361,17 +362,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::THREADS, 1)
             const int row0 = m0 + 128 * rank + 32 * quarter, col0 = n0 + 128 * half;
             {  // this half's column scales and biases (its four warps only)
                 const int c = threadIdx.x & 127;
-                float2 v = make_float2(0.f, 0.f);
+                float scale = 0.f, bias = 0.f;
                 if (col0 + c < p.N) {
-                    v.x = p.w_scales[col0 + c];
-                    if (p.bias) v.y = load16<BF16>(p.bias + col0 + c);
+                    scale = p.w_scales[col0 + c];
+                    if (p.bias) bias = load16<BF16>(p.bias + col0 + c);
                 }
                 asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");
-                cols[c] = v;
+                col_scale[c] = scale;
+                col_bias[c] = bias;
                 asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");
             }
             if (dead) continue;
-            const float sx = row0 + lane < p.M ? p.x_scales[row0 + lane] : 0.f;
+            const float row_scale = row0 + lane < p.M ? p.x_scales[row0 + lane] : 0.f;
+            const uint64_t sx = f2_pack(row_scale, row_scale);
             const bool ok = mbar_wait_cluster(&ctl->acc_full[i & 1], (i >> 1) & 1, abort_flag, p.timeout);
             if (!__all_sync(FULL, ok)) {
                 if (lane == 0) atomicOr(&g_int8_status, HB_DEV_TIMEOUT);
@@ -398,12 +401,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::THREADS, 1)
                 for (int j = 0; j < 8; j++) {
                     uint32_t o[4];
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
+                    for (int e = 0; e < 4; e += 2) {  // four columns
                         const int x = 8 * j + 2 * e;
-                        const float4 sb = *reinterpret_cast<const float4*>(cols + c + x);
-                        const int u = (int)(x < 32 ? lo[x & 31] : hi[x & 31]);
-                        const int v = (int)(x < 32 ? lo[(x + 1) & 31] : hi[(x + 1) & 31]);
-                        o[e] = pack2<BF16>(finish<ACT>(u, sx, sb.x, sb.y), finish<ACT>(v, sx, sb.z, sb.w));
+                        const ulonglong2 sw = *reinterpret_cast<const ulonglong2*>(col_scale + c + x);
+                        const ulonglong2 sb = *reinterpret_cast<const ulonglong2*>(col_bias + c + x);
+                        const uint32_t(&r)[32] = x < 32 ? lo : hi;
+                        o[e] = finish2<BF16, ACT>((int)r[x & 31], (int)r[(x + 1) & 31], sx, sw.x, sb.x);
+                        o[e + 1] = finish2<BF16, ACT>((int)r[(x + 2) & 31], (int)r[(x + 3) & 31], sx, sw.y, sb.y);
                     }
                     // 128-byte rows with the map's swizzle: conflict-free 16-byte stores
                     *reinterpret_cast<uint4*>(stg + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
