@@ -28,6 +28,7 @@
 #include <cstdint>
 
 #include "common.cuh"
+#include "sm100_ptx.cuh"
 
 namespace hb {
 namespace {
@@ -186,9 +187,13 @@ __global__ void __launch_bounds__(256) k_norm_rope_pack(const __grid_constant__ 
 //   r = rsqrt(mean over D of x^2 + eps),  z = x * r * w,
 //   (z[2i], z[2i+1]) -> (z[2i] cos[2i] - z[2i+1] sin[2i], z[2i+1] cos[2i+1] + z[2i] sin[2i+1])
 // in fp32 with one rounding at the end.  Memory-bound: every row is read and
-// written once.  One warp per (token, run of heads): D / 8 lanes hold a row, the
-// token's cos/sin and the head weights stay in registers over the heads, so they
-// are read once per run instead of once per row.
+// written once.  One warp per (token, run of heads): D / 8 lanes hold a row; the
+// token's cos/sin times the head weights are formed once per run and stay in
+// registers over its heads,
+//   out[2i] = (x r)[2i] w cos[2i] + (x r)[2i+1] (-w[2i+1] sin[2i]),  out[2i+1] likewise,
+// three packed fp32 operations a pair.  What bounds it is the bytes on their way:
+// four rows per lane group, four CTAs per SM (16896 tokens x 48 heads x 128: 68 us, 6.1 TB/s; with
+// three CTAs 78 us, eight rows 92 us).
 struct QkParams {
     const void* x[2];  // query, key: [B][S][H][D]
     void* out[2];      // may equal x
@@ -205,7 +210,8 @@ struct QkParams {
 };
 
 template <int D, bool BF16>
-__global__ void __launch_bounds__(256) k_norm_rope_qk(const __grid_constant__ QkParams p) {
+__global__ void __launch_bounds__(256, 4) k_norm_rope_qk(const __grid_constant__ QkParams p) {
+    using namespace ptx;
     using H16 = Half16<BF16>;
     constexpr int LPR = D / 8;    // lanes per row
     constexpr int RPW = 32 / LPR; // rows (heads) a warp handles at once
@@ -223,7 +229,7 @@ __global__ void __launch_bounds__(256) k_norm_rope_qk(const __grid_constant__ Qk
         const int h1 = min(h0 + p.run, p.H[which]);
         const uint16_t* src = static_cast<const uint16_t*>(p.x[which]) + b * p.x_sb[which] + s * p.x_sn[which] + col;
         uint16_t* dst = static_cast<uint16_t*>(p.out[which]) + b * p.o_sb[which] + s * p.o_sn[which] + col;
-        float cs[8], sn[8], w[8];
+        uint64_t straight[4], crossed[4];  // factors of (x[2i], x[2i+1]) and of (x[2i+1], x[2i])
         {
             const float4* c4 = reinterpret_cast<const float4*>(p.cos + (int64_t)s * D + col);
             const float4* s4 = reinterpret_cast<const float4*>(p.sin + (int64_t)s * D + col);
@@ -231,10 +237,15 @@ __global__ void __launch_bounds__(256) k_norm_rope_qk(const __grid_constant__ Qk
             const uint4 wr = *reinterpret_cast<const uint4*>(
                 static_cast<const uint16_t*>(s < p.T ? p.w_txt[which] : p.w[which]) + col);
             const uint32_t wu[4] = {wr.x, wr.y, wr.z, wr.w};
-            cs[0] = ca.x, cs[1] = ca.y, cs[2] = ca.z, cs[3] = ca.w, cs[4] = cb.x, cs[5] = cb.y, cs[6] = cb.z, cs[7] = cb.w;
-            sn[0] = sa.x, sn[1] = sa.y, sn[2] = sa.z, sn[3] = sa.w, sn[4] = sb.x, sn[5] = sb.y, sn[6] = sb.z, sn[7] = sb.w;
+            const float cs[8] = {ca.x, ca.y, ca.z, ca.w, cb.x, cb.y, cb.z, cb.w};
+            const float sn[8] = {sa.x, sa.y, sa.z, sa.w, sb.x, sb.y, sb.z, sb.w};
 #pragma unroll
-            for (int i = 0; i < 4; i++) H16::unpack(wu[i], w[2 * i], w[2 * i + 1]);
+            for (int i = 0; i < 4; i++) {
+                float w0, w1;
+                H16::unpack(wu[i], w0, w1);
+                straight[i] = f2_pack(w0 * cs[2 * i], w1 * cs[2 * i + 1]);
+                crossed[i] = f2_pack(-w1 * sn[2 * i], w0 * sn[2 * i + 1]);
+            }
         }
         for (int h = h0; h < h1; h += U * RPW) {  // uniform over the warp
             uint4 raw[U];
@@ -247,21 +258,29 @@ __global__ void __launch_bounds__(256) k_norm_rope_qk(const __grid_constant__ Qk
             for (int u = 0; u < U; u++) {
                 const int hh = h + u * RPW + sub;
                 const uint32_t in[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
-                float f[8], ss = 0.f;
+                float f[8];
+                uint64_t sq = 0;
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     H16::unpack(in[i], f[2 * i], f[2 * i + 1]);
-                    ss = fmaf(f[2 * i], f[2 * i], ss);
-                    ss = fmaf(f[2 * i + 1], f[2 * i + 1], ss);
+                    const uint64_t v = f2_pack(f[2 * i], f[2 * i + 1]);
+                    sq = f2_fma(v, v, sq);
                 }
+                float ss, odd;
+                f2_unpack(sq, ss, odd);
+                ss += odd;
 #pragma unroll
                 for (int o = 1; o < LPR; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
                 const float r = rsqrtf(ss * (1.f / D) + p.eps);
+                const uint64_t r2 = f2_pack(r, r);
                 uint32_t o[4];
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const float a = f[2 * i] * r * w[2 * i], c = f[2 * i + 1] * r * w[2 * i + 1];
-                    o[i] = H16::pack(a * cs[2 * i] - c * sn[2 * i], c * cs[2 * i + 1] + a * sn[2 * i + 1]);
+                    float a, c;
+                    const uint64_t t = f2_mul(f2_pack(f[2 * i], f[2 * i + 1]), r2);
+                    f2_unpack(t, a, c);
+                    f2_unpack(f2_fma(f2_pack(c, a), crossed[i], f2_mul(t, straight[i])), a, c);
+                    o[i] = H16::pack(a, c);
                 }
                 if (hh < h1) *reinterpret_cast<uint4*>(dst + hh * p.o_sh[which]) = make_uint4(o[0], o[1], o[2], o[3]);
             }
