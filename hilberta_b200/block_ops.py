@@ -21,7 +21,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .int8 import _empty_rows, _span
+from .int8 import _apart, _empty_rows, _overlaps_itself
 
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1}
 
@@ -126,8 +126,11 @@ def _call_int8(x, y, gate, shift, scale, x_out, eps):
                 raise ValueError(f"{name} must match x's shape, dtype and device")
         y_rs, xo_rs = _rows(y, "y")[1], _rows(x_out, "x_out")[1]
         y_ptr, gate_ptr, xo_ptr = y.data_ptr(), gate.data_ptr(), x_out.data_ptr()
-        if x_out is not x:
-            _check_apart(x_out, x, y, *mods)
+        if _overlaps_itself(x_out):
+            raise ValueError("the new stream must not overlap itself")
+        for t in (x, y, *mods):
+            if not _same_view(x_out, t) and not _apart(x_out, t):
+                raise ValueError("the new stream must be x itself or apart from every input")
     rows = _empty_rows(x.shape, kind, dev)
     with _lib.on_device(dev) as stream:
         rc = _lib.lib().hb_adaln_residual_int8(
@@ -141,13 +144,8 @@ def _call_int8(x, y, gate, shift, scale, x_out, eps):
     return rows
 
 
-def _check_apart(out, *inputs):
-    """``out`` is x itself elsewhere; here it must share no memory with what is read."""
-    begin, end = _span(out)
-    for t in inputs:
-        first, last = _span(t)
-        if begin < last and first < end:
-            raise ValueError("x_out must be x itself or apart from every input")
+def _same_view(a, b):
+    return a.data_ptr() == b.data_ptr() and a.shape == b.shape and a.stride() == b.stride()
 
 
 def adaln_int8(x, shift, scale, eps=1e-6):

@@ -446,11 +446,12 @@ extern "C" int hb_adaln_residual_int8(const void* x, int64_t x_rs, const void* y
                                       int64_t xo_rs, int8_t* codes, int64_t codes_rs, float* scales, int rows,
                                       int rows_per_batch, int C, float eps, int dtype, void* stream) {
     using namespace hb;
-    if (!x || !codes || !scales || !shift || !scale || rows < 0 || rows_per_batch <= 0 || C <= 0 || !(eps >= 0.f))
-        return HB_ERR_ARG;
-    if (y && (!gate || !x_out)) return HB_ERR_ARG;  // residual needs its gate and destination
+    if (rows < 0 || rows_per_batch <= 0 || C <= 0 || !(eps >= 0.f)) return HB_ERR_ARG;
     if (dtype != 0 && dtype != 1) return HB_ERR_UNSUPPORTED;
     if (C % 256 || C > 256 * kMaxVec) return HB_ERR_UNSUPPORTED;
+    if (rows == 0) return HB_OK;
+    if (!x || !codes || !scales || !shift || !scale) return HB_ERR_ARG;
+    if (y && (!gate || !x_out)) return HB_ERR_ARG;  // residual needs its gate and destination
     if (rows > 1 && codes_rs < C) return HB_ERR_ARG;
     auto a16 = [](const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15) == 0; };
     auto s8 = [](int64_t st) { return st % 8 == 0; };
@@ -458,7 +459,6 @@ extern "C" int hb_adaln_residual_int8(const void* x, int64_t x_rs, const void* y
         (reinterpret_cast<uintptr_t>(scales) & 3))
         return HB_ERR_ALIGN;
     if (!s8(x_rs) || !s8(y_rs) || !s8(xo_rs) || !s8(mod_bs) || codes_rs % 16) return HB_ERR_ALIGN;
-    if (rows == 0) return HB_OK;
     const AdaInt8Params p{{x, y, gate, shift, scale, x_out, nullptr, x_rs, y_rs, xo_rs, 0, mod_bs, rows, rows_per_batch, C, eps},
                           codes, codes_rs, scales};
     cudaStream_t st = static_cast<cudaStream_t>(stream);

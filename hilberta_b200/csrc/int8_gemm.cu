@@ -523,7 +523,6 @@ int launch_tile(const Int8Problem& q, GemmParams& p, int dev, const DeviceInfo& 
     if ((rc = make_tmap_2d(&p.tmap_x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, q.x, p.M, p.K, q.x_rs, BT))) return rc;
     if ((rc = make_tmap_2d(&p.tmap_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, q.w, p.N, p.K, q.w_rs, C::BC))) return rc;
     const int64_t tn = ceil_div(p.N, C::BC), tm = ceil_div(p.M, BT);
-    if (tm > 65535) return HB_ERR_UNSUPPORTED;
     const int split = tile_split(p, BT, di.sms);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(tn * split), (unsigned)tm);
@@ -613,7 +612,7 @@ int launch_gemm(const Int8Problem& q, GemmParams& p, int dev, const DeviceInfo& 
     if (p.M <= 16) return launch_tile<BF16, 16>(q, p, dev, di, st);
     if (p.M <= 32) return launch_tile<BF16, 32>(q, p, dev, di, st);
     const int64_t narrow = tile_cost(p, 64, di.sms), wide = tile_cost(p, 128, di.sms);
-    if (p.M > 64 && pair_cost(p, di.sms) < std::min(narrow, wide))
+    if (p.M > 64 && (pair_cost(p, di.sms) < std::min(narrow, wide) || ceil_div(p.M, 64) > 65535))  // 65535: grid rows
         return p.act ? launch_pair<BF16, 1>(q, p, dev, st) : launch_pair<BF16, 0>(q, p, dev, st);
     if (p.M <= 64 || narrow <= wide) return launch_tile<BF16, 64>(q, p, dev, di, st);
     return launch_tile<BF16, 128>(q, p, dev, di, st);

@@ -220,7 +220,7 @@ int check_linear(const void* x, const int8_t* w, int64_t w_rs, const float* w_sc
     if ((M > 1 && out_rs < N) || (N > 1 && w_rs < K)) return HB_ERR_ARG;
     if (!aligned(w, 16) || (N > 1 && w_rs % 16) || !aligned(w_scales, 4) || !aligned(bias, 2) || !aligned(out, 2))
         return HB_ERR_ALIGN;
-    if (ceil_div(M, 128) > 65535 || ceil_div(M, 128) * ceil_div(N, 128) > INT32_MAX / 8) return HB_ERR_UNSUPPORTED;
+    if (M > 1 << 30 || N > 1 << 30 || ceil_div(M, 128) * ceil_div(N, 128) > INT32_MAX / 8) return HB_ERR_UNSUPPORTED;
     return HB_OK;
 }
 

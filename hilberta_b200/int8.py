@@ -190,19 +190,21 @@ def int8_linear(x, weight, bias=None, *, activation=None, out=None):
 
 
 def _check_out(out, x, weight, bias):
-    strides = sorted((st, n) for st, n in zip(out.stride(), out.shape) if n > 1)
-    reach = 0
-    for st, n in strides:
-        if st <= reach:
-            raise ValueError("out must not overlap itself")
-        reach += st * (n - 1)
-    begin, end = _span(out)
+    if _overlaps_itself(out):
+        raise ValueError("out must not overlap itself")
     parts = [x.values, x.scales] if isinstance(x, Int8Rows) else [x]
     for t in (*parts, weight.values, weight.scales, bias):
-        if t is not None:
-            first, last = _span(t)
-            if begin < last and first < end:
-                raise ValueError("out cannot alias inputs")
+        if t is not None and not _apart(out, t):
+            raise ValueError("out cannot alias inputs")
+
+
+def _overlaps_itself(t):
+    reach = 0
+    for st, n in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n > 1):
+        if st <= reach:
+            return True
+        reach += st * (n - 1)
+    return False
 
 
 def _span(t):
@@ -210,6 +212,23 @@ def _span(t):
         return t.data_ptr(), t.data_ptr()
     extent = sum((n - 1) * st for n, st in zip(t.shape, t.stride())) + 1
     return t.data_ptr(), t.data_ptr() + extent * t.element_size()
+
+
+def _apart(a, b):
+    """No element of a is one of b: their memory ranges are apart, or both are rows of
+    one spacing that lie side by side (column slices of one buffer)."""
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    if a1 <= b0 or b1 <= a0:
+        return True
+    ra, rb = _row_stride(a), _row_stride(b)
+    if ra is None or rb is None or a.ndim < 2 or b.ndim < 2:
+        return False
+    pitch = ra * a.element_size()
+    wa, wb = a.shape[-1] * a.element_size(), b.shape[-1] * b.element_size()
+    if pitch != rb * b.element_size() or pitch <= 0:
+        return False
+    shift = (b0 - a0) % pitch
+    return shift >= wa and shift + wb <= pitch
 
 
 def _product(x, coded, weight, bias, act, out, dev):

@@ -26,6 +26,7 @@ import ctypes
 import torch
 
 from . import _lib
+from .int8 import _overlaps_itself, _span
 
 
 def _dtype_code(t: torch.Tensor) -> int:
@@ -107,12 +108,6 @@ def prepare_qkv(q_txt, k_txt, v_txt, q_img, k_img, v_img, *, heads, norm_q, norm
 _Strides = ctypes.c_int64 * 12
 
 
-def _bytes(t):
-    """First byte and one past the last of a tensor's elements."""
-    extent = sum((n - 1) * st for n, st in zip(t.shape, t.stride())) + 1
-    return t.data_ptr(), t.data_ptr() + (extent * t.element_size() if t.numel() else 0)
-
-
 def norm_rope_qk(q, k, *, weight_q, weight_k, cos, sin, text_tokens=0, weight_txt_q=None, weight_txt_k=None, eps=1e-6,
                  out=None):
     """RMSNorm over the head dimension and rotary embedding of query and key heads,
@@ -180,20 +175,17 @@ def _check_qk_out(q, k, out, others):
             raise ValueError(f"the output of {name} must match its shape, dtype and device with contiguous D")
         if torch.is_grad_enabled() and o.requires_grad:
             raise ValueError("Inference output cannot require gradients")
-        reach = 0
-        for st, n in sorted((st, n) for st, n in zip(o.stride(), o.shape) if n > 1):
-            if st <= reach:
-                raise ValueError(f"the output of {name} must not overlap itself")
-            reach += st * (n - 1)
+        if _overlaps_itself(o):
+            raise ValueError(f"the output of {name} must not overlap itself")
     same = [o.data_ptr() == x.data_ptr() and o.stride() == x.stride() for x, o in ((q, q_out), (k, k_out))]
     if all(same) and _interleaved(q, k):
         return
     for o, in_place, own in ((q_out, same[0], q), (k_out, same[1], k)):
-        begin, end = _bytes(o)
+        begin, end = _span(o)
         for t in (q, k, *others, *(x for x in out if x is not o)):
             if in_place and t is own:
                 continue
-            first, last = _bytes(t)
+            first, last = _span(t)
             if begin < last and first < end and not (t.dtype == o.dtype and _interleaved(o, t)):
                 raise ValueError("outputs must be their inputs in place or must not overlap any input")
 

@@ -181,6 +181,60 @@ def test_int8_linear_out_views_and_neighbours(m):
     assert torch.equal(buf[:, 5:], hb.int8_linear(x3, w)) and bool((buf[:, :5] == 7.0).all())
 
 
+def test_int8_linear_empty_and_one():
+    import hilberta_b200 as hb
+    from hilberta_b200.block_ops import adaln_int8
+
+    w = hb.quantize_rows(_rows(40, 64, BF16, seed=1))
+    x = _rows(6, 64, BF16, seed=2)
+    assert hb.int8_linear(x[:0], w).shape == (0, 40) and hb.int8_linear(hb.quantize_rows(x[:0]), w).shape == (0, 40)
+    assert hb.int8_linear(x, w.row_slice(0, 0)).shape == (6, 0)
+    want = hb.int8_linear(x, w)
+    assert torch.equal(hb.int8_linear(x[3], w), want[3]) and torch.equal(hb.int8_linear(x.view(2, 3, 64), w), want.view(2, 3, 40))
+    assert torch.equal(hb.int8_linear(x, w.row_slice(7, 8)), want[:, 7:8])
+    m = torch.zeros(1, 256, dtype=BF16, device="cuda")
+    assert adaln_int8(torch.zeros(1, 0, 256, dtype=BF16, device="cuda"), m, m).shape == (1, 0, 256)
+
+
+def test_int8_linear_more_tokens_than_grid_rows():
+    """8.4 million tokens: past 65535 tiles of 128, outputs past 2^31 bytes."""
+    import hilberta_b200 as hb
+
+    m, k, n = 8_400_003, 16, 136
+    x = torch.randint(-127, 128, (m, k), dtype=torch.int8, device="cuda", generator=_gen(1))
+    rows = hb.Int8Rows(x, torch.full((m,), 0.5, device="cuda"), BF16)
+    w = hb.quantize_rows(_rows(n, k, BF16, seed=2))
+    got = hb.int8_linear(rows, w)
+    for lo in (0, m // 2, m - 1000):
+        _check_product(got[lo:lo + 1000], x[lo:lo + 1000], rows.scales[lo:lo + 1000], w.values, w.scales, None, None)
+    assert hb.device_status() == 0
+
+
+def test_slices_of_one_buffer():
+    """Inputs and outputs that lie side by side in one buffer share no element."""
+    import hilberta_b200 as hb
+    from hilberta_b200.block_ops import gate_residual_adaln_int8
+
+    buf = _rows(33, 256 + 512 + 64, BF16, seed=1)
+    w = hb.quantize_rows(_rows(512, 256, BF16, seed=2))
+    want = hb.int8_linear(buf[:, :256].clone(), w)
+    before = buf.clone()
+    hb.int8_linear(buf[:, :256], w, out=buf[:, 256:768])
+    assert torch.equal(buf[:, 256:768], want)
+    assert torch.equal(buf[:, :256], before[:, :256]) and torch.equal(buf[:, 768:], before[:, 768:])
+    both = _rows(2 * 21, 1024, BF16, seed=3).view(2, 21, 1024)
+    x, y = both[..., :512], both[..., 512:]
+    shift, scale, gate, *_ = _modulation(2, 512, BF16, seed=4)
+    want_x, want_rows = gate_residual_adaln_int8(x.contiguous(), y.contiguous(), gate, shift, scale)
+    got, rows = gate_residual_adaln_int8(x, y, gate, shift, scale)
+    assert got is x and torch.equal(x, want_x) and torch.equal(rows.values, want_rows.values)
+    with pytest.raises(ValueError, match="apart"):
+        gate_residual_adaln_int8(x, both[..., 256:768], gate, shift, scale)
+    with pytest.raises(ValueError, match="overlap itself"):
+        row = both[:1, :1, :512].expand(1, 21, 512)
+        gate_residual_adaln_int8(row, both[:1, :, 512:].contiguous(), gate[:1], shift[:1], scale[:1])
+
+
 def test_int8_linear_row_does_not_depend_on_its_batch():
     import hilberta_b200 as hb
 
