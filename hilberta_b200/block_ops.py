@@ -109,15 +109,12 @@ def _call_int8(x, y, gate, shift, scale, x_out, eps):
         raise ValueError("x must be float16 or bfloat16")
     x3, x_rs, B, S = _rows(x, "x")
     C = x3.shape[2]
-    mods = (shift, scale) if gate is None else (shift, scale, gate)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, y, *mods)):
+    if torch.is_grad_enabled() and (x.requires_grad or shift.requires_grad or scale.requires_grad
+                                    or (y is not None and (y.requires_grad or gate.requires_grad))):
         raise ValueError("Inference only; disable autograd")
-    mod_bs = None
-    for name, m in zip(("shift", "scale", "gate"), mods):
-        _, bs = _mod(m, B, C, x, name)
-        if mod_bs is not None and bs != mod_bs:
-            raise ValueError("gate, shift and scale must share one batch stride")
-        mod_bs = bs
+    mod_bs = _mod(shift, B, C, x, "shift")[1]
+    if _mod(scale, B, C, x, "scale")[1] != mod_bs or (gate is not None and _mod(gate, B, C, x, "gate")[1] != mod_bs):
+        raise ValueError("gate, shift and scale must share one batch stride")
     y_rs = xo_rs = 0
     y_ptr = gate_ptr = xo_ptr = None
     if y is not None:
@@ -128,10 +125,10 @@ def _call_int8(x, y, gate, shift, scale, x_out, eps):
         y_ptr, gate_ptr, xo_ptr = y.data_ptr(), gate.data_ptr(), x_out.data_ptr()
         if _overlaps_itself(x_out):
             raise ValueError("the new stream must not overlap itself")
-        for t in (x, y, *mods):
+        for t in (x, y, shift, scale, gate):
             if not _same_view(x_out, t) and not _apart(x_out, t):
                 raise ValueError("the new stream must be x itself or apart from every input")
-    rows = _empty_rows(x.shape, kind, dev)
+    rows = _empty_rows(x.shape, x)
     with _lib.on_device(dev) as stream:
         rc = _lib.lib().hb_adaln_residual_int8(
             x.data_ptr(), x_rs, y_ptr, y_rs, gate_ptr, shift.data_ptr(), scale.data_ptr(), mod_bs, xo_ptr, xo_rs,

@@ -92,14 +92,15 @@ class Int8Rows:
         return Int8Rows(self.values[start:stop], self.scales[start:stop], self.dtype)
 
 
-def _empty_rows(shape, dtype, device):
+def _empty_rows(shape, like):
+    """Uninitialised ``Int8Rows`` of a shape, on the device and standing in for the type of ``like``."""
     K = shape[-1]
     pitch = -(-K // 16) * 16
-    values = torch.empty((*shape[:-1], pitch), dtype=torch.int8, device=device)
+    values = like.new_empty((*shape[:-1], pitch), dtype=torch.int8)
     rows = object.__new__(Int8Rows)  # right by construction: none of the checks of Int8Rows(...)
     rows.values = values if pitch == K else values[..., :K]
-    rows.scales = torch.empty(shape[:-1], dtype=torch.float32, device=device)
-    rows.dtype, rows.row_stride = dtype, pitch
+    rows.scales = like.new_empty(shape[:-1], dtype=torch.float32)
+    rows.dtype, rows.row_stride = like.dtype, pitch
     return rows
 
 
@@ -132,7 +133,7 @@ def quantize_rows(x, *, joined=None):
         raise ValueError("rows must be equally spaced")
     if ka + kb > _lib.HB_INT8_MAX_K:
         raise NotImplementedError(f"rows of more than {_lib.HB_INT8_MAX_K} values are not supported")
-    out = _empty_rows((*x.shape[:-1], ka + kb), x.dtype, x.device)
+    out = _empty_rows((*x.shape[:-1], ka + kb), x)
     rows = out.scales.numel()
     if rows >= 1 << 31:
         raise NotImplementedError("2^31 rows or more are not supported")
@@ -178,7 +179,7 @@ def int8_linear(x, weight, bias=None, *, activation=None, out=None):
             raise ValueError("Inference only; disable autograd")
     shape = (*x_shape[:-1], N)
     if out is None:
-        out = torch.empty(shape, dtype=kind, device=dev) if coded else x.new_empty(shape)
+        out = (x.values if coded else x).new_empty(shape, dtype=kind)
     else:
         if out.shape != shape or out.dtype != kind or out.device != dev or (N > 1 and out.stride(-1) != 1):
             raise ValueError("out must be [..., N] of x's type and device with a contiguous last dimension")

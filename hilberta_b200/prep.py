@@ -136,21 +136,24 @@ def norm_rope_qk(q, k, *, weight_q, weight_k, cos, sin, text_tokens=0, weight_tx
         raise ValueError("text_tokens must lie within the tokens")
     if T > 0 and (weight_txt_q is None or weight_txt_k is None):
         raise ValueError("text tokens need weight_txt_q and weight_txt_k")
-    weights = [w for w in (weight_q, weight_k, weight_txt_q, weight_txt_k) if w is not None]
+    weights = (weight_q, weight_k) if weight_txt_q is None and weight_txt_k is None else (weight_q, weight_k, weight_txt_q,
+                                                                                        weight_txt_k)
     for w in weights:
-        if w.shape != (D,) or w.dtype != kind or w.device != dev or (D > 1 and w.stride(0) != 1):
+        if w is not None and (w.shape != (D,) or w.dtype != kind or w.device != dev or (D > 1 and w.stride(0) != 1)):
             raise ValueError("norm weights must be contiguous [D] in the heads' dtype")
     for c in (cos, sin):
         if c.shape != (S, D) or c.dtype != torch.float32 or c.device != dev or not c.is_contiguous():
             raise ValueError("cos/sin must be contiguous fp32 [S, D] on the heads' device")
     if not eps >= 0:
         raise ValueError("eps must not be negative")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, cos, sin, *weights)):
-        raise ValueError("Inference only; disable autograd")
+    if torch.is_grad_enabled():
+        for t in (q, k, cos, sin, *weights):
+            if t is not None and t.requires_grad:
+                raise ValueError("Inference only; disable autograd")
     if out is None:
         q_out, k_out = q.new_empty((B, S, Hq, D)), k.new_empty((B, S, Hk, D))
     else:
-        _check_qk_out(q, k, out, (cos, sin, *weights))
+        _check_qk_out(q, k, out, [t for t in (cos, sin, *weights) if t is not None])
         q_out, k_out = out
     strides = _Strides(*q.stride()[:3], *k.stride()[:3], *q_out.stride()[:3], *k_out.stride()[:3])
     with _lib.on_device(dev) as stream:
