@@ -369,6 +369,7 @@ __global__ void __launch_bounds__(128) k_adaln_int8(const __grid_constant__ AdaI
             }
         }
     };
+    grid_launch_dependents();  // the product's CTAs may set themselves up meanwhile
     int row = blockIdx.x * RPC + threadIdx.x / T;
 #pragma unroll
     for (int k = 0; k < DEPTH; ++k) fetch(row + k * step, x[k], y[k]);

@@ -119,6 +119,8 @@ struct Int8Problem {
 };
 bool int8_few_takes(int M, int K);  // int8_few.cu: tokens it serves
 int launch_int8_few(const Int8Problem& p, const DeviceInfo& di, cudaStream_t st);
-int launch_int8_gemm(const Int8Problem& p, int dev, const DeviceInfo& di, cudaStream_t st);  // int8_gemm.cu
+// int8_gemm.cu; early_weights: the weights are not written by the kernel before this
+// launch, so they may be fetched before it has ended.
+int launch_int8_gemm(const Int8Problem& p, int dev, const DeviceInfo& di, bool early_weights, cudaStream_t st);
 
 }  // namespace hb

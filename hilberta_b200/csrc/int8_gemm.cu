@@ -1,6 +1,8 @@
 // 8-bit products on the tensor cores (tcgen05 kind::i8, 32-bit integer sums in TMEM):
 // 256 x 256 tiles by CTA pairs for large products, 128 channels x up to 128 tokens by
-// single CTAs, which may split K, for small ones.
+// single CTAs, which may split K, for small ones.  Both are launched as dependents of
+// the kernel before them: they set themselves up while it ends, and wait for its end
+// before they read its results.
 #include <algorithm>
 #include <climits>
 #include <mutex>
@@ -28,6 +30,7 @@ struct GemmParams {
     int M, N, K, act;
     int tma_out;  // out rows start on 16 bytes: TMA stores
     int tiles_m, tiles_n;
+    int early_weights;  // the first weights are fetched before grid_wait
     long long timeout;
 };
 
@@ -85,12 +88,20 @@ __global__ void __launch_bounds__(256, 2) k_int8_tile(const __grid_constant__ Ge
         mbar_init(&ctl->done, 1);
         ctl->abort = 0;
         fence_barrier_init();
+        if (p.early_weights) {
+            for (int s = 0; s < min(stages, kb1 - kb0); s++) {
+                mbar_arrive_expect_tx(&ctl->full[s], C::STAGE);
+                tma_load_2d(smem + s * C::STAGE, &p.tmap_w, &ctl->full[s], (kb0 + s) * C::BK, n0);
+            }
+        }
     }
     if (warp == 2) {
         tmem_alloc(&ctl->tmem_base, C::TMEM_COLS);
         tmem_relinquish();
         tc_fence_before();
     }
+    __syncwarp();
+    grid_wait();
     const int channel = threadIdx.x & 127, n = n0 + channel;  // this thread's channel
     const int t0 = (warp >> 2) * C::HALF;                     // and the first of its tokens
     const float sw = n < p.N ? p.w_scales[n] : 0.f, bias = n < p.N && p.bias ? load16<BF16>(p.bias + n) : 0.f;
@@ -108,8 +119,10 @@ __global__ void __launch_bounds__(256, 2) k_int8_tile(const __grid_constant__ Ge
                 break;
             }
             uint8_t* st = smem + s * C::STAGE;
-            mbar_arrive_expect_tx(&ctl->full[s], C::STAGE);
-            tma_load_2d(st, &p.tmap_w, &ctl->full[s], kb * C::BK, n0);
+            if (round > 0 || !p.early_weights) {
+                mbar_arrive_expect_tx(&ctl->full[s], C::STAGE);
+                tma_load_2d(st, &p.tmap_w, &ctl->full[s], kb * C::BK, n0);
+            }
             tma_load_2d(st + C::W_BYTES, &p.tmap_x, &ctl->full[s], kb * C::BK, m0);
             if (++s == stages) s = 0, round++;
         }
@@ -300,6 +313,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::THREADS, 1)
 
     if (warp == 0) {
         if (lane == 0) {
+            int early = 0;
+            if (p.early_weights) {
+                int m0, n0;
+                pair_tile(p, first, m0, n0);
+                early = min(C::STAGES, nkb);  // blocks of the first tile
+                for (int s = 0; s < early; s++) {
+                    if (rank == 0) mbar_arrive_expect_tx(&ctl->full[s], 2 * C::STAGE);
+                    tma_load_2d_pair(smem + s * C::STAGE + C::A_BYTES, &p.tmap_w, cluster_map(smem_u32(&ctl->full[s]), 0),
+                                     s * C::BK, n0 + 128 * rank);
+                }
+            }
+            grid_wait();
             int it = 0;
             bool ok = true;
             for (int t = first; t < tiles && ok; t += step) {
@@ -313,10 +338,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::THREADS, 1)
                         break;
                     }
                     uint8_t* st = smem + s * C::STAGE;
-                    if (rank == 0) mbar_arrive_expect_tx(&ctl->full[s], 2 * C::STAGE);
+                    if (rank == 0 && it >= early) mbar_arrive_expect_tx(&ctl->full[s], 2 * C::STAGE);
                     const uint32_t bar = cluster_map(smem_u32(&ctl->full[s]), 0);
                     tma_load_2d_pair(st, &p.tmap_x, bar, kb * C::BK, m0 + 128 * rank);
-                    tma_load_2d_pair(st + C::A_BYTES, &p.tmap_w, bar, kb * C::BK, n0 + 128 * rank);
+                    if (it >= early) tma_load_2d_pair(st + C::A_BYTES, &p.tmap_w, bar, kb * C::BK, n0 + 128 * rank);
                 }
             }
             if (!ok) {  // gave up: time for the copies and MMAs in flight to end before the memory is given back
@@ -353,6 +378,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::THREADS, 1)
     } else if (warp >= 4) {
         const int ew = warp - 4, quarter = warp & 3, half = ew >> 2;
         uint8_t* stg = smem + C::STG_OFF + ew * C::STAGING;
+        grid_wait();
         float *col_scale = ctl->col_scale + 128 * half, *col_bias = ctl->col_bias + 128 * half;
         int i = 0;
         bool dead = false;  // a wait ran out: only the barriers of the remaining tiles are kept, so that no warp is left at one
@@ -530,13 +556,15 @@ int launch_tile(const Int8Problem& q, GemmParams& p, int dev, const DeviceInfo& 
     const int stages = tn * tm * split <= di.sms ? C::STAGES_ALONE : C::STAGES;
     cfg.dynamicSmemBytes = C::smem(stages);
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = split;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = split;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = split > 1;
+    cfg.numAttrs = split > 1 ? 2 : 1;
     HB_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, p, split, stages));
     return HB_OK;
 }
@@ -586,8 +614,17 @@ int launch_pair(const Int8Problem& q, GemmParams& p, int dev, cudaStream_t st) {
                            p.M, p.N, p.out_rs * 2, 32)))
         return rc;
     const int tiles = p.tiles_m * p.tiles_n;
-    kern<<<2 * std::min(tiles, pairs), C::THREADS, C::SMEM, st>>>(p);
-    HB_LAUNCH_CHECK();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2 * (unsigned)std::min(tiles, pairs));
+    cfg.blockDim = dim3(C::THREADS);
+    cfg.dynamicSmemBytes = C::SMEM;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    HB_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, p));
     return HB_OK;
 }
 
@@ -620,7 +657,7 @@ int launch_gemm(const Int8Problem& q, GemmParams& p, int dev, const DeviceInfo& 
 
 }  // namespace
 
-int launch_int8_gemm(const Int8Problem& q, int dev, const DeviceInfo& di, cudaStream_t st) {
+int launch_int8_gemm(const Int8Problem& q, int dev, const DeviceInfo& di, bool early_weights, cudaStream_t st) {
     GemmParams p;
     p.x_scales = q.x_scales;
     p.w_scales = q.w_scales;
@@ -631,6 +668,7 @@ int launch_int8_gemm(const Int8Problem& q, int dev, const DeviceInfo& di, cudaSt
     p.N = q.N;
     p.K = q.K;
     p.act = q.act;
+    p.early_weights = early_weights;
     p.timeout = 2000LL * di.clock_khz;
     return q.dtype == 1 ? launch_gemm<true>(q, p, dev, di, st) : launch_gemm<false>(q, p, dev, di, st);
 }

@@ -112,6 +112,7 @@ __global__ void __launch_bounds__(T < 128 ? 128 : T) k_quantize_rows(const __gri
     __shared__ uint32_t s_max[2][CTA / 32];
     const int t = threadIdx.x % T;
     const int64_t step = (int64_t)gridDim.x * RPC;
+    ptx::grid_launch_dependents();  // the product's CTAs may set themselves up meanwhile
     int64_t row = (int64_t)blockIdx.x * RPC + threadIdx.x / T;
     uint4 next[NV];
     auto fetch = [&](int64_t r) {
@@ -147,6 +148,7 @@ template <bool BF16, bool VEC>
 __global__ void __launch_bounds__(512) k_quantize_long(const __grid_constant__ QuantParams p) {
     __shared__ uint32_t s_max[16];
     const int64_t row = blockIdx.x;
+    ptx::grid_launch_dependents();
     const int n = (p.k + 8 * 512 - 1) / (8 * 512);
     uint32_t m = 0;
 #pragma unroll 4
@@ -224,11 +226,11 @@ int check_linear(const void* x, const int8_t* w, int64_t w_rs, const float* w_sc
     return HB_OK;
 }
 
-int linear(const Int8Problem& p, bool few, cudaStream_t st) {
+int linear(const Int8Problem& p, bool few, bool early_weights, cudaStream_t st) {
     int dev = 0, rc;
     DeviceInfo di;
     if ((rc = current_device(&dev)) || (rc = device_info(dev, &di))) return rc;
-    return few ? launch_int8_few(p, di, st) : launch_int8_gemm(p, dev, di, st);
+    return few ? launch_int8_few(p, di, st) : launch_int8_gemm(p, dev, di, early_weights, st);
 }
 }  // namespace
 }  // namespace hb
@@ -242,7 +244,7 @@ extern "C" int hb_int8_linear(const int8_t* x, int64_t x_rs, const float* x_scal
     if (!aligned(x, 16) || (M > 1 && x_rs % 16) || !aligned(x_scales, 4)) return HB_ERR_ALIGN;
     const Int8Problem p{x, x_rs, x_scales, w, w_rs, w_scales, static_cast<const uint16_t*>(bias), static_cast<uint16_t*>(out),
                         out_rs, M, N, K, act, dtype};
-    return linear(p, int8_few_takes(M, K), static_cast<cudaStream_t>(stream));
+    return linear(p, int8_few_takes(M, K), false, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" size_t hb_int8_linear16_workspace_bytes(int M, int K) {
@@ -268,5 +270,7 @@ extern "C" int hb_int8_linear16(const void* x, int64_t x_rs, const int8_t* w, in
         p.x_rs = code_pitch(K);
         p.x_scales = scales;
     }
-    return linear(p, !need, static_cast<cudaStream_t>(stream));
+    // The kernel before the product is the quantisation, an ordinary launch that does
+    // not write the weights: they are final when it starts.
+    return linear(p, !need, need != 0, static_cast<cudaStream_t>(stream));
 }

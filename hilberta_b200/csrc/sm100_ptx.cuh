@@ -184,6 +184,13 @@ __device__ __forceinline__ void bulk_wait() {
 }
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
+// ---- dependent launches -----------------------------------------------------
+// This kernel's dependents may be scheduled (they still wait for its end).
+__device__ __forceinline__ void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+// Until the kernels this one depends on have ended and their writes are visible
+// (at once in an ordinary launch).
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ---- clusters ---------------------------------------------------------------
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
