@@ -608,7 +608,6 @@ int launch_pair(const Int8Problem& q, GemmParams& p, int dev, cudaStream_t st) {
     if ((rc = make_tmap_2d(&p.tmap_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, q.w, p.N, p.K, q.w_rs, 128))) return rc;
     p.tiles_m = (int)ceil_div(p.M, C::BM);
     p.tiles_n = (int)ceil_div(p.N, C::BN);
-    p.tma_out = aligned(p.out, 16) && (p.M == 1 || p.out_rs % 8 == 0);
     if (p.tma_out &&
         (rc = make_tmap_2d(&p.tmap_out, BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, p.out,
                            p.M, p.N, p.out_rs * 2, 32)))
@@ -641,7 +640,8 @@ int64_t tile_cost(const GemmParams& p, int bt, int sms) {
     return (bt == 128 ? 550 : 430) + (split > 1 ? 100 : 0) + (waves - 1) * 130 + kb * (waves == 1 ? 28 : waves * 47 / 2);
 }
 int64_t pair_cost(const GemmParams& p, int sms) {
-    return 700 + ceil_div(p.K, 128) * 29 * ceil_div(ceil_div(p.M, 256) * ceil_div(p.N, 256), sms / 2);
+    const int64_t rounds = ceil_div(ceil_div(p.M, 256) * ceil_div(p.N, 256), sms / 2);
+    return 700 + rounds * (ceil_div(p.K, 128) * 29 + (p.tma_out ? 0 : 250));  // 250: stores by value
 }
 
 template <bool BF16>
@@ -668,6 +668,7 @@ int launch_int8_gemm(const Int8Problem& q, int dev, const DeviceInfo& di, bool e
     p.N = q.N;
     p.K = q.K;
     p.act = q.act;
+    p.tma_out = aligned(p.out, 16) && (p.M == 1 || p.out_rs % 8 == 0);
     p.early_weights = early_weights;
     p.timeout = 2000LL * di.clock_khz;
     return q.dtype == 1 ? launch_gemm<true>(q, p, dev, di, st) : launch_gemm<false>(q, p, dev, di, st);
