@@ -3,8 +3,10 @@
 // bytes of every channel's row, with 4-way 8-bit dot products; the tokens' codes lie
 // in shared memory, quantised there from 16 bits by each CTA (they are a few KB; the
 // first weights are on their way meanwhile).  Sums and results are those of the
-// tensor-core kernels, bit for bit.  1 x 18432 with K 3072: 11.8 us (4.8 TB/s) from
-// DRAM, 2.5 us of it the launch and the tokens.
+// tensor-core kernels, bit for bit.  1 x 18432 with K 3072: 11.5 us (4.9 TB/s) from
+// DRAM, 2.5 us of it the launch and the token, with four CTAs per SM (all 576 at once);
+// 14.3 us with three.  Rings of asynchronous copies per warp, 192 KB on their way per SM,
+// took 11.6 us and 0.5 us more for small products.
 #include <climits>
 
 #include "int8_common.cuh"
@@ -25,7 +27,7 @@ __device__ __forceinline__ int4 load_codes(const int8_t* p, int left) {
 }
 
 template <bool BF16, bool CODES, int M, int R>
-__global__ void __launch_bounds__(256) k_int8_few(const __grid_constant__ Int8Problem p) {
+__global__ void __launch_bounds__(256, M == 1 ? 4 : 2) k_int8_few(const __grid_constant__ Int8Problem p) {
     extern __shared__ __align__(16) int8_t s_codes[];  // [M][pitch]
     __shared__ uint32_t s_mag[M][8];
     __shared__ float s_scale[M];
