@@ -353,6 +353,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::THREADS, 1)
     } else if (warp == 1) {
         if (lane == 0 && rank == 0) {
             constexpr uint32_t idesc = idesc_i8(C::BM, C::BN);
+            grid_wait();  // the clock of the waits starts when the copies can
             int it = 0, i = 0;
             bool ok = true;
             for (int t = first; t < tiles && ok; t += step, i++) {
@@ -456,7 +457,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::THREADS, 1)
                         for (int e = 0; e < 8; e++) {
                             const uint8_t* line = stg + (r + e) * 128 + (lane & 7) * 2;
                             v[2 * e] = *reinterpret_cast<const uint16_t*>(line + (((lane >> 3) ^ e) << 4));
-                            v[2 * e + 1] = *reinterpret_cast<const uint16_t*>(line + (((lane >> 3) + 4 ^ e) << 4));
+                            v[2 * e + 1] = *reinterpret_cast<const uint16_t*>(line + ((((lane >> 3) + 4) ^ e) << 4));
                         }
 #pragma unroll
                         for (int e = 0; e < 8; e++) {

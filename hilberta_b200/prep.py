@@ -142,7 +142,7 @@ def norm_rope_qk(q, k, *, weight_q, weight_k, cos, sin, text_tokens=0, weight_tx
         if w is not None and (w.shape != (D,) or w.dtype != kind or w.device != dev or (D > 1 and w.stride(0) != 1)):
             raise ValueError("norm weights must be contiguous [D] in the heads' dtype")
     for c in (cos, sin):
-        if c.shape != (S, D) or c.dtype != torch.float32 or c.device != dev or not c.is_contiguous():
+        if c is None or c.shape != (S, D) or c.dtype != torch.float32 or c.device != dev or not c.is_contiguous():
             raise ValueError("cos/sin must be contiguous fp32 [S, D] on the heads' device")
     if not eps >= 0:
         raise ValueError("eps must not be negative")

@@ -270,6 +270,41 @@ def test_int8_linear_streams_graph_and_repeat():
         assert torch.equal(o, hb.int8_linear(x, w, activation="gelu_tanh"))
 
 
+@pytest.mark.parametrize("m,k,n", [(5, 512, 384), (40, 1024, 640), (200, 384, 2048), (3000, 256, 1024)])
+def test_calls_in_a_row_see_each_other(m, k, n):
+    """Producers, quantisation and products back to back, memory reused at once: every
+    product sees the values and the weights written just before it."""
+    import hilberta_b200 as hb
+    from hilberta_b200.block_ops import adaln_int8
+
+    x = _rows(m, k, BF16, seed=1, spread=0.3)
+    w = [_rows(n, k, BF16, seed=s, spread=0.0) for s in (2, 3)]
+    shift = torch.zeros(1, 256, dtype=BF16, device="cuda")
+    want = []
+    for i in range(4):
+        xi = x * (i + 1) if i % 2 == 0 else x - i
+        want.append(hb.int8_linear(hb.quantize_rows(xi), hb.quantize_rows(w[i % 2])))
+        torch.cuda.synchronize()
+    narrow = x[None, :, :256].contiguous()
+    rows = adaln_int8(narrow, shift, shift)
+    torch.cuda.synchronize()
+    w256 = hb.quantize_rows(w[0][:, :256])
+    want_mod = hb.int8_linear(rows, w256)
+    torch.cuda.synchronize()
+    buf, spare = torch.empty_like(x), torch.empty_like(w[0])
+    got, mods = [], []
+    for r in range(25):
+        for i in range(4):
+            torch.mul(x, i + 1, out=buf) if i % 2 == 0 else torch.sub(x, i, out=buf)
+            spare.copy_(w[i % 2])
+            got.append(hb.int8_linear(buf, hb.quantize_rows(spare)))
+        mods.append(hb.int8_linear(adaln_int8(narrow, shift, shift), w256))
+    torch.cuda.synchronize()
+    for j, g in enumerate(got):
+        assert torch.equal(g, want[j % 4]), j
+    assert all(torch.equal(g, want_mod) for g in mods)
+
+
 def _modulation(b, c, dtype, seed):
     return (torch.randn(b, 6 * c, generator=_gen(seed), device="cuda") * 0.5).to(dtype).chunk(6, dim=-1)
 
