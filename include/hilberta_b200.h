@@ -337,9 +337,10 @@ int hb_quantize_rows(const void* a, int64_t a_rs, int ka, const void* b, int64_t
 
 /* out[m][n] = act(sum_k x[m][k] w[n][k] * (x_scales[m] * w_scales[n]) + bias[n]) for
  * x [M][K], w [N][K] in 8 bits.  bias: [N] in the output type or NULL; act 0 none,
- * 1 tanh-GELU; out: 16-bit rows (dtype) with element row stride out_rs.  The sum
+ * 1 tanh-GELU; out: 16-bit rows (dtype) with element row stride out_rs >= N.  The sum
  * is exact; the rest is fp32, rounded once.  A NaN scale makes its outputs NaN.
- * M or N 0 is a no-op. */
+ * Strides of a single row are not used; out, bias and scales need no alignment beyond
+ * their elements'.  out must not overlap what is read.  M or N 0 is a no-op. */
 int hb_int8_linear(const int8_t* x, int64_t x_rs, const float* x_scales, const int8_t* w, int64_t w_rs,
                    const float* w_scales, const void* bias, void* out, int64_t out_rs, int M, int N,
                    int K, int act, int dtype, void* stream);
@@ -348,7 +349,8 @@ int hb_int8_linear(const int8_t* x, int64_t x_rs, const float* x_scales, const i
  * hb_quantize_rows does: the result equals hb_quantize_rows + hb_int8_linear bit for
  * bit.  A few tokens are quantised inside the product's kernel; otherwise the codes
  * and scales go to the workspace (16-byte aligned, at least
- * hb_int8_linear16_workspace_bytes(M, K), which is 0 when none is needed). */
+ * hb_int8_linear16_workspace_bytes(M, K), which is 0 when none is needed; its contents
+ * matter during the call only, and calls that may overlap need separate ones). */
 size_t hb_int8_linear16_workspace_bytes(int M, int K);
 int hb_int8_linear16(const void* x, int64_t x_rs, const int8_t* w, int64_t w_rs, const float* w_scales,
                      const void* bias, void* out, int64_t out_rs, int M, int N, int K, int act,
