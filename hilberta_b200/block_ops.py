@@ -112,9 +112,16 @@ def _call_int8(x, y, gate, shift, scale, x_out, eps):
     if torch.is_grad_enabled() and (x.requires_grad or shift.requires_grad or scale.requires_grad
                                     or (y is not None and (y.requires_grad or gate.requires_grad))):
         raise ValueError("Inference only; disable autograd")
-    mod_bs = _mod(shift, B, C, x, "shift")[1]
-    if _mod(scale, B, C, x, "scale")[1] != mod_bs or (gate is not None and _mod(gate, B, C, x, "gate")[1] != mod_bs):
-        raise ValueError("gate, shift and scale must share one batch stride")
+    mod_bs = None
+    for name, m in (("shift", shift), ("scale", scale)) if gate is None else (("shift", shift), ("scale", scale), ("gate", gate)):
+        bs = m.stride()
+        if m.shape == (B, C) and bs[1] == 1 and m.dtype == kind and m.device == dev:
+            bs = bs[0] if B > 1 else 0
+        else:  # one row for a batch of one, or the refusal
+            bs = _mod(m, B, C, x, name)[1]
+        if mod_bs is not None and bs != mod_bs:
+            raise ValueError("gate, shift and scale must share one batch stride")
+        mod_bs = bs
     y_rs = xo_rs = 0
     y_ptr = gate_ptr = xo_ptr = None
     if y is not None:

@@ -186,7 +186,7 @@ def int8_linear(x, weight, bias=None, *, activation=None, out=None):
         if out.requires_grad and torch.is_grad_enabled():
             raise ValueError("Inference output cannot require gradients")
         _check_out(out, x, weight, bias)
-    _product(x, coded, weight, bias, act, out, dev)
+    _product(x, coded, weight, bias, act, out, kind, dev)
     return out
 
 
@@ -232,32 +232,33 @@ def _apart(a, b):
     return shift >= wa and shift + wb <= pitch
 
 
-def _product(x, coded, weight, bias, act, out, dev):
+def _product(x, coded, weight, bias, act, out, kind, dev):
     out_rs = _row_stride(out)
     x_rs = x.row_stride if coded else _row_stride(x)
     if out_rs is None or x_rs is None:  # a leading index at a time
         for i in range(out.shape[0]):
             part = Int8Rows(x.values[i], x.scales[i], x.dtype) if coded else x[i]
-            _product(part, coded, weight, bias, act, out[i], dev)
+            _product(part, coded, weight, bias, act, out[i], kind, dev)
         return
     lib = _lib.lib()
     w = weight.values
     N, K = w.shape
     M = x.scales.numel() if coded else x.numel() // K
     tail = (w.data_ptr(), weight.row_stride, weight.scales.data_ptr(), None if bias is None else bias.data_ptr(),
-            out.data_ptr(), out_rs, M, N, K, act, _DTYPES[out.dtype])
+            out.data_ptr(), out_rs, M, N, K, act, _DTYPES[kind])
     with _lib.on_device(dev) as stream:
         if coded:
             rc = lib.hb_int8_linear(x.values.data_ptr(), x_rs, x.scales.data_ptr(), *tail, stream)
-        elif nbytes := lib.hb_int8_linear16_workspace_bytes(M, K):
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-            rc = lib.hb_int8_linear16(x.data_ptr(), x_rs, *tail, ws.data_ptr(), nbytes, stream)
         else:
-            rc = lib.hb_int8_linear16(x.data_ptr(), x_rs, *tail, None, 0, stream)
+            nbytes = lib.hb_int8_linear16_workspace_bytes(M, K)
+            ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+            rc = lib.hb_int8_linear16(x.data_ptr(), x_rs, *tail, None if ws is None else ws.data_ptr(), nbytes, stream)
+    if rc == 0:
+        _used.add(dev.index)
+        return
     if rc == _lib.HB_ERR_UNSUPPORTED:
         raise NotImplementedError(f"int8_linear: {_lib.status_text(rc)}")
     _lib.check(rc, "hb_int8_linear")
-    _used.add(dev.index)
 
 
 class Int8Linear(torch.nn.Module):
