@@ -432,3 +432,21 @@ def test_refusals():
     m = torch.zeros(1, 128, dtype=BF16, device="cuda")
     with pytest.raises(NotImplementedError, match="multiple of 256"):
         adaln_int8(torch.zeros(1, 8, 128, dtype=BF16, device="cuda"), m, m)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("align", [1, 2, 4, 8])
+@pytest.mark.parametrize("k", [16, 1000, 1816, 6008, 15992, 16408])
+def test_quantize_rows_by_alignment(k, align, dtype):
+    """Rows, parts and lengths that start on 2, 4, 8 or 16 bytes and no more."""
+    import hilberta_b200 as hb
+
+    big = _rows(37, k + 5 * align, dtype, seed=k + align)
+    pitch = 8 * ((k + 5 * align) // 8 + 1) + align  # elements between rows
+    room = torch.full((37 * pitch + 8,), math.nan, dtype=dtype, device="cuda")
+    view = room.as_strided((37, k + 5 * align), (pitch, 1), align)
+    view.copy_(big)
+    for a, b in ((view, None), (view[:, : 3 * align], view[:, 3 * align :]), (view[::2, align:k], view[::2, k:])):
+        got = hb.quantize_rows(a, joined=b)
+        codes, scales = _quantised(a if b is None else torch.cat([a, b], 1))
+        assert torch.equal(got.values, codes) and torch.equal(got.scales, scales)
