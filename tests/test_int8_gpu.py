@@ -450,3 +450,26 @@ def test_quantize_rows_by_alignment(k, align, dtype):
         got = hb.quantize_rows(a, joined=b)
         codes, scales = _quantised(a if b is None else torch.cat([a, b], 1))
         assert torch.equal(got.values, codes) and torch.equal(got.scales, scales)
+
+
+@pytest.mark.parametrize("b,s,c", [(2, 7001, 256), (1, 9003, 512), (3, 1100, 768), (2, 1501, 1280), (1, 1999, 1536), (2, 801, 2560),
+                                   (1, 1201, 2816), (1, 1101, 3328), (3, 602, 3840), (1, 1801, 2048)])
+def test_adaln_int8_layouts(b, s, c):
+    """Every number of vectors per lane, one warp per row to thirteen, more rows than
+    the grid has CTAs, and batch entries that change inside a CTA's rows."""
+    from hilberta_b200.block_ops import adaln_int8, gate_residual, gate_residual_adaln_int8
+
+    x = (_rows(b * s, c, BF16, seed=s, spread=0.5) - 0.25).view(b, s, c)
+    y = _rows(b * s, c, BF16, seed=s + 1).view(b, s, c)
+    shift, scale, gate, *_ = _modulation(b, c, BF16, seed=c)
+    stream, joined = gate_residual_adaln_int8(x, y, gate, shift, scale, x_out=torch.empty_like(x))
+    assert torch.equal(stream, gate_residual(x.clone(), y, gate))
+    for f, rows in ((x.double(), adaln_int8(x, shift, scale)), (stream.double(), joined)):
+        h = (f - f.mean(-1, keepdim=True)) / (f.var(-1, correction=0, keepdim=True) + 1e-6).sqrt()
+        h = h * (1 + scale.double()[:, None]) + shift.double()[:, None]
+        top = h.abs().amax(-1)
+        # fp32 mean and variance over C elements and five elementwise steps
+        fuzz = 2.0**-19 * (h.abs() + shift.double()[:, None].abs() + top[..., None])
+        assert bool(((rows.scales.double() - top / 127).abs() <= top / 127 * 2.0**-17).all())
+        off = (rows.values.double() * rows.scales.double()[..., None] - h).abs()
+        assert bool((off <= rows.scales.double()[..., None] * 0.5 + fuzz).all())
