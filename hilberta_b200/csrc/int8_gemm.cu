@@ -1,8 +1,8 @@
 // 8-bit products on the tensor cores (tcgen05 kind::i8, 32-bit integer sums in TMEM):
 // 256 x 256 tiles by CTA pairs for large products, 128 channels x up to 128 tokens by
-// single CTAs, which may split K, for small ones.  Both are launched as dependents of
-// the kernel before them: they set themselves up while it ends, and wait for its end
-// before they read its results.
+// single CTAs for small ones; several of either may split K.  Both are launched as
+// dependents of the kernel before them: they set themselves up while it ends, and wait
+// for its end before they read its results.
 #include <algorithm>
 #include <climits>
 #include <mutex>
@@ -239,7 +239,8 @@ __global__ void __launch_bounds__(256, 2) k_int8_tile(const __grid_constant__ Ge
 // x 256 x 32: each CTA stages 128 rows of both operands, so a CTA reads half of
 // the weight tile's bytes that it would need alone, and both keep 128 rows of the
 // accumulator.  Two accumulators fill the TMEM: the epilogue of a tile runs under
-// the products of the next.
+// the products of the next.  With SPLIT 2 or 4 that many pairs, one cluster, share the K
+// of one tile and exchange their sums (one tile each, for products of few tiles).
 struct PairCfg {
     static constexpr int BM = 256, BN = 256, BK = 128;
     static constexpr int A_BYTES = 128 * BK, B_BYTES = 128 * BK, STAGE = A_BYTES + B_BYTES;
@@ -258,6 +259,7 @@ struct PairCfg {
     static constexpr int CTL_OFF = STG_OFF + EPI_WARPS * STAGING;
     static constexpr int SMEM = CTL_OFF + (int)((sizeof(Ctl) + 15) / 16 * 16);
     static_assert(SMEM <= 227 * 1024, "shared memory of one CTA");
+    static_assert(3 * EPI_WARPS * 32 * 64 * 4 <= STAGES * STAGE, "sums of three other pairs reuse the stages");
     // Tiles are walked down columns of GROUP row tiles, so the tiles in flight at
     // one time share few rows of both operands (both stay in L2).
     static constexpr int GROUP = 8;
@@ -271,17 +273,19 @@ __device__ __forceinline__ void pair_tile(const GemmParams& p, int t, int& m0, i
     n0 = r / gm * PairCfg::BN;
 }
 
-template <bool BF16, int ACT>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::THREADS, 1)
+template <bool BF16, int ACT, int SPLIT>
+__global__ void __cluster_dims__(2 * SPLIT, 1, 1) __launch_bounds__(PairCfg::THREADS, 1)
     k_int8_pair(const __grid_constant__ GemmParams p) {
     using C = PairCfg;
     extern __shared__ __align__(1024) uint8_t smem[];
     auto* ctl = reinterpret_cast<C::Ctl*>(smem + C::CTL_OFF);
     volatile int* abort_flag = &ctl->abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int rank = (int)cluster_rank();
-    const int first = blockIdx.x >> 1, step = gridDim.x >> 1, tiles = p.tiles_m * p.tiles_n;
-    const int nkb = (p.K + C::BK - 1) / C::BK;
+    const int cta = (int)cluster_rank(), rank = cta & 1, lead = cta & ~1;  // in the cluster, in the pair, the pair's first
+    const int part = cta >> 1;                                            // of K
+    const int first = blockIdx.x / (2 * SPLIT), step = gridDim.x / (2 * SPLIT), tiles = p.tiles_m * p.tiles_n;
+    const int blocks = (p.K + C::BK - 1) / C::BK;
+    const int kb0 = blocks * part / SPLIT, nkb = blocks * (part + 1) / SPLIT - kb0;
 
     if (smem_u32(smem) & 1023) {  // the same in both CTAs
         if (threadIdx.x == 0) atomicOr(&g_int8_status, HB_DEV_SMEM_ALIGN);
@@ -320,8 +324,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::THREADS, 1)
                 early = min(C::STAGES, nkb);  // blocks of the first tile
                 for (int s = 0; s < early; s++) {
                     if (rank == 0) mbar_arrive_expect_tx(&ctl->full[s], 2 * C::STAGE);
-                    tma_load_2d_pair(smem + s * C::STAGE + C::A_BYTES, &p.tmap_w, cluster_map(smem_u32(&ctl->full[s]), 0),
-                                     s * C::BK, n0 + 128 * rank);
+                    tma_load_2d_pair(smem + s * C::STAGE + C::A_BYTES, &p.tmap_w, cluster_map(smem_u32(&ctl->full[s]), lead),
+                                     (kb0 + s) * C::BK, n0 + 128 * rank);
                 }
             }
             grid_wait();
@@ -339,9 +343,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::THREADS, 1)
                     }
                     uint8_t* st = smem + s * C::STAGE;
                     if (rank == 0 && it >= early) mbar_arrive_expect_tx(&ctl->full[s], 2 * C::STAGE);
-                    const uint32_t bar = cluster_map(smem_u32(&ctl->full[s]), 0);
-                    tma_load_2d_pair(st, &p.tmap_x, bar, kb * C::BK, m0 + 128 * rank);
-                    if (it >= early) tma_load_2d_pair(st + C::A_BYTES, &p.tmap_w, bar, kb * C::BK, n0 + 128 * rank);
+                    const uint32_t bar = cluster_map(smem_u32(&ctl->full[s]), lead);
+                    const int k = (kb0 + kb) * C::BK;
+                    tma_load_2d_pair(st, &p.tmap_x, bar, k, m0 + 128 * rank);
+                    if (it >= early) tma_load_2d_pair(st + C::A_BYTES, &p.tmap_w, bar, k, n0 + 128 * rank);
                 }
             }
             if (!ok) {  // gave up: time for the copies and MMAs in flight to end before the memory is given back
@@ -371,9 +376,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::THREADS, 1)
 #pragma unroll
                     for (int k = 0; k < C::BK; k += 32)
                         mma_i8_ss_pair(d, desc_sw128(a + k, 16, 1024), desc_sw128(b + k, 16, 1024), idesc, kb > 0 || k > 0);
-                    tc_commit_pair(&ctl->empty[s], 3);
+                    tc_commit_pair(&ctl->empty[s], 3 << lead);
                 }
-                if (ok) tc_commit_pair(&ctl->acc_full[i & 1], 3);
+                if (ok) tc_commit_pair(&ctl->acc_full[i & 1], 3 << lead);
             }
         }
     } else if (warp >= 4) {
@@ -402,26 +407,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::THREADS, 1)
             if (dead) continue;
             const float row_scale = row0 + lane < p.M ? p.x_scales[row0 + lane] : 0.f;
             const uint64_t sx = f2_pack(row_scale, row_scale);
-            const bool ok = mbar_wait_cluster(&ctl->acc_full[i & 1], (i >> 1) & 1, abort_flag, p.timeout);
-            if (!__all_sync(FULL, ok)) {
-                if (lane == 0) atomicOr(&g_int8_status, HB_DEV_TIMEOUT);
-                dead = true;
-                continue;
-            }
-            tc_fence_after();
-            const uint32_t acc = tmem + ((uint32_t)(32 * quarter) << 16) + (i & 1) * C::BN + 128 * half;
-#pragma unroll
-            for (int c = 0; c < 128; c += 64) {
-                uint32_t lo[32], hi[32];
-                tmem_ld32_async(acc + c, lo);
-                tmem_ld32_async(acc + c + 32, hi);
-                tmem_wait_ld(lo);
-                tmem_wait_ld(hi);
-                if (c == 64) {  // the accumulator is in registers: the next tile but one may take its place
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive_cluster(cluster_map(smem_u32(&ctl->acc_empty[i & 1]), 0));
-                }
+            // 64 columns of the warp's 32 rows from column c of its half: finished, staged, stored.
+            auto finish_columns = [&](int c, const uint32_t (&lo)[32], const uint32_t (&hi)[32]) {
                 if (lane == 0) bulk_wait_read<0>();
                 __syncwarp();
 #pragma unroll
@@ -469,11 +456,79 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::THREADS, 1)
                     }
                     __syncwarp();
                 }
+            };
+            const bool ok = __all_sync(FULL, mbar_wait_cluster(&ctl->acc_full[i & 1], (i >> 1) & 1, abort_flag, p.timeout));
+            if (!ok) {
+                if (lane == 0) atomicOr(&g_int8_status, HB_DEV_TIMEOUT);
+                dead = true;
+            }
+            tc_fence_after();
+            const uint32_t acc = tmem + ((uint32_t)(32 * quarter) << 16) + (i & 1) * C::BN + 128 * half;
+            uint32_t lo[32], hi[32];
+            auto read = [&](int c) {
+                tmem_ld32_async(acc + c, lo);
+                tmem_ld32_async(acc + c + 32, hi);
+                tmem_wait_ld(lo);
+                tmem_wait_ld(hi);
+            };
+            if constexpr (SPLIT == 1) {
+                if (dead) continue;
+#pragma unroll
+                for (int c = 0; c < 128; c += 64) {
+                    read(c);
+                    if (c == 64) {  // the accumulator is in registers: the next tile but one may take its place
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_cluster(cluster_map(smem_u32(&ctl->acc_empty[i & 1]), lead));
+                    }
+                    finish_columns(c, lo, hi);
+                }
+            } else {
+                // Every 64 columns have an owner among the pairs, to whom the others send
+                // their sums ([source][warp][column / 4][row][4], in the stages, which every
+                // MMA has read by the first barrier).  Every thread of the cluster arrives at
+                // both barriers, whatever happened before.
+                const uint32_t at = smem_u32(smem) + (ew * 16 * 32 + lane) * 16;
+                __syncwarp();
+                cluster_sync();
+#pragma unroll
+                for (int c = 0; c < 128; c += 64) {
+                    const int owner = (2 * half + c / 64) & (SPLIT - 1);
+                    if (dead || owner == part) continue;
+                    read(c);
+                    const uint32_t slot = (part - owner - 1) & (SPLIT - 1);
+                    const uint32_t to = cluster_map(at + slot * (C::EPI_WARPS * 16 * 32 * 16), 2 * owner + rank);
+#pragma unroll
+                    for (int v = 0; v < 32; v += 4) {
+                        st_cluster_v4(to + v / 4 * 512, lo[v], lo[v + 1], lo[v + 2], lo[v + 3]);
+                        st_cluster_v4(to + (v / 4 + 8) * 512, hi[v], hi[v + 1], hi[v + 2], hi[v + 3]);
+                    }
+                }
+                __syncwarp();
+                cluster_sync();
+                if (!dead && (SPLIT == 2 || half == part >> 1)) {  // this warp's columns of the owned ones
+                    const int c = 64 * (part & 1);
+                    read(c);
+                    for (int slot = 0; slot < SPLIT - 1; slot++) {
+                        const uint4* from = reinterpret_cast<const uint4*>(smem) + (slot * C::EPI_WARPS + ew) * 16 * 32 + lane;
+#pragma unroll
+                        for (int v = 0; v < 32; v += 4) {
+                            const uint4 a = from[v / 4 * 32], b = from[(v / 4 + 8) * 32];
+                            lo[v] += a.x, lo[v + 1] += a.y, lo[v + 2] += a.z, lo[v + 3] += a.w;
+                            hi[v] += b.x, hi[v + 1] += b.y, hi[v + 2] += b.z, hi[v + 3] += b.w;
+                        }
+                    }
+                    finish_columns(c, lo, hi);
+                }
             }
         }
         if (lane == 0) bulk_wait<0>();
     }
     __syncwarp();
+    if (SPLIT > 1 && warp < 4) {  // the two barriers of the exchange
+        cluster_sync();
+        cluster_sync();
+    }
     __syncthreads();
     cluster_sync();  // no CTA leaves while the other's MMAs read its memory or arrivals are on the way
     if (warp == 2) {
@@ -528,33 +583,72 @@ int configure(Kernel kern, int dev, int slot, int smem) {
     return HB_OK;
 }
 
-// CTAs that split K: doubled while each has an SM to itself, with two blocks of K at
-// least.  Clusters of four and more count 16 SMs of each of the eight processing
-// clusters only: the others cannot hold a whole one, and a second wave of a few
-// clusters costs as much as the first (128 x 3072, K 3072: 8.9 us with 2 CTAs for K,
-// 14.9 us with 3 on 144 SMs).
-int tile_split(const GemmParams& p, int bt, int sms) {
+// Clusters of 1, 2, 4 and 8 CTAs, one CTA per SM, that can be resident at once: not all
+// SMs' worth, since a cluster lies within one of the device's groups of SMs, and those
+// differ in size.
+struct Fit {
+    int clusters[4];
+};
+
+template <class Kernel>
+int max_clusters(Kernel kern, int size, int* n) {
+    HB_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, PairCfg::SMEM));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(size);
+    cfg.blockDim = dim3(PairCfg::THREADS);
+    cfg.dynamicSmemBytes = PairCfg::SMEM;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = size;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    HB_CUDA_TRY(cudaOccupancyMaxActiveClusters(n, kern, &cfg));
+    return HB_OK;
+}
+int cluster_fit(int dev, int sms, Fit* fit) {
+    static Fit known[64];
+    static bool asked[64];
+    std::lock_guard<std::mutex> lk(g_mu);
+    if (!asked[dev]) {
+        int rc;
+        int* n = known[dev].clusters;
+        n[0] = sms;
+        if ((rc = max_clusters(k_int8_pair<true, 0, 1>, 2, n + 1))) return rc;
+        if ((rc = max_clusters(k_int8_pair<true, 0, 2>, 4, n + 2))) return rc;
+        if ((rc = max_clusters(k_int8_pair<true, 0, 4>, 8, n + 3))) return rc;
+        asked[dev] = true;
+    }
+    *fit = known[dev];
+    return HB_OK;
+}
+
+// CTAs that split K: doubled while one round of their clusters holds every tile, with
+// two blocks of K at least; a second round of a few clusters costs as much as the first
+// (96 x 2048, K 8192: 10.5 us with 4 CTAs for K, 18.3 us with 8 on 128 SMs).
+int tile_split(const GemmParams& p, int bt, const Fit& fit) {
     const int64_t tiles = ceil_div(p.N, 128) * ceil_div(p.M, bt), nkb = ceil_div(p.K, 128);
-    int split = 1;
-    while (split < 8 && tiles * split * 2 <= (split == 1 ? sms : std::min(sms, 128)) && nkb >= 4 * split) split *= 2;
-    return split;
+    int log = 0;
+    while (log < 3 && tiles <= fit.clusters[log + 1] && nkb >= 4 << log) log++;
+    return 1 << log;
 }
 
 template <bool BF16, int BT>
-int launch_tile(const Int8Problem& q, GemmParams& p, int dev, const DeviceInfo& di, cudaStream_t st) {
+int launch_tile(const Int8Problem& q, GemmParams& p, const Fit& fit, int dev, cudaStream_t st) {
     using C = TileCfg<BT>;
     auto kern = k_int8_tile<BF16, BT>;
-    constexpr int slot = 8 + BF16 * 4 + (BT == 16 ? 0 : BT == 32 ? 1 : BT == 64 ? 2 : 3);
+    constexpr int slot = 16 + BF16 * 4 + (BT == 16 ? 0 : BT == 32 ? 1 : BT == 64 ? 2 : 3);
     int rc;
     if ((rc = configure(kern, dev, slot, C::smem(C::STAGES_ALONE)))) return rc;
     if ((rc = make_tmap_2d(&p.tmap_x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, q.x, p.M, p.K, q.x_rs, BT))) return rc;
     if ((rc = make_tmap_2d(&p.tmap_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, q.w, p.N, p.K, q.w_rs, C::BC))) return rc;
     const int64_t tn = ceil_div(p.N, C::BC), tm = ceil_div(p.M, BT);
-    const int split = tile_split(p, BT, di.sms);
+    const int split = tile_split(p, BT, fit);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(tn * split), (unsigned)tm);
     cfg.blockDim = dim3(256);
-    const int stages = tn * tm * split <= di.sms ? C::STAGES_ALONE : C::STAGES;
+    const int stages = tn * tm * split <= fit.clusters[0] ? C::STAGES_ALONE : C::STAGES;
     cfg.dynamicSmemBytes = C::smem(stages);
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
@@ -570,52 +664,23 @@ int launch_tile(const Int8Problem& q, GemmParams& p, int dev, const DeviceInfo& 
     return HB_OK;
 }
 
-// CTA pairs that can be resident at once (every SM, unless pairs do not fit some).
-template <class Kernel>
-int max_pairs(Kernel kern, int dev, int* pairs) {
-    static int known[64];
-    std::lock_guard<std::mutex> lk(g_mu);
-    int& n = known[dev];
-    if (!n) {
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(2);
-        cfg.blockDim = dim3(PairCfg::THREADS);
-        cfg.dynamicSmemBytes = PairCfg::SMEM;
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = 2;
-        attr[0].val.clusterDim.y = 1;
-        attr[0].val.clusterDim.z = 1;
-        cfg.attrs = attr;
-        cfg.numAttrs = 1;
-        HB_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, kern, &cfg));
-        if (n <= 0) {
-            n = 0;
-            return HB_ERR_UNSUPPORTED;
-        }
-    }
-    *pairs = n;
-    return HB_OK;
-}
-
-template <bool BF16, int ACT>
-int launch_pair(const Int8Problem& q, GemmParams& p, int dev, cudaStream_t st) {
+template <bool BF16, int ACT, int SPLIT>
+int launch_pair(const Int8Problem& q, GemmParams& p, const Fit& fit, int dev, cudaStream_t st) {
     using C = PairCfg;
-    auto kern = k_int8_pair<BF16, ACT>;
-    int pairs = 0, rc;
-    if ((rc = configure(kern, dev, BF16 * 2 + ACT, C::SMEM))) return rc;
-    if ((rc = max_pairs(kern, dev, &pairs))) return rc;
+    auto kern = k_int8_pair<BF16, ACT, SPLIT>;
+    const int clusters = fit.clusters[SPLIT == 4 ? 3 : SPLIT];
+    if (clusters <= 0) return HB_ERR_UNSUPPORTED;
+    int rc;
+    if ((rc = configure(kern, dev, (SPLIT / 2 * 2 + BF16) * 2 + ACT, C::SMEM))) return rc;
     if ((rc = make_tmap_2d(&p.tmap_x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, q.x, p.M, p.K, q.x_rs, 128))) return rc;
     if ((rc = make_tmap_2d(&p.tmap_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, q.w, p.N, p.K, q.w_rs, 128))) return rc;
-    p.tiles_m = (int)ceil_div(p.M, C::BM);
-    p.tiles_n = (int)ceil_div(p.N, C::BN);
     if (p.tma_out &&
         (rc = make_tmap_2d(&p.tmap_out, BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, p.out,
                            p.M, p.N, p.out_rs * 2, 32)))
         return rc;
     const int tiles = p.tiles_m * p.tiles_n;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(2 * (unsigned)std::min(tiles, pairs));
+    cfg.gridDim = dim3(2 * SPLIT * (unsigned)(SPLIT > 1 ? tiles : std::min(tiles, clusters)));  // split: one tile each
     cfg.blockDim = dim3(C::THREADS);
     cfg.dynamicSmemBytes = C::SMEM;
     cfg.stream = st;
@@ -627,6 +692,12 @@ int launch_pair(const Int8Problem& q, GemmParams& p, int dev, cudaStream_t st) {
     HB_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, p));
     return HB_OK;
 }
+template <bool BF16>
+int launch_pair(const Int8Problem& q, GemmParams& p, int split, const Fit& fit, int dev, cudaStream_t st) {
+    if (split == 4) return p.act ? launch_pair<BF16, 1, 4>(q, p, fit, dev, st) : launch_pair<BF16, 0, 4>(q, p, fit, dev, st);
+    if (split == 2) return p.act ? launch_pair<BF16, 1, 2>(q, p, fit, dev, st) : launch_pair<BF16, 0, 2>(q, p, fit, dev, st);
+    return p.act ? launch_pair<BF16, 1, 1>(q, p, fit, dev, st) : launch_pair<BF16, 0, 1>(q, p, fit, dev, st);
+}
 
 // Expected times in hundredths of a microsecond, from 70 shapes (65 to 4096 tokens, 640
 // to 12288 channels, K 256 to 12288) timed with every kernel.  A k-block of 128 bytes
@@ -635,25 +706,39 @@ int launch_pair(const Int8Problem& q, GemmParams& p, int dev, cudaStream_t st) {
 // 3072, K 3072 12.5 us in tiles of 128 tokens and 13.7 us in pairs, 1024 tokens 15.5
 // and 14.2 us; 512 x 3072 12.6 us in tiles of 64 and 12.2 us of 128, 192 tokens 9.1
 // and 10.6 us.
-int64_t tile_cost(const GemmParams& p, int bt, int sms) {
-    const int64_t split = tile_split(p, bt, sms);
+int64_t tile_cost(const GemmParams& p, int bt, const Fit& fit) {
+    const int64_t split = tile_split(p, bt, fit), sms = fit.clusters[0];
     const int64_t waves = ceil_div(ceil_div(p.N, 128) * ceil_div(p.M, bt) * split, sms), kb = ceil_div(ceil_div(p.K, 128), split);
     return (bt == 128 ? 550 : 430) + (split > 1 ? 100 : 0) + (waves - 1) * 130 + kb * (waves == 1 ? 28 : waves * 47 / 2);
 }
-int64_t pair_cost(const GemmParams& p, int sms) {
-    const int64_t rounds = ceil_div(ceil_div(p.M, 256) * ceil_div(p.N, 256), sms / 2);
-    return 700 + rounds * (ceil_div(p.K, 128) * 29 + (p.tma_out ? 0 : 250));  // 250: stores by value
+int64_t pair_cost(const GemmParams& p, int split, const Fit& fit) {
+    const int64_t rounds = ceil_div((int64_t)p.tiles_m * p.tiles_n * split, fit.clusters[0] / 2);
+    const int64_t kb = ceil_div(ceil_div(p.K, 128), split), by_value = p.tma_out ? 0 : 250;
+    return 700 + (split > 1 ? 200 : 0) + rounds * (kb * 29 + by_value);
+}
+// Pairs that split K: the best of those whose clusters hold every tile in one round
+// (512 x 4096, K 14336: 26.4 us with 2 pairs for K, 38.9 us with 1; 256 x 3072, K 12288:
+// 17.6 us with 4, 22.4 us with 2, 34.1 us with 1).
+int pair_split(const GemmParams& p, const Fit& fit) {
+    const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n, nkb = ceil_div(p.K, 128);
+    int split = 1;
+    if (tiles <= fit.clusters[2] && nkb >= 4 && pair_cost(p, 2, fit) < pair_cost(p, 1, fit)) split = 2;
+    if (tiles <= fit.clusters[3] && nkb >= 8 && pair_cost(p, 4, fit) < pair_cost(p, split, fit)) split = 4;
+    return split;
 }
 
 template <bool BF16>
-int launch_gemm(const Int8Problem& q, GemmParams& p, int dev, const DeviceInfo& di, cudaStream_t st) {
-    if (p.M <= 16) return launch_tile<BF16, 16>(q, p, dev, di, st);
-    if (p.M <= 32) return launch_tile<BF16, 32>(q, p, dev, di, st);
-    const int64_t narrow = tile_cost(p, 64, di.sms), wide = tile_cost(p, 128, di.sms);
-    if (p.M > 64 && (pair_cost(p, di.sms) < std::min(narrow, wide) || ceil_div(p.M, 64) > 65535))  // 65535: grid rows
-        return p.act ? launch_pair<BF16, 1>(q, p, dev, st) : launch_pair<BF16, 0>(q, p, dev, st);
-    if (p.M <= 64 || narrow <= wide) return launch_tile<BF16, 64>(q, p, dev, di, st);
-    return launch_tile<BF16, 128>(q, p, dev, di, st);
+int launch_gemm(const Int8Problem& q, GemmParams& p, const Fit& fit, int dev, cudaStream_t st) {
+    if (p.M <= 16) return launch_tile<BF16, 16>(q, p, fit, dev, st);
+    if (p.M <= 32) return launch_tile<BF16, 32>(q, p, fit, dev, st);
+    const int64_t narrow = tile_cost(p, 64, fit), wide = tile_cost(p, 128, fit);
+    if (p.M > 64) {
+        const int split = pair_split(p, fit);
+        if (pair_cost(p, split, fit) < std::min(narrow, wide) || ceil_div(p.M, 64) > 65535)  // 65535: grid rows
+            return launch_pair<BF16>(q, p, split, fit, dev, st);
+    }
+    if (p.M <= 64 || narrow <= wide) return launch_tile<BF16, 64>(q, p, fit, dev, st);
+    return launch_tile<BF16, 128>(q, p, fit, dev, st);
 }
 
 }  // namespace
@@ -669,10 +754,14 @@ int launch_int8_gemm(const Int8Problem& q, int dev, const DeviceInfo& di, bool e
     p.N = q.N;
     p.K = q.K;
     p.act = q.act;
+    p.tiles_m = (int)ceil_div(p.M, PairCfg::BM);
+    p.tiles_n = (int)ceil_div(p.N, PairCfg::BN);
     p.tma_out = aligned(p.out, 16) && (p.M == 1 || p.out_rs % 8 == 0);
     p.early_weights = early_weights;
     p.timeout = 2000LL * di.clock_khz;
-    return q.dtype == 1 ? launch_gemm<true>(q, p, dev, di, st) : launch_gemm<false>(q, p, dev, di, st);
+    Fit fit;
+    if (const int rc = cluster_fit(dev, di.sms, &fit)) return rc;
+    return q.dtype == 1 ? launch_gemm<true>(q, p, fit, dev, st) : launch_gemm<false>(q, p, fit, dev, st);
 }
 
 }  // namespace hb

@@ -473,3 +473,31 @@ def test_adaln_int8_layouts(b, s, c):
         assert bool(((rows.scales.double() - top / 127).abs() <= top / 127 * 2.0**-17).all())
         off = (rows.values.double() * rows.scales.double()[..., None] - h).abs()
         assert bool((off <= rows.scales.double()[..., None] * 0.5 + fuzz).all())
+
+
+# Few large tiles and a long K: two CTA pairs share a tile's K (500, 700 tokens), or four.
+@pytest.mark.parametrize("dtype,act", [(BF16, None), (FP16, "gelu_tanh")])
+@pytest.mark.parametrize("m,n,k", [(500, 3080, 9001), (500, 3079, 9001), (700, 1999, 9000), (1000, 648, 6000),
+                                   (260, 1500, 14000), (130, 3330, 14336), (512, 3072, 12288)])
+def test_products_with_split_inner_size(m, n, k, dtype, act):
+    import hilberta_b200 as hb
+
+    x, w16 = _rows(m, k, dtype, seed=k), _rows(n, k, dtype, seed=n, spread=0.0) * 0.05
+    w, bias = hb.quantize_rows(w16), _rows(1, n, dtype, seed=4)[0]
+    rows = hb.quantize_rows(x)
+    got = hb.int8_linear(rows, w, bias, activation=act)
+    _check_product(got, rows.values, rows.scales, w.values, w.scales, bias, act is not None)
+    assert torch.equal(got, hb.int8_linear(x, w, bias, activation=act))  # quantised in the call
+    few = torch.cat([hb.int8_linear(rows.row_slice(i, i + 60), w, bias, activation=act) for i in range(0, m, 60)])
+    assert torch.equal(got, few)  # other kernels, the same integers
+    wide = torch.full((m, n + 72), 7.0, dtype=dtype, device="cuda")
+    hb.int8_linear(rows, w, bias, activation=act, out=wide[:, 8 : n + 8])
+    assert torch.equal(wide[:, 8 : n + 8], got) and bool((wide[:, :8] == 7).all()) and bool((wide[:, n + 8 :] == 7).all())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        again = [hb.int8_linear(rows, w, bias, activation=act) for _ in range(3)]
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, got) for a in again)
+    assert hb.device_status() == 0
