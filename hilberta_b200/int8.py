@@ -20,6 +20,7 @@ from . import _lib
 
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1}
 _ACTIVATIONS = {None: 0, "gelu_tanh": 1}
+_MAX_ROWS = (1 << 31) - 1
 _used: set = set()  # devices with int8 launches (read by paired_kernel.device_status)
 
 
@@ -133,10 +134,10 @@ def quantize_rows(x, *, joined=None):
         raise ValueError("rows must be equally spaced")
     if ka + kb > _lib.HB_INT8_MAX_K:
         raise NotImplementedError(f"rows of more than {_lib.HB_INT8_MAX_K} values are not supported")
-    out = _empty_rows((*x.shape[:-1], ka + kb), x)
-    rows = out.scales.numel()
-    if rows >= 1 << 31:
+    rows = x.numel() // ka
+    if rows > _MAX_ROWS:
         raise NotImplementedError("2^31 rows or more are not supported")
+    out = _empty_rows((*x.shape[:-1], ka + kb), x)
     with _lib.on_device(x.device) as stream:
         rc = _lib.lib().hb_quantize_rows(
             x.data_ptr(), x_rs, ka, None if joined is None else joined.data_ptr(), j_rs, kb, rows, out.values.data_ptr(),
@@ -167,6 +168,8 @@ def int8_linear(x, weight, bias=None, *, activation=None, out=None):
     kind, dev = x.dtype, x.device
     if x_shape[-1] != K:
         raise ValueError("x and weight must have the same inner size")
+    if N > _MAX_ROWS or (x.scales.numel() if coded else x.numel() // K) > _MAX_ROWS:
+        raise NotImplementedError("2^31 rows or more are not supported")
     if weight.values.device != dev:
         raise ValueError("x and weight must be on the same CUDA device")
     act = _ACTIVATIONS.get(activation)

@@ -475,6 +475,18 @@ def test_adaln_int8_layouts(b, s, c):
         assert bool((off <= rows.scales.double()[..., None] * 0.5 + fuzz).all())
 
 
+@pytest.mark.parametrize("rows", [2**31, 2**32 + 5])
+def test_more_rows_than_32_bits_count_are_refused(rows):
+    import hilberta_b200 as hb
+
+    w = hb.quantize_rows(_rows(1, 1, BF16, seed=1))
+    x = torch.ones(1, 1, dtype=BF16, device="cuda").expand(rows, 1)  # rows of one element, all the same
+    with pytest.raises(NotImplementedError, match="2.31"):
+        hb.quantize_rows(x)
+    with pytest.raises(NotImplementedError, match="2.31"):
+        hb.int8_linear(x, w)
+
+
 # Few large tiles and a long K: two CTA pairs share a tile's K (500, 700 tokens), or four.
 @pytest.mark.parametrize("dtype,act", [(BF16, None), (FP16, "gelu_tanh")])
 @pytest.mark.parametrize("m,n,k", [(500, 3080, 9001), (500, 3079, 9001), (700, 1999, 9000), (1000, 648, 6000),
