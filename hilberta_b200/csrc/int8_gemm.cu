@@ -30,6 +30,8 @@ struct GemmParams {
     int M, N, K, act;
     int tma_out;  // out rows start on 16 bytes: TMA stores
     int tiles_m, tiles_n;
+    int tile0, tiles;  // pair kernel: of these tiles [tile0, tiles)
+    int turn;          // pair kernel: 1 or 2 of two launches that share the tiles, else 0
     int early_weights;  // the first weights are fetched before grid_wait
     long long timeout;
 };
@@ -283,7 +285,7 @@ __global__ void __cluster_dims__(2 * SPLIT, 1, 1) __launch_bounds__(PairCfg::THR
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int cta = (int)cluster_rank(), rank = cta & 1, lead = cta & ~1;  // in the cluster, in the pair, the pair's first
     const int part = cta >> 1;                                            // of K
-    const int first = blockIdx.x / (2 * SPLIT), step = gridDim.x / (2 * SPLIT), tiles = p.tiles_m * p.tiles_n;
+    const int first = p.tile0 + blockIdx.x / (2 * SPLIT), step = gridDim.x / (2 * SPLIT), tiles = p.tiles;
     const int blocks = (p.K + C::BK - 1) / C::BK;
     const int kb0 = blocks * part / SPLIT, nkb = blocks * (part + 1) / SPLIT - kb0;
 
@@ -328,7 +330,10 @@ __global__ void __cluster_dims__(2 * SPLIT, 1, 1) __launch_bounds__(PairCfg::THR
                                      (kb0 + s) * C::BK, n0 + 128 * rank);
                 }
             }
-            grid_wait();
+            // The second launch reads what the first has waited for, and starts on every
+            // SM that the first has left; its other warps wait for all of the first.
+            if (p.turn != 2) grid_wait();
+            if (p.turn == 1) grid_launch_dependents();
             int it = 0;
             bool ok = true;
             for (int t = first; t < tiles && ok; t += step) {
@@ -358,7 +363,7 @@ __global__ void __cluster_dims__(2 * SPLIT, 1, 1) __launch_bounds__(PairCfg::THR
     } else if (warp == 1) {
         if (lane == 0 && rank == 0) {
             constexpr uint32_t idesc = idesc_i8(C::BM, C::BN);
-            grid_wait();  // the clock of the waits starts when the copies can
+            if (p.turn != 2) grid_wait();  // the clock of the waits starts when the copies can
             int it = 0, i = 0;
             bool ok = true;
             for (int t = first; t < tiles && ok; t += step, i++) {
@@ -664,21 +669,15 @@ int launch_tile(const Int8Problem& q, GemmParams& p, const Fit& fit, int dev, cu
     return HB_OK;
 }
 
+// Tiles [p.tile0, p.tiles) by SPLIT pairs each.
 template <bool BF16, int ACT, int SPLIT>
-int launch_pair(const Int8Problem& q, GemmParams& p, const Fit& fit, int dev, cudaStream_t st) {
+int launch_pair(GemmParams& p, const Fit& fit, int dev, cudaStream_t st) {
     using C = PairCfg;
     auto kern = k_int8_pair<BF16, ACT, SPLIT>;
-    const int clusters = fit.clusters[SPLIT == 4 ? 3 : SPLIT];
+    const int clusters = fit.clusters[SPLIT == 4 ? 3 : SPLIT], tiles = p.tiles - p.tile0;
     if (clusters <= 0) return HB_ERR_UNSUPPORTED;
     int rc;
     if ((rc = configure(kern, dev, (SPLIT / 2 * 2 + BF16) * 2 + ACT, C::SMEM))) return rc;
-    if ((rc = make_tmap_2d(&p.tmap_x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, q.x, p.M, p.K, q.x_rs, 128))) return rc;
-    if ((rc = make_tmap_2d(&p.tmap_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, q.w, p.N, p.K, q.w_rs, 128))) return rc;
-    if (p.tma_out &&
-        (rc = make_tmap_2d(&p.tmap_out, BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, p.out,
-                           p.M, p.N, p.out_rs * 2, 32)))
-        return rc;
-    const int tiles = p.tiles_m * p.tiles_n;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2 * SPLIT * (unsigned)(SPLIT > 1 ? tiles : std::min(tiles, clusters)));  // split: one tile each
     cfg.blockDim = dim3(C::THREADS);
@@ -693,10 +692,30 @@ int launch_pair(const Int8Problem& q, GemmParams& p, const Fit& fit, int dev, cu
     return HB_OK;
 }
 template <bool BF16>
-int launch_pair(const Int8Problem& q, GemmParams& p, int split, const Fit& fit, int dev, cudaStream_t st) {
-    if (split == 4) return p.act ? launch_pair<BF16, 1, 4>(q, p, fit, dev, st) : launch_pair<BF16, 0, 4>(q, p, fit, dev, st);
-    if (split == 2) return p.act ? launch_pair<BF16, 1, 2>(q, p, fit, dev, st) : launch_pair<BF16, 0, 2>(q, p, fit, dev, st);
-    return p.act ? launch_pair<BF16, 1, 1>(q, p, fit, dev, st) : launch_pair<BF16, 0, 1>(q, p, fit, dev, st);
+int launch_pair(GemmParams& p, int split, const Fit& fit, int dev, cudaStream_t st) {
+    if (split == 4) return p.act ? launch_pair<BF16, 1, 4>(p, fit, dev, st) : launch_pair<BF16, 0, 4>(p, fit, dev, st);
+    if (split == 2) return p.act ? launch_pair<BF16, 1, 2>(p, fit, dev, st) : launch_pair<BF16, 0, 2>(p, fit, dev, st);
+    return p.act ? launch_pair<BF16, 1, 1>(p, fit, dev, st) : launch_pair<BF16, 0, 1>(p, fit, dev, st);
+}
+// All tiles: the first `whole` by a pair each, the others by `split`.
+template <bool BF16>
+int launch_pairs(const Int8Problem& q, GemmParams& p, int whole, int split, const Fit& fit, int dev, cudaStream_t st) {
+    int rc;
+    if ((rc = make_tmap_2d(&p.tmap_x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, q.x, p.M, p.K, q.x_rs, 128))) return rc;
+    if ((rc = make_tmap_2d(&p.tmap_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, q.w, p.N, p.K, q.w_rs, 128))) return rc;
+    if (p.tma_out &&
+        (rc = make_tmap_2d(&p.tmap_out, BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, p.out,
+                           p.M, p.N, p.out_rs * 2, 32)))
+        return rc;
+    const int tiles = p.tiles_m * p.tiles_n;
+    p.tile0 = 0;
+    p.tiles = whole;
+    p.turn = whole > 0 && whole < tiles;
+    if (whole > 0 && (rc = launch_pair<BF16>(p, 1, fit, dev, st))) return rc;
+    p.tile0 = whole;
+    p.tiles = tiles;
+    if (p.turn) p.turn = 2, p.early_weights = 0;
+    return whole < tiles ? launch_pair<BF16>(p, split, fit, dev, st) : HB_OK;
 }
 
 // Expected times in hundredths of a microsecond, from 70 shapes (65 to 4096 tokens, 640
@@ -711,20 +730,26 @@ int64_t tile_cost(const GemmParams& p, int bt, const Fit& fit) {
     const int64_t waves = ceil_div(ceil_div(p.N, 128) * ceil_div(p.M, bt) * split, sms), kb = ceil_div(ceil_div(p.K, 128), split);
     return (bt == 128 ? 550 : 430) + (split > 1 ? 100 : 0) + (waves - 1) * 130 + kb * (waves == 1 ? 28 : waves * 47 / 2);
 }
-int64_t pair_cost(const GemmParams& p, int split, const Fit& fit) {
-    const int64_t rounds = ceil_div((int64_t)p.tiles_m * p.tiles_n * split, fit.clusters[0] / 2);
-    const int64_t kb = ceil_div(ceil_div(p.K, 128), split), by_value = p.tma_out ? 0 : 250;
-    return 700 + (split > 1 ? 200 : 0) + rounds * (kb * 29 + by_value);
-}
-// Pairs that split K: the best of those whose clusters hold every tile in one round
-// (512 x 4096, K 14336: 26.4 us with 2 pairs for K, 38.9 us with 1; 256 x 3072, K 12288:
-// 17.6 us with 4, 22.4 us with 2, 34.1 us with 1).
-int pair_split(const GemmParams& p, const Fit& fit) {
-    const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n, nkb = ceil_div(p.K, 128);
-    int split = 1;
-    if (tiles <= fit.clusters[2] && nkb >= 4 && pair_cost(p, 2, fit) < pair_cost(p, 1, fit)) split = 2;
-    if (tiles <= fit.clusters[3] && nkb >= 8 && pair_cost(p, 4, fit) < pair_cost(p, split, fit)) split = 4;
-    return split;
+// Pairs: whole rounds of tiles first, and what is left (or everything, if that is less
+// than a round) with as many pairs for each tile's K as their clusters fit, if that pays:
+// 512 x 4096, K 14336: 26.4 us with 2 pairs for K, 38.9 us with 1; 256 x 3072, K 12288:
+// 17.6 us with 4, 22.4 us with 2, 34.1 us with 1; 1280 x 4096 (74 tiles and 6), K 14336:
+// 58.7 us with 4 for the 6, 74.1 us with 1; K 4096: 28.6 and 26.8 us.
+struct PairPlan {
+    int64_t cost;
+    int whole, split;
+};
+PairPlan plan_pairs(const GemmParams& p, const Fit& fit) {
+    const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n, nkb = ceil_div(p.K, 128), pairs = fit.clusters[1];
+    const int64_t by_value = p.tma_out ? 0 : 250, round = nkb * 29 + by_value, left = tiles % pairs;
+    PairPlan best = {700 + ceil_div(tiles, pairs) * round, (int)tiles, 1};
+    for (int log = 1; log < 3 && nkb >= 4 << (log - 1); log++) {
+        if (left > fit.clusters[log + 1]) break;
+        const int64_t start = tiles < pairs ? 200 : log == 1 ? 700 : 880;  // the exchange, and of a second launch
+        const int64_t cost = 700 + tiles / pairs * round + start + ceil_div(nkb, 1 << log) * 29 + by_value;
+        if (left && cost < best.cost) best = {cost, (int)(tiles - left), 1 << log};
+    }
+    return best;
 }
 
 template <bool BF16>
@@ -732,10 +757,10 @@ int launch_gemm(const Int8Problem& q, GemmParams& p, const Fit& fit, int dev, cu
     if (p.M <= 16) return launch_tile<BF16, 16>(q, p, fit, dev, st);
     if (p.M <= 32) return launch_tile<BF16, 32>(q, p, fit, dev, st);
     const int64_t narrow = tile_cost(p, 64, fit), wide = tile_cost(p, 128, fit);
-    if (p.M > 64) {
-        const int split = pair_split(p, fit);
-        if (pair_cost(p, split, fit) < std::min(narrow, wide) || ceil_div(p.M, 64) > 65535)  // 65535: grid rows
-            return launch_pair<BF16>(q, p, split, fit, dev, st);
+    if (p.M > 64 && fit.clusters[1] > 0) {
+        const PairPlan plan = plan_pairs(p, fit);
+        if (plan.cost < std::min(narrow, wide) || ceil_div(p.M, 64) > 65535)  // 65535: grid rows
+            return launch_pairs<BF16>(q, p, plan.whole, plan.split, fit, dev, st);
     }
     if (p.M <= 64 || narrow <= wide) return launch_tile<BF16, 64>(q, p, fit, dev, st);
     return launch_tile<BF16, 128>(q, p, fit, dev, st);

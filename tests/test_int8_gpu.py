@@ -513,3 +513,36 @@ def test_products_with_split_inner_size(m, n, k, dtype, act):
     torch.cuda.synchronize()
     assert all(torch.equal(a, got) for a in again)
     assert hb.device_status() == 0
+
+
+# A round of tiles and a few more: the few are shared by two or four pairs each, in a
+# second launch that begins while the first ends.
+@pytest.mark.parametrize("m,n,k", [(1280, 4096, 9000), (2600, 4093, 8200), (19201, 256, 6200)])
+def test_products_with_a_split_last_round(m, n, k):
+    import hilberta_b200 as hb
+
+    x, w16 = _rows(m, k, BF16, seed=k), _rows(n, k, BF16, seed=n, spread=0.0) * 0.05
+    w, bias = hb.quantize_rows(w16), _rows(1, n, BF16, seed=4)[0]
+    rows = hb.quantize_rows(x)
+    got = hb.int8_linear(rows, w, bias, activation="gelu_tanh")
+    for i in range(0, m, 3000):
+        part = rows.row_slice(i, min(m, i + 3000))
+        _check_product(got[i : i + 3000], part.values, part.scales, w.values, w.scales, bias, True)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        again = [hb.int8_linear(x, w, bias, activation="gelu_tanh") for _ in range(3)]
+        after = hb.quantize_rows(again[2])  # reads all of the product's tiles
+    for _ in range(3):
+        for a in again:
+            a.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, got) for a in again)
+    want = hb.quantize_rows(got)
+    assert torch.equal(after.values, want.values) and torch.equal(after.scales, want.scales)
+    # back to back: codes rewritten by the next call's quantisation as soon as a product ends
+    other = x * 0.5
+    want = hb.int8_linear(other, w, bias, activation="gelu_tanh")
+    for _ in range(10):
+        a, b = hb.int8_linear(x, w, bias, activation="gelu_tanh"), hb.int8_linear(other, w, bias, activation="gelu_tanh")
+    assert torch.equal(a, got) and torch.equal(b, want) and hb.device_status() == 0
