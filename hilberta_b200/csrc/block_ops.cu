@@ -213,16 +213,16 @@ __device__ __forceinline__ float sum_of(int n, float v) {  // over n lanes, a po
 // instructions, so two fp32 operations go in one, a lane holds as many elements as C
 // divides into (the reductions' instructions are per lane), every lane equally many
 // (no tests), and mean and variance share one barrier.  The CTAs are persistent, keep
-// the modulation of their batch entry and fetch DEPTH rows ahead; the register limits
+// the modulation of their batch entry and fetch a row ahead; the register limits
 // keep 12 to 16 warps on an SM (16384 x 3072 with the residual: 55.8 us at 128
 // registers, 60.9 at 156).  16384 x 3072, bf16, from DRAM: 55.8 us (6.3 TB/s) with the
-// residual, 32.7 (4.6 TB/s) without; 33975 x 1280: 59.0 and 45.6 (one vector per lane,
-// so the reductions weigh most).
+// residual, 31.9 (4.7 TB/s) without, 32.7 with two rows ahead; 33975 x 1280: 58.2 and
+// 43.8 (one vector per lane, so the reductions weigh most).
 //
 // Mean and variance: from the means m and the sums d of squared deviations of sets of
 // n elements each, mean = sum m / sets and d = sum (d + n (m - mean)^2), first over a
 // warp's lanes, then over the warps; large sums are never subtracted.
-template <bool BF16, bool RESIDUAL, int NV, int DEPTH>
+template <bool BF16, bool RESIDUAL, int NV>
 __global__ void __launch_bounds__(NV == 1 ? 512 : NV == 4 ? 128 : 256, NV == 4 ? 3 : 2)
     k_adaln_int8(const __grid_constant__ AdaInt8Params q) {
     using namespace ptx;
@@ -241,8 +241,8 @@ __global__ void __launch_bounds__(NV == 1 ? 512 : NV == 4 ? 128 : 256, NV == 4 ?
         s_mag[threadIdx.x] = 0;
     }
     __syncthreads();
-    uint4 x[DEPTH][NV], y[DEPTH][NV];
-    auto fetch = [&](int row, uint4 (&x)[NV], uint4 (&y)[NV]) {
+    uint4 x[NV], y[NV];
+    auto fetch = [&](int row) {
         if (row >= p.rows) return;
         const E* px = static_cast<const E*>(p.x) + row * p.x_rs + c0;
         const E* py = static_cast<const E*>(p.y) + row * p.y_rs + c0;
@@ -256,7 +256,9 @@ __global__ void __launch_bounds__(NV == 1 ? 512 : NV == 4 ? 128 : 256, NV == 4 ?
     uint4 gate[NV];
     int batch_end = 0;  // modulation of rows [.., batch_end)
     const uint64_t one = f2_pack(1.f, 1.f), magic = f2_pack(12582912.f, 12582912.f);
-    auto work = [&](int row, uint4 (&x)[NV], uint4 (&y)[NV]) {
+    grid_launch_dependents();  // the product's CTAs may set themselves up meanwhile
+    fetch(blockIdx.x);
+    for (int row = blockIdx.x; row < p.rows; row += step) {  // the same for the whole CTA
         if (row >= batch_end) {
             const int batch = row / p.rows_per_batch;
             batch_end = (batch + 1) * p.rows_per_batch;
@@ -286,7 +288,7 @@ __global__ void __launch_bounds__(NV == 1 ? 512 : NV == 4 ? 128 : 256, NV == 4 ?
             }
             sum = f2_add(sum, f2_add(f2_add(f[i][0], f[i][1]), f2_add(f[i][2], f[i][3])));
         }
-        fetch(row + DEPTH * step, x, y);
+        fetch(row + step);
         constexpr float n = 8.f * NV;
         float a, b;
         f2_unpack(sum, a, b);
@@ -346,17 +348,6 @@ __global__ void __launch_bounds__(NV == 1 ? 512 : NV == 4 ? 128 : 256, NV == 4 ?
             if (!rs.live) o = make_uint2(0, 0);
             *reinterpret_cast<uint2*>(out + i * cs) = o;
         }
-    };
-    grid_launch_dependents();  // the product's CTAs may set themselves up meanwhile
-    int row = blockIdx.x;
-#pragma unroll
-    for (int k = 0; k < DEPTH; ++k) fetch(row + k * step, x[k], y[k]);
-    while (row < p.rows) {  // the same for the whole CTA
-#pragma unroll
-        for (int k = 0; k < DEPTH; ++k) {
-            if (row < p.rows) work(row, x[k], y[k]);
-            row += step;
-        }
     }
 }
 
@@ -375,8 +366,7 @@ int resident_ctas(Kernel kern, int variant, int threads, int* n) {
 
 template <bool BF16, bool RESIDUAL, int NV>
 int launch_adaln_int8(const AdaInt8Params& p, int sms, cudaStream_t st) {
-    constexpr int DEPTH = RESIDUAL ? 1 : 2;  // the residual's second stream doubles what is in flight
-    auto kern = k_adaln_int8<BF16, RESIDUAL, NV, DEPTH>;
+    auto kern = k_adaln_int8<BF16, RESIDUAL, NV>;
     const int threads = p.a.C / (8 * NV);
     int per_sm = 0;
     if (const int rc = resident_ctas(kern, (BF16 * 2 + RESIDUAL) * 4 + NV - 1, threads, &per_sm)) return rc;
@@ -391,8 +381,8 @@ int launch_adaln_int8(const AdaInt8Params& p, cudaStream_t st) {
     HB_CUDA_TRY(cudaGetDevice(&dev));
     HB_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
     // Vectors per lane: three or four if they divide the row into whole warps, else two
-    // or one.  With and without the residual, 16384 x 3072: three 55.9 and 32.7 us, four
-    // 56.6 and 33.2, two 69.1 and 47.3; 3590 x 2048: four 9.1 and 6.7, two 9.6 and 7.4.
+    // or one.  With and without the residual, 16384 x 3072: three 55.7 and 31.9 us, four
+    // 56.6 and 31.6, two 68.8 and 46.2; 3590 x 2048: four 9.1 and 6.3, two 9.6 and 7.1.
     const int groups = p.a.C / 256;
     if (groups % 3 == 0) return launch_adaln_int8<BF16, RESIDUAL, 3>(p, sms, st);
     if (groups % 4 == 0) return launch_adaln_int8<BF16, RESIDUAL, 4>(p, sms, st);
