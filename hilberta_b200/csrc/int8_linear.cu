@@ -100,7 +100,7 @@ __device__ __forceinline__ void store8(const QuantParams& p, int64_t row, int t,
     }
 }
 
-// T threads per row (a warp, or the whole CTA), up to kQuantVec vectors of 8
+// T threads per row (a warp of four, or the whole CTA), up to kQuantVec vectors of 8
 // values each: the row is read once and stays in registers between its maximum
 // and its codes.  Memory-bound (2 K bytes read, K written per row): CTAs are
 // persistent and each thread fetches its part of the next row before it works on
@@ -108,8 +108,8 @@ __device__ __forceinline__ void store8(const QuantParams& p, int64_t row, int t,
 constexpr int kQuantVec = 4;
 
 template <bool BF16, int W, int T>
-__global__ void __launch_bounds__(T < 128 ? 128 : T) k_quantize_rows(const __grid_constant__ QuantParams p) {
-    constexpr int CTA = T < 128 ? 128 : T;
+__global__ void __launch_bounds__(T == 32 ? 128 : T) k_quantize_rows(const __grid_constant__ QuantParams p) {
+    constexpr int CTA = T == 32 ? 128 : T;
     constexpr int RPC = CTA / T;
     constexpr int NV = kQuantVec;
     __shared__ uint32_t s_max[2][CTA / 32];
@@ -171,18 +171,30 @@ __global__ void __launch_bounds__(512) k_quantize_long(const __grid_constant__ Q
 
 template <bool BF16, int W>
 int launch_quantize(const QuantParams& p, int sms, cudaStream_t st) {
-    // Threads per row: the fewest whose registers hold it (a warp up to 1024
-    // columns); persistent CTAs, as many as fill the SMs' 2048 threads.
-    const int64_t groups = p.k <= 8 * kQuantVec * 32 ? ceil_div(p.rows, 4) : p.rows;
-    auto grid = [&](int cta) { return (unsigned)std::min<int64_t>(groups, (int64_t)sms * (2048 / cta)); };
-    if (p.k <= 8 * kQuantVec * 32)
-        k_quantize_rows<BF16, W, 32><<<grid(128), 128, 0, st>>>(p);
-    else if (p.k <= 8 * kQuantVec * 128)
-        k_quantize_rows<BF16, W, 128><<<grid(128), 128, 0, st>>>(p);
-    else if (p.k <= 8 * kQuantVec * 256)
-        k_quantize_rows<BF16, W, 256><<<grid(256), 256, 0, st>>>(p);
-    else if (p.k <= 8 * kQuantVec * 512)
-        k_quantize_rows<BF16, W, 512><<<grid(512), 512, 0, st>>>(p);
+    // Threads per row: the fewest of these whose registers hold it (8192 x 2048: 8.7 us
+    // with 64, 13.5 with 128; 16384 x 3072: 23.8 us with 96, 25.4 with 128; a number only
+    // known at run time costs a quarter more than any); persistent CTAs, as many as fill
+    // the SMs' 2048 threads.
+    const int64_t warps = ceil_div(p.k, 8 * kQuantVec * 32);
+    auto start = [&](auto kern, int cta, int rows) {
+        kern<<<(unsigned)std::min<int64_t>(ceil_div(p.rows, rows), (int64_t)sms * (2048 / cta)), cta, 0, st>>>(p);
+    };
+    if (warps <= 1)
+        start(k_quantize_rows<BF16, W, 32>, 128, 4);
+    else if (warps <= 2)
+        start(k_quantize_rows<BF16, W, 64>, 64, 1);
+    else if (warps <= 3)
+        start(k_quantize_rows<BF16, W, 96>, 96, 1);
+    else if (warps <= 4)
+        start(k_quantize_rows<BF16, W, 128>, 128, 1);
+    else if (warps <= 6)
+        start(k_quantize_rows<BF16, W, 192>, 192, 1);
+    else if (warps <= 8)
+        start(k_quantize_rows<BF16, W, 256>, 256, 1);
+    else if (warps <= 12)
+        start(k_quantize_rows<BF16, W, 384>, 384, 1);
+    else if (warps <= 16)
+        start(k_quantize_rows<BF16, W, 512>, 512, 1);
     else
         k_quantize_long<BF16, W><<<p.rows, 512, 0, st>>>(p);
     HB_LAUNCH_CHECK();
