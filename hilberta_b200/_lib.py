@@ -158,8 +158,7 @@ _SIGS = {
     ),
     "hb_norm_rope_qk": (
         _I,
-        [_P, _P, _P, _P, ctypes.POINTER(ctypes.c_int64), _I, _I, _I, _I, _I, _I, _P, _P, _P, _P, ctypes.c_float, _P, _P,
-         _I, _P],
+        [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P, _P, _P, ctypes.c_float, _P, _P, _I, _P],
     ),
     "hb_paired_fwd_noalloc": (
         _I,

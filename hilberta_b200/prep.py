@@ -22,6 +22,7 @@ order, giving the physical layout the plain kernel reads).  No CPU path.
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import torch
 
@@ -105,7 +106,7 @@ def prepare_qkv(q_txt, k_txt, v_txt, q_img, k_img, v_img, *, heads, norm_q, norm
     return q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2)
 
 
-_Strides = ctypes.c_int64 * 12
+_STRIDES = struct.Struct("12q")
 
 
 def norm_rope_qk(q, k, *, weight_q, weight_k, cos, sin, text_tokens=0, weight_txt_q=None, weight_txt_k=None, eps=1e-6,
@@ -121,7 +122,7 @@ def norm_rope_qk(q, k, *, weight_q, weight_k, cos, sin, text_tokens=0, weight_tx
     one rounding at the end (``norm_rope_pack`` keeps the rounding of the separate
     ops it replaces).  ``out`` is a pair of tensors like q and k, ``(q, k)`` itself
     for in place; by default new contiguous ones.  Returns the pair."""
-    if q.ndim != 4 or k.ndim != 4 or not q.is_cuda or q.stride(3) != 1 or k.stride(3) != 1:
+    if q.ndim != 4 or k.ndim != 4 or not q.is_cuda or q.stride()[3] != 1 or k.stride()[3] != 1:
         raise ValueError("q and k must be CUDA tensors [B, S, heads, D] with contiguous D")
     kind, dev = q.dtype, q.device
     dtype = _dtype_code(q)
@@ -139,7 +140,7 @@ def norm_rope_qk(q, k, *, weight_q, weight_k, cos, sin, text_tokens=0, weight_tx
     weights = (weight_q, weight_k) if weight_txt_q is None and weight_txt_k is None else (weight_q, weight_k, weight_txt_q,
                                                                                         weight_txt_k)
     for w in weights:
-        if w is not None and (w.shape != (D,) or w.dtype != kind or w.device != dev or (D > 1 and w.stride(0) != 1)):
+        if w is not None and (w.shape != (D,) or w.dtype != kind or w.device != dev or not w.is_contiguous()):
             raise ValueError("norm weights must be contiguous [D] in the heads' dtype")
     for c in (cos, sin):
         if c is None or c.shape != (S, D) or c.dtype != torch.float32 or c.device != dev or not c.is_contiguous():
@@ -151,11 +152,11 @@ def norm_rope_qk(q, k, *, weight_q, weight_k, cos, sin, text_tokens=0, weight_tx
             if t is not None and t.requires_grad:
                 raise ValueError("Inference only; disable autograd")
     if out is None:
-        q_out, k_out = q.new_empty((B, S, Hq, D)), k.new_empty((B, S, Hk, D))
+        q_out, k_out = q.new_empty(B, S, Hq, D), k.new_empty(B, S, Hk, D)
     else:
         _check_qk_out(q, k, out, [t for t in (cos, sin, *weights) if t is not None])
         q_out, k_out = out
-    strides = _Strides(*q.stride()[:3], *k.stride()[:3], *q_out.stride()[:3], *k_out.stride()[:3])
+    strides = _STRIDES.pack(*q.stride()[:3], *k.stride()[:3], *q_out.stride()[:3], *k_out.stride()[:3])
     with _lib.on_device(dev) as stream:
         rc = _lib.lib().hb_norm_rope_qk(
             q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr(), strides, B, S, T, Hq, Hk, D,
