@@ -172,7 +172,8 @@ __global__ void __launch_bounds__(512) k_quantize_long(const __grid_constant__ Q
 template <bool BF16, int W>
 int launch_quantize(const QuantParams& p, int sms, cudaStream_t st) {
     // Threads per row: the fewest of these whose registers hold it (8192 x 2048: 8.7 us
-    // with 64, 13.5 with 128; 16384 x 3072: 23.8 us with 96, 25.4 with 128; a number only
+    // with 64, 13.5 with 128; 16384 x 3072: 23.8 us with 96, 25.4 with 128; 8192 x 5120:
+    // 20.6 us with 160, 21.9 with 192; 8192 x 14336: the same with 448 and 512; a number only
     // known at run time costs a quarter more than any); persistent CTAs, as many as fill
     // the SMs' 2048 threads.
     const int64_t warps = ceil_div(p.k, 8 * kQuantVec * 32);
@@ -187,10 +188,14 @@ int launch_quantize(const QuantParams& p, int sms, cudaStream_t st) {
         start(k_quantize_rows<BF16, W, 96>, 96, 1);
     else if (warps <= 4)
         start(k_quantize_rows<BF16, W, 128>, 128, 1);
+    else if (warps <= 5)
+        start(k_quantize_rows<BF16, W, 160>, 160, 1);
     else if (warps <= 6)
         start(k_quantize_rows<BF16, W, 192>, 192, 1);
     else if (warps <= 8)
         start(k_quantize_rows<BF16, W, 256>, 256, 1);
+    else if (warps <= 10)
+        start(k_quantize_rows<BF16, W, 320>, 320, 1);
     else if (warps <= 12)
         start(k_quantize_rows<BF16, W, 384>, 384, 1);
     else if (warps <= 16)

@@ -548,7 +548,7 @@ def test_products_with_a_split_last_round(m, n, k):
     assert torch.equal(a, got) and torch.equal(b, want) and hb.device_status() == 0
 
 
-@pytest.mark.parametrize("k", [1024, 1025, 2048, 2049, 3080, 4096, 4100, 6144, 6160, 8192, 8193, 12288, 12296, 16384, 16385])
+@pytest.mark.parametrize("k", [1024, 1025, 2048, 2049, 3080, 4096, 4100, 5120, 5128, 6144, 6160, 8192, 8193, 10240, 10241, 12288, 12296, 16384, 16385])
 def test_quantize_rows_at_every_width_of_a_row(k):
     """The longest row of every number of threads, and one that needs more; more rows than CTAs."""
     import hilberta_b200 as hb
