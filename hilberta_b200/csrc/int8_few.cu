@@ -3,10 +3,11 @@
 // bytes of every channel's row, with 4-way 8-bit dot products; the tokens' codes lie
 // in shared memory, quantised there from 16 bits by each CTA (they are a few KB; the
 // first weights are on their way meanwhile).  Sums and results are those of the
-// tensor-core kernels, bit for bit.  1 x 18432 with K 3072: 11.5 us (4.9 TB/s) from
-// DRAM, 2.5 us of it the launch and the token, with four CTAs per SM (all 576 at once);
-// 14.3 us with three.  Rings of asynchronous copies per warp, 192 KB on their way per SM,
-// took 11.6 us and 0.5 us more for small products.
+// tensor-core kernels, bit for bit.  1 x 18432 with K 3072: 11.2 us (5.1 TB/s) from
+// DRAM, 2.5 us of it the launch and the token, with four CTAs per SM (all 576 at once),
+// 14.3 us with three; two tokens 12.7 us, 16.0 us with two CTAs per SM.  Rings of
+// asynchronous copies per warp, 192 KB on their way per SM, took 11.6 us for one token
+// and 0.5 us more for small products.
 #include <climits>
 
 #include "int8_common.cuh"
@@ -17,6 +18,7 @@ namespace {
 constexpr unsigned FULL = 0xffffffffu;
 constexpr int kRows = 2;
 constexpr int kSmem = 40 * 1024;  // codes of the tokens, at most
+constexpr int kResident = 4;      // CTAs per SM
 
 // 16 bytes of a row of codes, of which `left` (at least 1) are inside it.
 __device__ __forceinline__ int4 load_codes(const int8_t* p, int left) {
@@ -27,7 +29,7 @@ __device__ __forceinline__ int4 load_codes(const int8_t* p, int left) {
 }
 
 template <bool BF16, bool CODES, int M, int R>
-__global__ void __launch_bounds__(256, M == 1 ? 4 : 2) k_int8_few(const __grid_constant__ Int8Problem p) {
+__global__ void __launch_bounds__(256, kResident) k_int8_few(const __grid_constant__ Int8Problem p) {
     extern __shared__ __align__(16) int8_t s_codes[];  // [M][pitch]
     __shared__ uint32_t s_mag[M][8];
     __shared__ float s_scale[M];
@@ -147,11 +149,15 @@ int launch(const Int8Problem& p, cudaStream_t st) {
 
 template <bool BF16, bool CODES>
 int launch(const Int8Problem& p, int sms, cudaStream_t st) {
-    // Channels per warp: four where that leaves every SM a CTA, so that a token's
-    // codes are read from shared memory once for four channels.
-    const bool wide = p.N >= 32 * sms;
-    if (p.M == 1) return wide ? launch<BF16, CODES, 1, 4>(p, st) : launch<BF16, CODES, 1, 1>(p, st);
-    return wide ? launch<BF16, CODES, 2, 4>(p, st) : launch<BF16, CODES, 2, 1>(p, st);
+    // Channels per warp: the fewest of 1, 2 and 4 for which all CTAs run at once, since
+    // each begins with the tokens' codes; and 4 past that.  One token: 8192 x 8192 14.5 us
+    // with 2, 16.8 with 4, 17.5 with 1; 9216 x 3072 7.4 with 2, 8.3 with 4, 9.7 with 1; 4096
+    // x 14336 15.0 with 1, 20.9 with 4; 12288 x 3072 9.4 with 4, 10.8 with 2.
+    const int64_t warps = 8LL * sms * kResident;
+    const int r = p.N <= warps ? 1 : p.N <= 2 * warps ? 2 : 4;
+    if (p.M == 1)
+        return r == 1 ? launch<BF16, CODES, 1, 1>(p, st) : r == 2 ? launch<BF16, CODES, 1, 2>(p, st) : launch<BF16, CODES, 1, 4>(p, st);
+    return r == 1 ? launch<BF16, CODES, 2, 1>(p, st) : r == 2 ? launch<BF16, CODES, 2, 2>(p, st) : launch<BF16, CODES, 2, 4>(p, st);
 }
 
 }  // namespace

@@ -557,3 +557,18 @@ def test_quantize_rows_at_every_width_of_a_row(k):
     got = hb.quantize_rows(x)
     codes, scales = _quantised(x)
     assert torch.equal(got.values, codes) and torch.equal(got.scales, scales)
+
+
+@pytest.mark.parametrize("m", [1, 2])
+@pytest.mark.parametrize("n,k", [(1, 4096), (4736, 1000), (4737, 515), (9472, 131), (9475, 1001), (20001, 272), (600, 20480)])
+def test_one_and_two_tokens(n, k, m):
+    """Every number of channels per warp, with channels left over, aligned and odd rows."""
+    import hilberta_b200 as hb
+
+    x, w = _rows(m, k, FP16, seed=k), hb.quantize_rows(_rows(n, k, FP16, seed=n % 97, spread=0.0) * 0.05)
+    bias, rows = _rows(1, n, FP16, seed=4)[0], hb.quantize_rows(x)
+    got = hb.int8_linear(x, w, bias)
+    _check_product(got, rows.values, rows.scales, w.values, w.scales, bias, False)
+    assert torch.equal(got, hb.int8_linear(rows, w, bias))
+    many = hb.int8_linear(torch.cat([x, x, x]), w, bias)  # the tensor-core kernels
+    assert torch.equal(many[:m], got)
