@@ -117,7 +117,7 @@ struct Int8Problem {
     int64_t out_rs;
     int M, N, K, act, dtype;
 };
-bool int8_few_takes(int M, int K);  // int8_few.cu: tokens it serves
+bool int8_few_takes(int M, int64_t N, int K);  // int8_few.cu: products it serves
 int launch_int8_few(const Int8Problem& p, const DeviceInfo& di, cudaStream_t st);
 // int8_gemm.cu; early_weights: the weights are not written by the kernel before this
 // launch, so they may be fetched before it has ended.

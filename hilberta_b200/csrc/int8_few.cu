@@ -1,4 +1,4 @@
-// 8-bit products of one or two tokens: every weight is read once, and the bytes of
+// 8-bit products of one to four tokens: every weight is read once, and the bytes of
 // the weights bound it.  A warp forms R output channels at a time, each lane 16
 // bytes of every channel's row, with 4-way 8-bit dot products; the tokens' codes lie
 // in shared memory, quantised there from 16 bits by each CTA (they are a few KB; the
@@ -7,7 +7,8 @@
 // DRAM, 2.5 us of it the launch and the token, with four CTAs per SM (all 576 at once),
 // 14.3 us with three; two tokens 12.7 us, 16.0 us with two CTAs per SM.  Rings of
 // asynchronous copies per warp, 192 KB on their way per SM, took 11.6 us for one token
-// and 0.5 us more for small products.
+// and 0.5 us more for small products.  Three and four tokens: while the weights are few
+// (int8_few_takes), past that the dot products weigh more than the weights' bytes.
 #include <climits>
 
 #include "int8_common.cuh"
@@ -16,9 +17,9 @@ namespace hb {
 namespace {
 
 constexpr unsigned FULL = 0xffffffffu;
-constexpr int kRows = 2;
+constexpr int kRows = 4;
 constexpr int kSmem = 40 * 1024;  // codes of the tokens, at most
-constexpr int kResident = 4;      // CTAs per SM
+constexpr int resident(int tokens) { return tokens <= 2 ? 4 : 3; }  // CTAs per SM
 
 // 16 bytes of a row of codes, of which `left` (at least 1) are inside it.
 __device__ __forceinline__ int4 load_codes(const int8_t* p, int left) {
@@ -29,7 +30,7 @@ __device__ __forceinline__ int4 load_codes(const int8_t* p, int left) {
 }
 
 template <bool BF16, bool CODES, int M, int R>
-__global__ void __launch_bounds__(256, kResident) k_int8_few(const __grid_constant__ Int8Problem p) {
+__global__ void __launch_bounds__(256, resident(M)) k_int8_few(const __grid_constant__ Int8Problem p) {
     extern __shared__ __align__(16) int8_t s_codes[];  // [M][pitch]
     __shared__ uint32_t s_mag[M][8];
     __shared__ float s_scale[M];
@@ -147,22 +148,35 @@ int launch(const Int8Problem& p, cudaStream_t st) {
     return HB_OK;
 }
 
-template <bool BF16, bool CODES>
+template <bool BF16, bool CODES, int M>
 int launch(const Int8Problem& p, int sms, cudaStream_t st) {
     // Channels per warp: the fewest of 1, 2 and 4 for which all CTAs run at once, since
     // each begins with the tokens' codes; and 4 past that.  One token: 8192 x 8192 14.5 us
     // with 2, 16.8 with 4, 17.5 with 1; 9216 x 3072 7.4 with 2, 8.3 with 4, 9.7 with 1; 4096
     // x 14336 15.0 with 1, 20.9 with 4; 12288 x 3072 9.4 with 4, 10.8 with 2.
-    const int64_t warps = 8LL * sms * kResident;
-    const int r = p.N <= warps ? 1 : p.N <= 2 * warps ? 2 : 4;
-    if (p.M == 1)
-        return r == 1 ? launch<BF16, CODES, 1, 1>(p, st) : r == 2 ? launch<BF16, CODES, 1, 2>(p, st) : launch<BF16, CODES, 1, 4>(p, st);
-    return r == 1 ? launch<BF16, CODES, 2, 1>(p, st) : r == 2 ? launch<BF16, CODES, 2, 2>(p, st) : launch<BF16, CODES, 2, 4>(p, st);
+    const int64_t warps = 8LL * sms * resident(M);
+    if (p.N <= warps) return launch<BF16, CODES, M, 1>(p, st);
+    return p.N <= 2 * warps ? launch<BF16, CODES, M, 2>(p, st) : launch<BF16, CODES, M, 4>(p, st);
+}
+template <bool BF16, bool CODES>
+int launch(const Int8Problem& p, int sms, cudaStream_t st) {
+    switch (p.M) {
+        case 1: return launch<BF16, CODES, 1>(p, sms, st);
+        case 2: return launch<BF16, CODES, 2>(p, sms, st);
+        case 3: return launch<BF16, CODES, 3>(p, sms, st);
+        default: return launch<BF16, CODES, 4>(p, sms, st);
+    }
 }
 
 }  // namespace
 
-bool int8_few_takes(int M, int K) { return M <= kRows && code_pitch(K) * M <= kSmem; }
+// From 16 bits, against the quantisation and the tensor cores: 3 x 4096, K 4096 8.3 us
+// and 9.8, 3 x 9216, K 3072 9.8 and 11.9, 4 x 2048, K 2048 5.4 and 6.8; 4 x 5120, K 5120
+// 13.5 and 12.6, 3 x 3000, K 12288 16.4 and 14.1, 4 x 18432, K 3072 20.2 and 14.4.
+bool int8_few_takes(int M, int64_t N, int K) {
+    if (M > kRows || code_pitch(K) * M > kSmem) return false;
+    return M <= 2 || M * N * K <= 96000000;
+}
 
 int launch_int8_few(const Int8Problem& p, const DeviceInfo& di, cudaStream_t st) {
     if (p.x_scales) return p.dtype == 1 ? launch<true, true>(p, di.sms, st) : launch<false, true>(p, di.sms, st);

@@ -272,11 +272,11 @@ extern "C" int hb_int8_linear(const int8_t* x, int64_t x_rs, const float* x_scal
     if (!aligned(x, 16) || (M > 1 && x_rs % 16) || !aligned(x_scales, 4)) return HB_ERR_ALIGN;
     const Int8Problem p{x, x_rs, x_scales, w, w_rs, w_scales, static_cast<const uint16_t*>(bias), static_cast<uint16_t*>(out),
                         out_rs, M, N, K, act, dtype};
-    return linear(p, int8_few_takes(M, K), false, static_cast<cudaStream_t>(stream));
+    return linear(p, int8_few_takes(M, N, K), false, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" size_t hb_int8_linear16_workspace_bytes(int M, int K) {
-    if (M <= 0 || K <= 0 || K > HB_INT8_MAX_K || int8_few_takes(M, K)) return 0;
+    if (M <= 0 || K <= 0 || K > HB_INT8_MAX_K || int8_few_takes(M, INT32_MAX, K)) return 0;
     return (size_t)(code_pitch(K) * M + 4 * (int64_t)M);
 }
 
@@ -286,7 +286,7 @@ extern "C" int hb_int8_linear16(const void* x, int64_t x_rs, const int8_t* w, in
     int rc = check_linear(x, w, w_rs, w_scales, bias, out, out_rs, M, N, K, act, dtype);
     if (rc) return rc > 0 ? HB_OK : rc;
     if (!aligned(x, 2)) return HB_ERR_ALIGN;
-    const size_t need = hb_int8_linear16_workspace_bytes(M, K);
+    const size_t need = int8_few_takes(M, N, K) ? 0 : hb_int8_linear16_workspace_bytes(M, K);
     if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16))) return HB_ERR_WORKSPACE;
     Int8Problem p{x, x_rs, nullptr, w, w_rs, w_scales, static_cast<const uint16_t*>(bias), static_cast<uint16_t*>(out),
                   out_rs, M, N, K, act, dtype};

@@ -572,3 +572,22 @@ def test_one_and_two_tokens(n, k, m):
     assert torch.equal(got, hb.int8_linear(rows, w, bias))
     many = hb.int8_linear(torch.cat([x, x, x]), w, bias)  # the tensor-core kernels
     assert torch.equal(many[:m], got)
+
+
+@pytest.mark.parametrize("m", [3, 4])
+@pytest.mark.parametrize("n,k", [(1, 515), (3551, 1001), (3553, 272), (7104, 1000), (7107, 3080), (9000, 131), (20001, 2056), (60, 10240),
+                                 (60, 20480)])
+def test_three_and_four_tokens(n, k, m):
+    """On both sides of the sizes at which the tensor cores take over; every number of
+    channels per warp."""
+    import hilberta_b200 as hb
+
+    x, w = _rows(m, k, BF16, seed=k), hb.quantize_rows(_rows(n, k, BF16, seed=n % 97, spread=0.0) * 0.05)
+    bias, rows = _rows(1, n, BF16, seed=4)[0], hb.quantize_rows(x)
+    got = hb.int8_linear(x, w, bias, activation="gelu_tanh")
+    _check_product(got, rows.values, rows.scales, w.values, w.scales, bias, True)
+    assert torch.equal(got, hb.int8_linear(rows, w, bias, activation="gelu_tanh"))
+    assert torch.equal(hb.int8_linear(torch.cat([x, x]), w, bias)[:m], hb.int8_linear(x, w, bias))
+    wide = torch.full((m, n + 5), 7.0, dtype=BF16, device="cuda")
+    hb.int8_linear(x, w, bias, activation="gelu_tanh", out=wide[:, 2 : n + 2])
+    assert torch.equal(wide[:, 2 : n + 2], got) and bool((wide[:, :2] == 7).all()) and bool((wide[:, n + 2 :] == 7).all())
