@@ -66,6 +66,7 @@ EXPORTS = (
     "hb_int8_linear16_workspace_bytes",
     "hb_int8_linear16",
     "hb_int8_status",
+    "hb_int8_set_wait_limit",
     "hb_adaln_residual_int8",
     "hb_norm_rope_qk",
 )
@@ -152,6 +153,7 @@ _SIGS = {
     "hb_int8_linear16_workspace_bytes": (ctypes.c_size_t, [_I, _I]),
     "hb_int8_linear16": (_I, [_P, _I64, _P, _I64, _P, _P, _P, _I64, _I, _I, _I, _I, _I, _P, ctypes.c_size_t, _P]),
     "hb_int8_status": (_I, [_I, ctypes.POINTER(ctypes.c_int32), _P]),
+    "hb_int8_set_wait_limit": (_I, [_I]),
     "hb_adaln_residual_int8": (
         _I,
         [_P, _I64, _P, _I64, _P, _P, _P, _I64, _P, _I64, _P, _I64, _P, _I, _I, _I, ctypes.c_float, _I, _P],

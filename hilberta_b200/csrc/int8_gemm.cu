@@ -4,6 +4,7 @@
 // dependents of the kernel before them: they set themselves up while it ends, and wait
 // for its end before they read its results.
 #include <algorithm>
+#include <atomic>
 #include <climits>
 #include <mutex>
 
@@ -33,8 +34,17 @@ struct GemmParams {
     int tile0, tiles;  // pair kernel: of these tiles [tile0, tiles)
     int turn;          // pair kernel: 1 or 2 of two launches that share the tiles, else 0
     int early_weights;  // the first weights are fetched before grid_wait
-    long long timeout;
+    // Cycles that a barrier wait may take (0: the products give up half-way), and that
+    // copies and products under way may take to end after a wait ran out.
+    long long timeout, drain;
 };
+
+// Until what arrives on `bar` has ended, whoever has given up.
+__device__ __forceinline__ void bar_drain(uint64_t* bar, uint32_t parity, long long limit) {
+    const long long t0 = clock64();
+    while (!mbar_try_wait_cluster(bar, parity) && clock64() - t0 <= limit) {
+    }
+}
 
 // Up to 128 tokens x 128 channels per CTA, the weights as the product's first
 // operand: its 128 rows are then always full, the tokens' side is as narrow as there
@@ -53,9 +63,10 @@ struct TileCfg {
     static constexpr int HALF = BT / 2;                // tokens per warp in the epilogue: two warps share a channel
     static constexpr int TMEM_COLS = BT < 64 ? 64 : BT;  // loads of 32 columns from the second half on stay inside
     struct Ctl {
-        uint64_t full[STAGES_ALONE], empty[STAGES_ALONE], done;
+        uint64_t full[STAGES_ALONE], empty[STAGES_ALONE], done, drained;
         uint32_t tmem_base;
-        int abort;
+        int abort;   // a wait of this CTA ran out
+        int failed;  // a CTA of the cluster has no sums to give
         float scales[BT + 8];  // of the tokens, read eight at a time
     };
     static constexpr int smem(int stages) { return stages * STAGE + (int)((sizeof(Ctl) + 15) / 16 * 16); }
@@ -88,7 +99,8 @@ __global__ void __launch_bounds__(256, 2) k_int8_tile(const __grid_constant__ Ge
             mbar_init(&ctl->empty[i], 1);
         }
         mbar_init(&ctl->done, 1);
-        ctl->abort = 0;
+        mbar_init(&ctl->drained, 1);
+        ctl->abort = ctl->failed = 0;
         fence_barrier_init();
         if (p.early_weights) {
             for (int s = 0; s < min(stages, kb1 - kb0); s++) {
@@ -112,14 +124,11 @@ __global__ void __launch_bounds__(256, 2) k_int8_tile(const __grid_constant__ Ge
     tc_fence_after();
     const uint32_t tmem = ctl->tmem_base;
 
+    int issued = 0;  // stages filled by the first thread
     if (warp == 0 && lane == 0) {
-        bool ok = true;
-        int s = 0, round = 0, it = 0;
-        for (int kb = kb0; kb < kb1; kb++, it++) {
-            if (round > 0 && !mbar_wait(&ctl->empty[s], (round - 1) & 1, abort_flag, p.timeout)) {
-                ok = false;
-                break;
-            }
+        int s = 0, round = 0;
+        for (int kb = kb0; kb < kb1; kb++, issued++) {
+            if (round > 0 && !mbar_wait(&ctl->empty[s], (round - 1) & 1, abort_flag, p.timeout)) break;
             uint8_t* st = smem + s * C::STAGE;
             if (round > 0 || !p.early_weights) {
                 mbar_arrive_expect_tx(&ctl->full[s], C::STAGE);
@@ -128,16 +137,13 @@ __global__ void __launch_bounds__(256, 2) k_int8_tile(const __grid_constant__ Ge
             tma_load_2d(st + C::W_BYTES, &p.tmap_x, &ctl->full[s], kb * C::BK, m0);
             if (++s == stages) s = 0, round++;
         }
-        if (!ok) {  // let the copies in flight land before the CTA gives up its memory
-            volatile int ignore = 0;
-            for (int j = max(0, it - stages); j < it; j++)
-                mbar_wait(&ctl->full[j % stages], (j / stages) & 1, &ignore, p.timeout);
-        }
     } else if (warp == 1 && lane == 0) {
         constexpr uint32_t idesc = idesc_i8(C::BC, BT);
-        bool ok = true;
+        const int end = p.timeout > 0 ? kb1 : (kb0 + kb1) / 2;
+        bool ok = end == kb1;
+        if (!ok) *abort_flag = 1;
         int s = 0, round = 0;
-        for (int kb = kb0; kb < kb1; kb++) {
+        for (int kb = kb0; kb < end; kb++) {
             if (!mbar_wait(&ctl->full[s], round & 1, abort_flag, p.timeout)) {
                 ok = false;
                 break;
@@ -153,8 +159,18 @@ __global__ void __launch_bounds__(256, 2) k_int8_tile(const __grid_constant__ Ge
         if (ok) tc_commit(&ctl->done);
     }
     __syncwarp();
+    // done: every product has been formed, so every copy has landed.
     bool ok = __all_sync(FULL, mbar_wait(&ctl->done, 0, abort_flag, p.timeout));
-    if (!ok && lane == 0) atomicOr(&g_int8_status, HB_DEV_TIMEOUT);
+    if (!ok) {  // whichever wait ran out: nothing may be under way when the CTA gives up its memory
+        if (lane == 0) atomicOr(&g_int8_status, HB_DEV_TIMEOUT);
+        if (threadIdx.x == 0) {
+            for (int j = max(0, issued - stages); j < issued; j++) bar_drain(&ctl->full[j % stages], (j / stages) & 1, p.drain);
+        } else if (threadIdx.x == 32) {
+            tc_commit(&ctl->drained);
+            bar_drain(&ctl->drained, 0, p.drain);
+        }
+        __syncwarp();
+    }
     // Finishes U tokens from j on: straight-line code, so that their latencies overlap.
     auto finish_tokens = [&](int j, int end, const int (&acc)[U]) {
         float y[U];
@@ -204,6 +220,7 @@ __global__ void __launch_bounds__(256, 2) k_int8_tile(const __grid_constant__ Ge
     const uint32_t mine = smem_u32(part + rank * share * C::PITCH + channel);
     ok = __syncthreads_and(ok);
     cluster_sync();  // every CTA arrives at both barriers, whatever happened before
+    if (!ok && threadIdx.x < split) st_cluster_s32(cluster_map(smem_u32(&ctl->failed), threadIdx.x), 1);
     if (ok) {
         tc_fence_after();
 #pragma unroll
@@ -225,7 +242,7 @@ __global__ void __launch_bounds__(256, 2) k_int8_tile(const __grid_constant__ Ge
         tc_fence_after();
         tmem_dealloc(tmem, C::TMEM_COLS);
     }
-    if (!ok) return;
+    if (*static_cast<volatile int*>(&ctl->failed)) return;  // a share of the sums is missing
     for (int j = U * (warp >> 2); j < share && rank * share + j < tokens; j += 2 * U) {
         int acc[U] = {};
         for (int q = 0; q < split; q++) {
@@ -251,9 +268,11 @@ struct PairCfg {
     static constexpr int STAGING = 32 * 128;    // per warp: 32 rows x 64 columns of the output
     static constexpr int THREADS = 128 + 32 * EPI_WARPS;
     struct Ctl {
-        uint64_t full[STAGES], empty[STAGES], acc_full[2], acc_empty[2];
+        uint64_t full[STAGES], empty[STAGES], acc_full[2], acc_empty[2], drained;
         uint32_t tmem_base;
-        int abort;
+        int abort;      // a wait of this CTA ran out
+        int failed;     // some CTA of the cluster did not see all of its sums
+        int issued[2];  // in the pair's first CTA: stages that each of the two filled before it gave up
         alignas(16) float col_scale[BN];  // of the tile's columns
         alignas(16) float col_bias[BN];
     };
@@ -302,7 +321,9 @@ __global__ void __cluster_dims__(2 * SPLIT, 1, 1) __launch_bounds__(PairCfg::THR
             mbar_init(&ctl->acc_full[i], 1);
             mbar_init(&ctl->acc_empty[i], 2 * C::EPI_WARPS);
         }
-        ctl->abort = 0;
+        mbar_init(&ctl->drained, 1);
+        ctl->abort = ctl->failed = 0;
+        ctl->issued[0] = ctl->issued[1] = INT_MAX;
         fence_barrier_init();
         prefetch_tmap(&p.tmap_x);
         prefetch_tmap(&p.tmap_w);
@@ -354,23 +375,21 @@ __global__ void __cluster_dims__(2 * SPLIT, 1, 1) __launch_bounds__(PairCfg::THR
                     if (it >= early) tma_load_2d_pair(st + C::A_BYTES, &p.tmap_w, bar, k, n0 + 128 * rank);
                 }
             }
-            if (!ok) {  // gave up: time for the copies and MMAs in flight to end before the memory is given back
-                const long long t0 = clock64();
-                while (clock64() - t0 < p.timeout / 1000) {
-                }
-            }
+            if (!ok) st_cluster_s32(cluster_map(smem_u32(&ctl->issued[rank]), lead), it);
         }
     } else if (warp == 1) {
         if (lane == 0 && rank == 0) {
             constexpr uint32_t idesc = idesc_i8(C::BM, C::BN);
             if (p.turn != 2) grid_wait();  // the clock of the waits starts when the copies can
+            const int end = p.timeout > 0 ? nkb : nkb / 2;
+            if (end < nkb) *abort_flag = 1;
             int it = 0, i = 0;
             bool ok = true;
             for (int t = first; t < tiles && ok; t += step, i++) {
                 const uint32_t d = tmem + (i & 1) * C::BN;
                 if (i >= 2 && !mbar_wait_cluster(&ctl->acc_empty[i & 1], (i / 2 - 1) & 1, abort_flag, p.timeout)) break;
                 tc_fence_after();
-                for (int kb = 0; kb < nkb; kb++, it++) {
+                for (int kb = 0; kb < end; kb++, it++) {
                     const int s = it % C::STAGES;
                     if (!mbar_wait_cluster(&ctl->full[s], (it / C::STAGES) & 1, abort_flag, p.timeout)) {
                         ok = false;
@@ -383,6 +402,7 @@ __global__ void __cluster_dims__(2 * SPLIT, 1, 1) __launch_bounds__(PairCfg::THR
                         mma_i8_ss_pair(d, desc_sw128(a + k, 16, 1024), desc_sw128(b + k, 16, 1024), idesc, kb > 0 || k > 0);
                     tc_commit_pair(&ctl->empty[s], 3 << lead);
                 }
+                ok = ok && end == nkb;
                 if (ok) tc_commit_pair(&ctl->acc_full[i & 1], 3 << lead);
             }
         }
@@ -465,6 +485,7 @@ __global__ void __cluster_dims__(2 * SPLIT, 1, 1) __launch_bounds__(PairCfg::THR
             const bool ok = __all_sync(FULL, mbar_wait_cluster(&ctl->acc_full[i & 1], (i >> 1) & 1, abort_flag, p.timeout));
             if (!ok) {
                 if (lane == 0) atomicOr(&g_int8_status, HB_DEV_TIMEOUT);
+                if (lane < 2 * SPLIT) st_cluster_s32(cluster_map(smem_u32(&ctl->failed), lane), 1);
                 dead = true;
             }
             tc_fence_after();
@@ -496,6 +517,7 @@ __global__ void __cluster_dims__(2 * SPLIT, 1, 1) __launch_bounds__(PairCfg::THR
                 const uint32_t at = smem_u32(smem) + (ew * 16 * 32 + lane) * 16;
                 __syncwarp();
                 cluster_sync();
+                if (*static_cast<volatile int*>(&ctl->failed)) dead = true;  // sums will be missing
 #pragma unroll
                 for (int c = 0; c < 128; c += 64) {
                     const int owner = (2 * half + c / 64) & (SPLIT - 1);
@@ -536,6 +558,25 @@ __global__ void __cluster_dims__(2 * SPLIT, 1, 1) __launch_bounds__(PairCfg::THR
     }
     __syncthreads();
     cluster_sync();  // no CTA leaves while the other's MMAs read its memory or arrivals are on the way
+    if (*static_cast<volatile int*>(&ctl->failed)) {  // the same in all CTAs: copies and MMAs may be under way
+        if (rank == 0 && threadIdx.x == 0) {
+            // Both CTAs' copies arrive here, STAGE bytes each.  The two may have given up a
+            // few stages apart: what only one has filled is completed for the other.
+            const int all = (tiles - first + step - 1) / step * nkb;
+            const int mine = min(ctl->issued[0], all), other = min(ctl->issued[1], all), most = max(mine, other);
+            for (int j = max(0, most - C::STAGES); j < most; j++) {
+                uint64_t* bar = &ctl->full[j % C::STAGES];
+                if (j >= mine) mbar_arrive_expect_tx(bar, C::STAGE);
+                if (j >= other) mbar_complete_tx(bar, C::STAGE);
+                bar_drain(bar, (j / C::STAGES) & 1, p.drain);
+            }
+        } else if (rank == 0 && threadIdx.x == 32) {
+            tc_commit_pair(&ctl->drained, 1 << lead);
+            bar_drain(&ctl->drained, 0, p.drain);
+        }
+        __syncwarp();
+        cluster_sync();
+    }
     if (warp == 2) {
         tc_fence_after();
         tmem_dealloc_pair(tmem, 512);
@@ -574,6 +615,9 @@ int make_tmap_2d(CUtensorMap* map, CUtensorMapDataType type, int size, const voi
                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? HB_OK : HB_ERR_TMA;
 }
+
+constexpr int kWaitMs = 2000;
+std::atomic<int> g_wait_ms{kWaitMs};  // hb_int8_set_wait_limit
 
 std::mutex g_mu;
 unsigned g_configured[64];  // per device: kernels whose shared-memory limit is set
@@ -783,7 +827,8 @@ int launch_int8_gemm(const Int8Problem& q, int dev, const DeviceInfo& di, bool e
     p.tiles_n = (int)ceil_div(p.N, PairCfg::BN);
     p.tma_out = aligned(p.out, 16) && (p.M == 1 || p.out_rs % 8 == 0);
     p.early_weights = early_weights;
-    p.timeout = 2000LL * di.clock_khz;
+    p.timeout = (long long)g_wait_ms.load(std::memory_order_relaxed) * di.clock_khz;
+    p.drain = (long long)kWaitMs * di.clock_khz;
     Fit fit;
     if (const int rc = cluster_fit(dev, di.sms, &fit)) return rc;
     return q.dtype == 1 ? launch_gemm<true>(q, p, fit, dev, st) : launch_gemm<false>(q, p, fit, dev, st);
@@ -792,6 +837,12 @@ int launch_int8_gemm(const Int8Problem& q, int dev, const DeviceInfo& di, bool e
 }  // namespace hb
 
 using namespace hb;
+
+extern "C" int hb_int8_set_wait_limit(int milliseconds) {
+    if (milliseconds < 0) return HB_ERR_ARG;
+    g_wait_ms.store(milliseconds, std::memory_order_relaxed);
+    return HB_OK;
+}
 
 extern "C" int hb_int8_status(int clear, int32_t* bits, void* stream) {
     if (!bits) return HB_ERR_ARG;

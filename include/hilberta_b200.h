@@ -357,9 +357,15 @@ int hb_int8_linear16(const void* x, int64_t x_rs, const int8_t* w, int64_t w_rs,
                      int dtype, void* workspace, size_t workspace_bytes, void* stream);
 
 /* HB_DEV_* bits that hb_int8_linear and hb_int8_linear16 launches on the current device reported
- * (HB_DEV_TIMEOUT: a bounded wait ran out, some outputs were not written); with
- * clear, resets them.  Synchronises `stream`. */
+ * (HB_DEV_TIMEOUT: a bounded wait ran out, some outputs were not written, and those
+ * that were are right); with clear, resets them.  Synchronises `stream`. */
 int hb_int8_status(int clear, int32_t* bits, void* stream);
+
+/* Milliseconds that one barrier wait of those kernels may take (2000 at the start), for
+ * all launches of this process from now on; a captured launch keeps its own.  0: each
+ * launch gives up half-way through its first tiles, with copies and products under way,
+ * as after a wait that ran out (to see what that leaves behind). */
+int hb_int8_set_wait_limit(int milliseconds);
 
 /* hb_adaln_residual with h quantised as hb_quantize_rows does, from its fp32
  * values: codes [rows][C] (row stride codes_rs bytes, a multiple of 16), one scale

@@ -128,3 +128,10 @@ def test_row_strides():
     assert _row_stride(t[:, :5]) is None and _row_stride(t[::2]) is None
     assert _row_stride(t[:1, :5]) == 32 and _row_stride(t[:, :1]) == 192 and _row_stride(t.view(2, 2, 6, 32)) == 32
     assert _row_stride(t[:1, :1]) == 32 and _row_stride(t[:, ::2]) == 64
+
+
+def test_wait_limit_checks(lib):
+    from hilberta_b200 import _lib
+
+    assert lib.hb_int8_set_wait_limit(-1) == _lib.HB_ERR_ARG
+    assert lib.hb_int8_set_wait_limit(0) == _lib.HB_OK and lib.hb_int8_set_wait_limit(2000) == _lib.HB_OK
