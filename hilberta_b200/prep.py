@@ -199,9 +199,15 @@ def _interleaved(a, b):
     stride (as the query and key parts of one joined projection), sharing no element."""
     if a.ndim != 4 or b.ndim != 4 or a.stride()[:2] != b.stride()[:2]:
         return False
-    if a.shape[0] > 1 and a.stride(0) < a.shape[1] * a.stride(1):
+    entry, token = a.stride()[:2]
+    many = max(a.shape[0], b.shape[0]) > 1
+    if many and entry < max(a.shape[1], b.shape[1]) * token:
         return False
     width = lambda t: ((t.shape[2] - 1) * t.stride(2) + t.shape[3]) * t.element_size()  # noqa: E731
-    pitch = a.stride(1) * a.element_size()
-    shift = (b.data_ptr() - a.data_ptr()) % pitch if pitch else 0
-    return pitch > 0 and shift >= width(a) and shift + width(b) <= pitch
+    pitch = token * a.element_size()
+    apart = b.data_ptr() - a.data_ptr()
+    # Batch entries that are no whole number of tokens apart: only a row's own
+    # neighbourhood is known, not where it meets the rows of another entry.
+    if pitch <= 0 or many and entry % token and abs(apart) >= pitch:
+        return False
+    return apart % pitch >= width(a) and apart % pitch + width(b) <= pitch
