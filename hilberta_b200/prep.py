@@ -172,17 +172,26 @@ def norm_rope_qk(q, k, *, weight_q, weight_k, cos, sin, text_tokens=0, weight_tx
 
 
 def _check_qk_out(q, k, out, others):
-    """Outputs: like q and k, each either its input in place or apart from everything read."""
+    """Outputs: like q and k, each either its input in place or apart from everything read.
+    ``others`` are contiguous."""
     q_out, k_out = out
     for name, x, o in (("q", q, q_out), ("k", k, k_out)):
-        if o.shape != x.shape or o.dtype != x.dtype or o.device != x.device or o.stride(-1) != 1:
-            raise ValueError(f"the output of {name} must match its shape, dtype and device with contiguous D")
-        if torch.is_grad_enabled() and o.requires_grad:
-            raise ValueError("Inference output cannot require gradients")
+        if o is not x:
+            if o.shape != x.shape or o.dtype != x.dtype or o.device != x.device or o.stride(-1) != 1:
+                raise ValueError(f"the output of {name} must match its shape, dtype and device with contiguous D")
+            if torch.is_grad_enabled() and o.requires_grad:
+                raise ValueError("Inference output cannot require gradients")
         if _overlaps_itself(o):
             raise ValueError(f"the output of {name} must not overlap itself")
     same = [o.data_ptr() == x.data_ptr() and o.stride() == x.stride() for x, o in ((q, q_out), (k, k_out))]
     if all(same) and _interleaved(q, k):
+        begin, end = _rows_span(q)
+        first, last = _rows_span(k)
+        begin, end = min(begin, first), max(end, last)
+        for t in others:
+            first = t.data_ptr()
+            if first < end and (first >= begin or first + t.numel() * t.element_size() > begin):
+                raise ValueError("norm weights and cos/sin must not overlap the outputs")
         return
     for o, in_place, own in ((q_out, same[0], q), (k_out, same[1], k)):
         begin, end = _span(o)
@@ -192,6 +201,14 @@ def _check_qk_out(q, k, out, others):
             first, last = _span(t)
             if begin < last and first < end and not (t.dtype == o.dtype and _interleaved(o, t)):
                 raise ValueError("outputs must be their inputs in place or must not overlap any input")
+
+
+def _rows_span(t):
+    """``_span`` of a nonempty 16-bit [B, S, heads, D] with contiguous D."""
+    B, S, H, D = t.shape
+    entry, token, head, _ = t.stride()
+    first = t.data_ptr()
+    return first, first + 2 * ((B - 1) * entry + (S - 1) * token + (H - 1) * head + D)
 
 
 def _interleaved(a, b):

@@ -85,3 +85,19 @@ def test_apart_and_self_overlap_accept_nothing_shared():
         if not _overlaps_itself(a):
             assert len(set(_elements(a))) == a.numel()
     assert accepted > 1000
+
+
+def test_norms_and_rotation_inside_an_in_place_output_are_refused():
+    import pytest
+
+    from hilberta_b200.prep import _check_qk_out
+
+    joint = torch.zeros(1, 9, 3, 4, 64, dtype=torch.float16)
+    q, k, v = joint.unbind(2)
+    cos, sin, weight = torch.zeros(9, 64), torch.zeros(9, 64), torch.zeros(64, dtype=torch.float16)
+    _check_qk_out(q, k, (q, k), [cos, sin, weight, weight])
+    for bad in (q[0, 4, 1], k[0, 0, 0], q.view(torch.float32)[0, 1, 0]):  # rewritten while other rows read them
+        with pytest.raises(ValueError, match="must not overlap"):
+            _check_qk_out(q, k, (q, k), [cos, sin, bad, weight])
+        with pytest.raises(ValueError, match="must not overlap"):
+            _check_qk_out(q, k, (q, k), [cos, sin, weight, bad])
