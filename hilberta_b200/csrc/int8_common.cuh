@@ -71,13 +71,20 @@ __device__ __forceinline__ float rcp(float x) {
 __device__ __forceinline__ float gelu_tanh(float v) {
     return v * rcp(1.f + ptx::ex2(v * fmaf(kGelu1, v * v, kGelu0)));
 }
+// (sum * x_scale) * w_scale + bias.  A sum below 2^31 times the scale of bf16 rows near
+// their type's end (up to 2^121) would pass fp32's range although w_scale brings the
+// product back, so the kernels take 2^-24 x_scale and 2^24 w_scale: exact for
+// x_scale >= 2^-102 (smaller ones lose up to 5 of 24 bits) and w_scale < 2^104.
+__device__ __forceinline__ float x_factor(float scale) { return scale * 0x1p-24f; }
+__device__ __forceinline__ float w_factor(float scale) { return scale * 0x1p24f; }
+// sx, sw: the factors above.
 template <int ACT>
 __device__ __forceinline__ float finish(int acc, float sx, float sw, float b) {
     const float v = fmaf(__int2float_rn(acc) * sx, sw, b);
     return ACT ? gelu_tanh(v) : v;
 }
 // Two neighbouring columns at once, the same operations in packed fp32: sx the row's
-// scale twice, sw and b the columns' scales and biases; packed to 16 bits.
+// factor twice, sw and b the columns' factors and biases; packed to 16 bits.
 template <bool BF16, int ACT>
 __device__ __forceinline__ uint32_t finish2(int acc0, int acc1, uint64_t sx, uint64_t sw, uint64_t b) {
     using namespace ptx;

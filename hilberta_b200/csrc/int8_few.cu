@@ -52,7 +52,7 @@ __global__ void __launch_bounds__(256, resident(M)) k_int8_few(const __grid_cons
     const int mine = lane < R * M ? n0 + lane / M : INT_MAX;  // the channel this lane finishes
     float ws = 0.f, bias = 0.f;
     if (mine < p.N) {
-        ws = p.w_scales[mine];
+        ws = w_factor(p.w_scales[mine]);
         if (p.bias) bias = load16<BF16>(p.bias + mine);
     }
 
@@ -62,7 +62,7 @@ __global__ void __launch_bounds__(256, resident(M)) k_int8_few(const __grid_cons
             *reinterpret_cast<int4*>(s_codes + m * pitch + 16 * c) =
                 load_codes(static_cast<const int8_t*>(p.x) + m * p.x_rs + 16 * c, p.K - 16 * c);
         }
-        if (threadIdx.x < M) s_scale[threadIdx.x] = p.x_scales[threadIdx.x];
+        if (threadIdx.x < M) s_scale[threadIdx.x] = x_factor(p.x_scales[threadIdx.x]);
         __syncthreads();
     } else {
         const uint16_t* x = static_cast<const uint16_t*>(p.x);
@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(256, resident(M)) k_int8_few(const __grid_cons
 #pragma unroll
             for (int i = 1; i < 8; i++) g = __vmaxu2(g, s_mag[m][i]);
             const RowScale s = row_scale(mag_value<BF16>(g));
-            if (threadIdx.x == 0) s_scale[m] = s.scale;
+            if (threadIdx.x == 0) s_scale[m] = x_factor(s.scale);
             for (int c = 8 * threadIdx.x; c < pitch; c += 8 * 256) {
                 const uint4 v = load8(m, c);
                 *reinterpret_cast<uint2*>(s_codes + m * pitch + c) = codes8<BF16>(v, s);

@@ -67,7 +67,7 @@ struct TileCfg {
         uint32_t tmem_base;
         int abort;   // a wait of this CTA ran out
         int failed;  // a CTA of the cluster has no sums to give
-        float scales[BT + 8];  // of the tokens, read eight at a time
+        float scales[BT + 8];  // factors of the tokens, read eight at a time
     };
     static constexpr int smem(int stages) { return stages * STAGE + (int)((sizeof(Ctl) + 15) / 16 * 16); }
     static_assert((BT + 8) * PITCH * 4 <= STAGES * STAGE, "partial sums reuse the stages");
@@ -118,8 +118,8 @@ __global__ void __launch_bounds__(256, 2) k_int8_tile(const __grid_constant__ Ge
     grid_wait();
     const int channel = threadIdx.x & 127, n = n0 + channel;  // this thread's channel
     const int t0 = (warp >> 2) * C::HALF;                     // and the first of its tokens
-    const float sw = n < p.N ? p.w_scales[n] : 0.f, bias = n < p.N && p.bias ? load16<BF16>(p.bias + n) : 0.f;
-    if (threadIdx.x < BT) ctl->scales[threadIdx.x] = m0 + (int)threadIdx.x < p.M ? p.x_scales[m0 + threadIdx.x] : 0.f;
+    const float sw = n < p.N ? w_factor(p.w_scales[n]) : 0.f, bias = n < p.N && p.bias ? load16<BF16>(p.bias + n) : 0.f;
+    if (threadIdx.x < BT) ctl->scales[threadIdx.x] = m0 + (int)threadIdx.x < p.M ? x_factor(p.x_scales[m0 + threadIdx.x]) : 0.f;
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = ctl->tmem_base;
@@ -273,7 +273,7 @@ struct PairCfg {
         int abort;      // a wait of this CTA ran out
         int failed;     // some CTA of the cluster did not see all of its sums
         int issued[2];  // in the pair's first CTA: stages that each of the two filled before it gave up
-        alignas(16) float col_scale[BN];  // of the tile's columns
+        alignas(16) float col_scale[BN];  // factors of the tile's columns
         alignas(16) float col_bias[BN];
     };
     static constexpr int STG_OFF = STAGES * STAGE;
@@ -421,7 +421,7 @@ __global__ void __cluster_dims__(2 * SPLIT, 1, 1) __launch_bounds__(PairCfg::THR
                 const int c = threadIdx.x & 127;
                 float scale = 0.f, bias = 0.f;
                 if (col0 + c < p.N) {
-                    scale = p.w_scales[col0 + c];
+                    scale = w_factor(p.w_scales[col0 + c]);
                     if (p.bias) bias = load16<BF16>(p.bias + col0 + c);
                 }
                 asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");
@@ -430,7 +430,7 @@ __global__ void __cluster_dims__(2 * SPLIT, 1, 1) __launch_bounds__(PairCfg::THR
                 asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");
             }
             if (dead) continue;
-            const float row_scale = row0 + lane < p.M ? p.x_scales[row0 + lane] : 0.f;
+            const float row_scale = row0 + lane < p.M ? x_factor(p.x_scales[row0 + lane]) : 0.f;
             const uint64_t sx = f2_pack(row_scale, row_scale);
             // 64 columns of the warp's 32 rows from column c of its half: finished, staged, stored.
             auto finish_columns = [&](int c, const uint32_t (&lo)[32], const uint32_t (&hi)[32]) {

@@ -2,7 +2,7 @@
 // a row, and the product of two such matrices with scales, bias and activation.
 //
 //   scale_m = max_k |x_mk| / 127            code_mk = rint(x_mk * (127 / max_k |x_mk|))
-//   y_mn = act((sum_k xcode_mk * wcode_nk) * (xscale_m * wscale_n) + bias_n)
+//   y_mn = act(((sum_k xcode_mk * wcode_nk) * xscale_m) * wscale_n + bias_n)
 //
 // The sum is exact in 32-bit integers (K <= 131072: 127^2 * K < 2^31), so the
 // order in which it is taken, and how K is split over CTAs, cannot change a

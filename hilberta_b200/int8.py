@@ -155,7 +155,9 @@ def int8_linear(x, weight, bias=None, *, activation=None, out=None):
     given): ``[..., N]`` in x's type with a contiguous last dimension; rows may be
     spaced (a slice of a wider buffer), a leading dimension whose rows are not
     equally spaced takes one launch per index.  Integer sums are exact, so equal
-    inputs give equal outputs whatever the number of tokens."""
+    inputs give equal outputs whatever the number of tokens.  Results are
+    ``(sum * x_scale) * weight_scale + bias`` in fp32, rounded once; weight scales must
+    be below 2^104 (weights below 2.5e33), tokens may reach their type's end."""
     if not isinstance(weight, Int8Rows) or weight.values.ndim != 2:
         raise TypeError("weight must be 2-D Int8Rows [N, K] (quantize_rows of a weight matrix)")
     coded = isinstance(x, Int8Rows)

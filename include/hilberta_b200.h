@@ -335,10 +335,13 @@ int hb_quantize_rows(const void* a, int64_t a_rs, int ka, const void* b, int64_t
                      int rows, int8_t* codes, int64_t codes_rs, float* scales, int dtype,
                      void* stream);
 
-/* out[m][n] = act(sum_k x[m][k] w[n][k] * (x_scales[m] * w_scales[n]) + bias[n]) for
+/* out[m][n] = act((sum_k x[m][k] w[n][k] * x_scales[m]) * w_scales[n] + bias[n]) for
  * x [M][K], w [N][K] in 8 bits.  bias: [N] in the output type or NULL; act 0 none,
  * 1 tanh-GELU; out: 16-bit rows (dtype) with element row stride out_rs >= N.  The sum
- * is exact; the rest is fp32, rounded once.  A NaN scale makes its outputs NaN.
+ * is exact; the rest is fp32, rounded once.  The first product does not overflow for any
+ * x_scales up to 2^121 (those of bf16 rows) where the second brings it back; w_scales must
+ * be below 2^104, and x_scales below 2^-102 keep 19 bits at least.  A NaN scale makes its
+ * outputs NaN.
  * Strides of a single row are not used; out, bias and scales need no alignment beyond
  * their elements'.  out must not overlap what is read.  M or N 0 is a no-op. */
 int hb_int8_linear(const int8_t* x, int64_t x_rs, const float* x_scales, const int8_t* w, int64_t w_rs,
