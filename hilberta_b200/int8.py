@@ -266,12 +266,23 @@ def _product(x, coded, weight, bias, act, out, kind, dev):
     _lib.check(rc, "hb_int8_linear")
 
 
+def _aligned_rows(values):
+    """[N, K] codes whose rows start on 16-byte boundaries: as they are, or a copy
+    (moving a tensor to another device lays its rows side by side)."""
+    N, K = values.shape
+    if N <= 1 or (values.stride(0) % 16 == 0 and (K == 1 or values.stride(1) == 1)):
+        return values
+    return values.new_empty(N, -(-K // 16) * 16)[:, :K].copy_(values)
+
+
 class Int8Linear(torch.nn.Module):
     """``torch.nn.Linear`` with 8-bit weights, quantised once from ``linear`` (a
     CUDA layer in float16 or bfloat16): y = int8_linear(x, weight, bias).
 
     ``forward`` takes 16-bit tensors or ``Int8Rows``.  ``weight`` is the layer's
-    ``Int8Rows``; its parts are the buffers ``values`` and ``scales``."""
+    ``Int8Rows``; its parts are the buffers ``values`` and ``scales``.  Casts of the
+    module change the 16-bit type that it stands in for and the bias, never codes and
+    scales; a cast to another type than those leaves the layer as it is."""
 
     def __init__(self, linear):
         super().__init__()
@@ -282,6 +293,37 @@ class Int8Linear(torch.nn.Module):
         self.register_buffer("values", rows.values)
         self.register_buffer("scales", rows.scales)
         self.register_buffer("bias", bias)
+
+    def _apply(self, fn, recurse=True):
+        values, scales, bias = self.values, self.scales, self.bias
+        super()._apply(fn, recurse)
+        device = self.scales.device
+        if self.scales.dtype in _DTYPES:  # a cast
+            self.dtype = self.scales.dtype
+        elif bias is not None and self.bias.dtype != self.dtype:
+            self.bias = bias.to(device)
+        if self.scales.dtype != torch.float32:
+            self.scales = scales.to(device)
+        self.values = _aligned_rows(self.values if self.values.dtype == torch.int8 else values.to(device))
+        return self
+
+    def _load_from_state_dict(self, *args):
+        super()._load_from_state_dict(*args)  # assign=True: the buffers are the file's own tensors
+        self.values, self.scales = _aligned_rows(self.values), self.scales.float()
+        if self.bias is not None and self.bias.dtype in _DTYPES:
+            self.dtype = self.bias.dtype
+
+    @property
+    def in_features(self):
+        return self.values.shape[1]
+
+    @property
+    def out_features(self):
+        return self.values.shape[0]
+
+    def extra_repr(self):
+        return (f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}, "
+                f"dtype={self.dtype}")
 
     @classmethod
     def joined(cls, linears):
