@@ -114,7 +114,9 @@ class Int8JointAttention(torch.nn.Module):
 
 def quantize_flux_model(model):
     """Rewrite ``model`` (a ``FluxTransformer`` on a CUDA device, not sharded) to 8-bit
-    weights and activations, in place and layer by layer; returns it."""
+    weights and activations, in place; returns it.  The 16-bit layers are given up when
+    all 8-bit ones exist (half as much memory again until then), so a call that fails
+    leaves the model as it was."""
     if not isinstance(model, FluxTransformer):
         raise TypeError("quantize_flux_model takes a flux_model.FluxTransformer; Int8Linear replaces single layers")
     if getattr(model, "int8", False):
@@ -125,17 +127,17 @@ def quantize_flux_model(model):
         raise ValueError("quantise the model outside persistent_flux_attention")
     if not model.x_embedder.weight.is_cuda:
         raise ValueError("quantize_flux_model needs the model on a CUDA device")
+    changes = []  # made when every layer exists: a failure on the way leaves the model as it was
     with torch.no_grad():
         for b in model.transformer_blocks:
-            b.mod_img, b.mod_txt = Int8Linear(b.mod_img), Int8Linear(b.mod_txt)
-            b.attn = Int8JointAttention(b.attn)
-            for ff in (b.ff_img, b.ff_txt):
-                ff[0], ff[1] = Int8Linear(ff[0]), Int8Linear(ff[1])
+            changes += [(b, "mod_img", Int8Linear(b.mod_img)), (b, "mod_txt", Int8Linear(b.mod_txt))]
+            changes.append((b, "attn", Int8JointAttention(b.attn)))
+            changes += [(ff, str(i), Int8Linear(ff[i])) for ff in (b.ff_img, b.ff_txt) for i in range(2)]
         for b in model.single_transformer_blocks:
-            b.mod = Int8Linear(b.mod)
-            b.attn = Int8JointAttention(b.attn)
-            b.proj_mlp = Int8Linear(b.proj_mlp)
-            b.proj_out = Int8JoinedLinear(b.proj_out)
+            changes += [(b, "mod", Int8Linear(b.mod)), (b, "attn", Int8JointAttention(b.attn))]
+            changes += [(b, "proj_mlp", Int8Linear(b.proj_mlp)), (b, "proj_out", Int8JoinedLinear(b.proj_out))]
+    for owner, name, layer in changes:
+        setattr(owner, name, layer)
     model.ops = Int8BlockOps()
     model.int8 = True
     return model.eval()
