@@ -127,6 +127,8 @@ def quantize_flux_model(model):
         raise ValueError("quantise the model outside persistent_flux_attention")
     if not model.x_embedder.weight.is_cuda:
         raise ValueError("quantize_flux_model needs the model on a CUDA device")
+    if type(model.ops) is not NativeBlockOps:
+        raise ValueError("the model's own block_ops would be replaced; 8-bit layers need those of this module")
     changes = []  # made when every layer exists: a failure on the way leaves the model as it was
     with torch.no_grad():
         for b in model.transformer_blocks:

@@ -55,3 +55,19 @@ def test_failure_part_of_the_way(made, monkeypatch):
     kinds = [m for name, m in model.named_modules() if ".ff_" in name or ".mod" in name or ".proj_" in name]
     assert not any(isinstance(m, torch.nn.Linear) for m in kinds)
     assert 1000 - _Stub.left == 2 * 10 + 2 * 4  # every projection once
+
+
+def test_own_block_operations_are_not_replaced(monkeypatch):
+    from hilberta_b200 import flux_int8
+    from hilberta_b200.block_ops import NativeBlockOps
+
+    class Own(NativeBlockOps):
+        pass
+
+    monkeypatch.setattr(flux_int8, "Int8Linear", _Stub)
+    _Stub.left = 1000
+    for ops in (Own(), object()):
+        model = _model(block_ops=ops)
+        with pytest.raises(ValueError, match="block_ops"):
+            flux_int8.quantize_flux_model(model)
+        assert model.ops is ops and isinstance(model.transformer_blocks[0].mod_img, torch.nn.Linear)
