@@ -21,6 +21,8 @@ The reference has no counterpart (its adapter reports "weights_modified: False")
 
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from .block_ops import NativeBlockOps, adaln_int8, gate_residual_adaln_int8
@@ -101,14 +103,23 @@ class Int8JointAttention(torch.nn.Module):
         width = self.to_qkv.values.shape[0]
         buf = torch.empty((B, T + n, width), dtype=hidden_states.dtype, device=hidden_states.device)
         self.to_qkv(hidden_states, out=buf[:, T:])
-        text = {}
+        text, norms = {}, [(self.norm_q, self.norm_k)]
         if T:
             self.add_qkv(encoder_hidden_states, out=buf[:, :T])
             text = dict(text_tokens=T, weight_txt_q=self.norm_added_q.weight, weight_txt_k=self.norm_added_k.weight)
+            norms.append((self.norm_added_q, self.norm_added_k))
         q, k, v = buf.view(B, T + n, 3, self.heads, width // 3 // self.heads).unbind(2)
         cos, sin = image_rotary_emb
-        norm_rope_qk(q, k, weight_q=self.norm_q.weight, weight_k=self.norm_k.weight, cos=cos, sin=sin,
-                     eps=float(self.norm_q.eps), out=(q, k), **text)
+        turn = functools.partial(norm_rope_qk, q, k, weight_q=self.norm_q.weight, weight_k=self.norm_k.weight, cos=cos, sin=sin,
+                                 **text)
+        eps = {float(norm.eps) for pair in norms for norm in pair}
+        if len(eps) == 1:
+            turn(eps=eps.pop(), out=(q, k))
+        else:  # a pass for each eps, of which every norm's rows are taken
+            turned = {e: turn(eps=e) for e in eps}
+            for rows, pair in zip((slice(T, None), slice(0, T)), norms):
+                for i, (x, norm) in enumerate(zip((q, k), pair)):
+                    x[:, rows] = turned[float(norm.eps)][i][:, rows]
         return q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2)
 
 
