@@ -591,3 +591,23 @@ def test_three_and_four_tokens(n, k, m):
     wide = torch.full((m, n + 5), 7.0, dtype=BF16, device="cuda")
     hb.int8_linear(x, w, bias, activation="gelu_tanh", out=wide[:, 2 : n + 2])
     assert torch.equal(wide[:, 2 : n + 2], got) and bool((wide[:, :2] == 7).all()) and bool((wide[:, n + 2 :] == 7).all())
+
+
+@pytest.mark.parametrize("m,k", [(1, 40960), (2, 20480), (3, 13648), (4, 10240), (2, 131072), (16, 131072), (60, 131072), (200, 131072),
+                                 (600, 131072), (1280, 131072)])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_int8_linear_largest_sums(m, k, sign):
+    """Every product 127 * 127 or its negative: sums up to 2114060288, just below 2^31, in
+    the dot-product kernel at its longest K and in the tensor-core kernels at theirs."""
+    import hilberta_b200 as hb
+
+    n = 144 if k * m < 10**8 else 4096
+    x = torch.full((m, k), 127 * sign, dtype=torch.int8, device="cuda")
+    w = torch.full((n, k), 127, dtype=torch.int8, device="cuda")
+    w[1::2] = -127
+    rows = hb.Int8Rows(x, torch.full((m,), 2.0**-16, device="cuda"), BF16)
+    weight = hb.Int8Rows(w, torch.ones(n, device="cuda"), BF16)
+    want = torch.full((m, n), 16129.0 * k * sign / 2**16, dtype=torch.float64, device="cuda")
+    want[:, 1::2] *= -1
+    assert torch.equal(hb.int8_linear(rows, weight), want.to(BF16))  # a power of two away from the exact sum
+    assert hb.device_status() == 0
