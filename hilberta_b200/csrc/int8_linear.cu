@@ -102,8 +102,8 @@ __device__ __forceinline__ void store8(const QuantParams& p, int64_t row, int t,
 
 // T threads per row (a warp of four, or the whole CTA), up to kQuantVec vectors of 8
 // values each: the row is read once and stays in registers between its maximum
-// and its codes.  Memory-bound (2 K bytes read, K written per row): CTAs are
-// persistent and each thread fetches its part of the next row before it works on
+// and its codes.  Memory-bound (2 K bytes read, K written per row): a CTA goes over
+// several rows, and each thread fetches its part of the next row before it works on
 // this one, so loads are in flight through the reduction and the stores.
 constexpr int kQuantVec = 4;
 
@@ -174,8 +174,10 @@ int launch_quantize(const QuantParams& p, int sms, cudaStream_t st) {
     // Threads per row: the fewest of these whose registers hold it (8192 x 2048: 8.7 us
     // with 64, 13.5 with 128; 16384 x 3072: 23.8 us with 96, 25.4 with 128; 8192 x 5120:
     // 20.6 us with 160, 21.9 with 192; 8192 x 14336: the same with 448 and 512; a number only
-    // known at run time costs a quarter more than any); persistent CTAs, as many as fill
-    // the SMs' 2048 threads.
+    // known at run time costs a quarter more than any).  CTAs: as many as fill the SMs' 2048
+    // threads, which is more than their registers let be resident (56 to 64 a thread for
+    // W = 8: about half, 80 to 97 for W = 1: a third or a quarter), so they come in that
+    // many rounds, and a dependent launch starts with the last of them.
     const int64_t warps = ceil_div(p.k, 8 * kQuantVec * 32);
     auto start = [&](auto kern, int cta, int rows) {
         kern<<<(unsigned)std::min<int64_t>(ceil_div(p.rows, rows), (int64_t)sms * (2048 / cta)), cta, 0, st>>>(p);

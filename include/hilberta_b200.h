@@ -329,8 +329,8 @@ int hb_adaln_residual(const void* x, int64_t x_rs, const void* y, int64_t y_rs, 
  * kb 0; element row strides a_rs, b_rs).  A row holding an infinity or NaN gets
  * codes 0 and scale NaN; a row whose magnitudes are all below 2^-100 codes 0 and
  * scale 0.  Bytes of a codes row past ka + kb are not written.  Any alignment of a
- * and b; 16-byte aligned rows with ka and kb
- * multiples of 8 are read in 16-byte vectors. */
+ * and b; they are read in vectors of 16, 8, 4 or 2 bytes, the widest on which every row
+ * and part starts. */
 int hb_quantize_rows(const void* a, int64_t a_rs, int ka, const void* b, int64_t b_rs, int kb,
                      int rows, int8_t* codes, int64_t codes_rs, float* scales, int dtype,
                      void* stream);
