@@ -212,19 +212,22 @@ def _rows_span(t):
 
 
 def _interleaved(a, b):
-    """a and b are slices of equally strided rows, side by side within the token
-    stride (as the query and key parts of one joined projection), sharing no element."""
+    """a and b are slices of equally strided rows, side by side within the token stride
+    (as the query and key parts of one joined projection) or the batch stride (as parts
+    of [B, 3, S, heads, D]), sharing no element."""
     if a.ndim != 4 or b.ndim != 4 or a.stride()[:2] != b.stride()[:2]:
         return False
     entry, token = a.stride()[:2]
-    many = max(a.shape[0], b.shape[0]) > 1
-    if many and entry < max(a.shape[1], b.shape[1]) * token:
-        return False
-    width = lambda t: ((t.shape[2] - 1) * t.stride(2) + t.shape[3]) * t.element_size()  # noqa: E731
-    pitch = token * a.element_size()
-    apart = b.data_ptr() - a.data_ptr()
+    many, tokens = max(a.shape[0], b.shape[0]) > 1, max(a.shape[1], b.shape[1])
+    width = lambda t: (t.shape[2] - 1) * t.stride(2) + t.shape[3]  # noqa: E731
+    wide, other = width(a), width(b)
+    apart = (b.data_ptr() - a.data_ptr()) // a.element_size()
     # Batch entries that are no whole number of tokens apart: only a row's own
     # neighbourhood is known, not where it meets the rows of another entry.
-    if pitch <= 0 or many and entry % token and abs(apart) >= pitch:
+    if token > 0 and (not many or entry >= tokens * token and (entry % token == 0 or abs(apart) < token)):
+        if apart % token >= wide and apart % token + other <= token:
+            return True
+    if not many or entry <= 0:
         return False
-    return apart % pitch >= width(a) and apart % pitch + width(b) <= pitch
+    wide, other = wide + (a.shape[1] - 1) * token, other + (b.shape[1] - 1) * token
+    return apart % entry >= wide and apart % entry + other <= entry

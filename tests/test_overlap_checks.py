@@ -101,3 +101,20 @@ def test_norms_and_rotation_inside_an_in_place_output_are_refused():
             _check_qk_out(q, k, (q, k), [cos, sin, bad, weight])
         with pytest.raises(ValueError, match="must not overlap"):
             _check_qk_out(q, k, (q, k), [cos, sin, weight, bad])
+
+
+def test_parts_that_follow_each_other_in_every_batch_entry():
+    """Queries and keys of [B, 3, S, H, D] or [B, 3, H, S, D] storage, in place."""
+    from hilberta_b200.prep import _check_qk_out, _interleaved
+
+    small = [torch.zeros(9, 32), torch.zeros(32, dtype=torch.float16)]
+    blocks = torch.zeros(3, 3, 9, 4, 32, dtype=torch.float16)
+    heads_first = torch.zeros(3, 3, 4, 9, 32, dtype=torch.float16).transpose(2, 3)
+    for joint in (blocks, heads_first):
+        q, k, v = joint.unbind(1)
+        assert _interleaved(q, k) and _interleaved(k, q) and _interleaved(v, q) and not _interleaved(q, q)
+        _check_qk_out(q, k, (q, k), small)
+        _check_qk_out(q[:, :4], k[:, :4], (v[:, :4], k[:, :4]), small)
+        assert not _interleaved(joint[:, 0, :6], joint[:, 0, 5:])
+    q, k, v = blocks.unbind(1)
+    _check_qk_out(q[:, :4], k[:, :4], (q[:, 4:8], v[:, :4]), small)
