@@ -175,15 +175,16 @@ def _check_qk_out(q, k, out, others):
     """Outputs: like q and k, each either its input in place or apart from everything read.
     ``others`` are contiguous."""
     q_out, k_out = out
+    in_place = q_out is q and k_out is k
     for name, x, o in (("q", q, q_out), ("k", k, k_out)):
-        if o is not x:
+        if not in_place:
             if o.shape != x.shape or o.dtype != x.dtype or o.device != x.device or o.stride(-1) != 1:
                 raise ValueError(f"the output of {name} must match its shape, dtype and device with contiguous D")
             if torch.is_grad_enabled() and o.requires_grad:
                 raise ValueError("Inference output cannot require gradients")
         if _overlaps_itself(o):
             raise ValueError(f"the output of {name} must not overlap itself")
-    same = [o.data_ptr() == x.data_ptr() and o.stride() == x.stride() for x, o in ((q, q_out), (k, k_out))]
+    same = [in_place or o.data_ptr() == x.data_ptr() and o.stride() == x.stride() for x, o in ((q, q_out), (k, k_out))]
     if all(same) and _interleaved(q, k):
         begin, end = _rows_span(q)
         first, last = _rows_span(k)
@@ -193,11 +194,9 @@ def _check_qk_out(q, k, out, others):
             if first < end and (first >= begin or first + t.numel() * t.element_size() > begin):
                 raise ValueError("norm weights and cos/sin must not overlap the outputs")
         return
-    for o, in_place, own in ((q_out, same[0], q), (k_out, same[1], k)):
+    for o, over, own, rest in ((q_out, same[0], q, (k, k_out)), (k_out, same[1], k, (q, q_out))):
         begin, end = _span(o)
-        for t in (q, k, *others, *(x for x in out if x is not o)):
-            if in_place and t is own:
-                continue
+        for t in (*rest, *others) if over else (own, *rest, *others):
             first, last = _span(t)
             if begin < last and first < end and not (t.dtype == o.dtype and _interleaved(o, t)):
                 raise ValueError("outputs must be their inputs in place or must not overlap any input")

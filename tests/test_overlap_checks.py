@@ -118,3 +118,19 @@ def test_parts_that_follow_each_other_in_every_batch_entry():
         assert not _interleaved(joint[:, 0, :6], joint[:, 0, 5:])
     q, k, v = blocks.unbind(1)
     _check_qk_out(q[:, :4], k[:, :4], (q[:, 4:8], v[:, :4]), small)
+
+
+def test_one_tensor_for_both_outputs_is_refused():
+    import pytest
+
+    from hilberta_b200.prep import _check_qk_out
+
+    small = [torch.zeros(9, 32), torch.zeros(32, dtype=torch.float16)]
+    q, k, out = (torch.zeros(2, 9, 4, 32, dtype=torch.float16) for _ in range(3))
+    for args in ((q, q, (q, q)), (q, k, (out, out)), (q, k, (q, q)), (q, k, (k, k)), (q, k, (k, q)), (q, q, (out, q)), (q, q, (q, out)),
+                 (q, q.view(q.shape), (q, q.view(q.shape)))):
+        with pytest.raises(ValueError, match="must not overlap"):
+            _check_qk_out(*args, small)
+    _check_qk_out(q, q, (out, k), small)
+    _check_qk_out(q, k, (q, out), small)
+    _check_qk_out(q, k, (out, k), small)
