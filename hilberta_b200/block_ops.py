@@ -111,7 +111,7 @@ def _call_int8(x, y, gate, shift, scale, x_out, eps):
     x3, x_rs, B, S = _rows(x, "x")
     C = x3.shape[2]
     if torch.is_grad_enabled() and (x.requires_grad or shift.requires_grad or scale.requires_grad
-                                    or (y is not None and (y.requires_grad or gate.requires_grad))):
+                                    or (y is not None and (y.requires_grad or gate.requires_grad or x_out.requires_grad))):
         raise ValueError("Inference only; disable autograd")
     mod_bs = None
     for m in (shift, scale) if gate is None else (shift, scale, gate):

@@ -611,3 +611,15 @@ def test_int8_linear_largest_sums(m, k, sign):
     want[:, 1::2] *= -1
     assert torch.equal(hb.int8_linear(rows, weight), want.to(BF16))  # a power of two away from the exact sum
     assert hb.device_status() == 0
+
+
+def test_modulation_refuses_a_new_stream_that_requires_gradients():
+    from hilberta_b200.block_ops import gate_residual_adaln_int8
+
+    x, y = (_rows(9, 256, BF16, seed=s).view(1, 9, 256) for s in (1, 2))
+    shift, scale, gate, *_ = _modulation(1, 256, BF16, seed=3)
+    out = torch.zeros_like(x, requires_grad=True)
+    with pytest.raises(ValueError, match="disable autograd"):
+        gate_residual_adaln_int8(x, y, gate, shift, scale, x_out=out)
+    with torch.no_grad():
+        assert gate_residual_adaln_int8(x, y, gate, shift, scale, x_out=out)[0] is out
