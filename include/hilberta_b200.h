@@ -367,7 +367,8 @@ int hb_int8_status(int clear, int32_t* bits, void* stream);
 /* Milliseconds that one barrier wait of those kernels may take (2000 at the start), for
  * all launches of this process from now on; a captured launch keeps its own.  0: each
  * launch gives up half-way through its first tiles, with copies and products under way,
- * as after a wait that ran out (to see what that leaves behind). */
+ * as after a wait that ran out (to see what that leaves behind); launches for a few
+ * tokens wait for nothing and are whole. */
 int hb_int8_set_wait_limit(int milliseconds);
 
 /* hb_adaln_residual with h quantised as hb_quantize_rows does, from its fp32
